@@ -302,6 +302,70 @@ int32_t pcb_cond_td_prob(pcb_circuit* c, pcb_workspace* ws, const int32_t* marke
 int32_t pcb_pairwise_mi(const uint8_t* data_dev, uint64_t num_rows, uint32_t num_vars, uint32_t num_cats,
                         float pseudocount, float* mi_dev, pcb_stream s);
 
+/* ---- categorical heads ----------------------------------------------------------------- */
+/* What stands between a network's categorical head and a circuit: scores of its logits, their gradient, soft
+ * evidence made of them, and a head whose weights are held in 4 bits.  No circuit is involved: like
+ * pcb_pairwise_mi these calls run on the current device.  They allocate nothing, do not synchronise, keep no state,
+ * and may be captured; calls that share no output may overlap.  The reference trains its teachers in PyTorch
+ * (src/models/) and has no counterpart.
+ * Logits are f32, bf16 or f16 with the category index fastest; strides are in elements. */
+enum { PCB_F32 = 0, PCB_BF16 = 1, PCB_F16 = 2 };
+
+/* For every row of x_dev [rows, cats], with s = x / temperature and logp = s - logsumexp(s):
+ *   logp_out_dev [rows]      logp of the row's token; tokens_dev [rows] is int32 or int64 (token_bytes 4 or 8, or
+ *                            tokens_dev NULL: no logp); a negative token means none: 0; one past the last category: NaN
+ *   entropy_dev [rows]       -sum exp(logp) logp
+ *   top_ids_dev [rows, top_k] (int64), top_logp_dev [rows, top_k]: the top_k <= 32 largest, in order, of equal ones the
+ *                            lowest index first, NaN before everything (top_k = 0: not written)
+ *   stats_dev [rows, 2]      the row's largest logit and the sum of exp(s - max s): what the gradient needs
+ * A row whose logits are all -inf has logp -inf everywhere, entropy 0 and gradient 0; NaN or +inf in a row makes its
+ * results NaN. */
+int32_t pcb_token_logprobs(const void* x_dev, int32_t dtype, uint64_t rows, uint32_t cats, uint64_t row_stride,
+                           float temperature, const void* tokens_dev, uint32_t token_bytes, uint32_t top_k,
+                           float* logp_out_dev, float* entropy_dev, float* stats_dev, int64_t* top_ids_dev,
+                           float* top_logp_dev, pcb_stream s);
+/* Gradient with respect to the logits: dx_dev [rows, cats] contiguous, in x's type (f32 sums, one rounding), from the
+ * gradients of logp (NULL: none; element r at r * g_logp_stride), of the entropy (likewise) and of the alternatives'
+ * log-probabilities [rows, top_k] (contiguous or NULL).  The other arguments as given to and filled by
+ * pcb_token_logprobs.  dx_dev may not overlap x_dev. */
+int32_t pcb_token_logprobs_backward(const void* x_dev, int32_t dtype, uint64_t rows, uint32_t cats, uint64_t row_stride,
+                                    float temperature, const void* tokens_dev, uint32_t token_bytes, uint32_t top_k,
+                                    const int64_t* top_ids_dev, const float* stats_dev, const float* entropy_dev,
+                                    const float* g_logp_dev, uint64_t g_logp_stride, const float* g_entropy_dev,
+                                    uint64_t g_entropy_stride, const float* g_top_dev, void* dx_dev, pcb_stream s);
+/* Soft evidence of logits x_dev [rows, vars, cats] (category fastest, the other two at their strides): the normalised
+ * log-weights logp, [rows, vars, cats] column-major in out_dev: what pcb_evidence.soft_dev takes.  A variable that is
+ * missing in a row (miss_dev, nonzero bytes at the two strides; may be NULL) gets 0 for every category.  stats_dev
+ * [rows, vars, 2] (may be NULL) as in pcb_token_logprobs. */
+int32_t pcb_soft_evidence(const void* x_dev, int32_t dtype, uint64_t rows, uint32_t vars, uint32_t cats,
+                          uint64_t row_stride, uint64_t var_stride, const uint8_t* miss_dev, uint64_t miss_row_stride,
+                          uint64_t miss_var_stride, float temperature, float* out_dev, float* stats_dev, pcb_stream s);
+/* Its gradient: dx_dev [rows, vars, cats] contiguous (category fastest) in x's type from g_dev, laid out as out_dev. */
+int32_t pcb_soft_evidence_backward(const void* x_dev, int32_t dtype, uint64_t rows, uint32_t vars, uint32_t cats,
+                                   uint64_t row_stride, uint64_t var_stride, const uint8_t* miss_dev,
+                                   uint64_t miss_row_stride, uint64_t miss_var_stride, float temperature,
+                                   const float* stats_dev, const float* g_dev, void* dx_dev, pcb_stream s);
+
+/* A head of `cats` x `features` weights in 4 bits: weight (n, k) = scale[n, k / group] * (code[n, k] - 8), codes 0..15,
+ * group 32, 64 or 128, scales bf16 or f16.  Codes come two a byte, [cats, (features + 1) / 2], the even column in the
+ * low half; scales [cats, ceil(features / group)]; both contiguous.
+ * pcb_head_quantize makes them of a weight matrix (contiguous, f32 / bf16 / f16): scale = max |w| / 7 rounded to
+ * scale_dtype, code = round(w / scale) + 8.  pcb_head_pack lays codes and scales out in the order in which
+ * pcb_head_logits reads them (packed_dev, as many bytes as pcb_head_packed_bytes says, 16-byte aligned); pcb_head_weight writes the
+ * weights that a packed head stands for, [cats, features] f32. */
+int32_t pcb_head_packed_bytes(uint32_t cats, uint32_t features, uint32_t group, uint64_t* bytes_out);
+int32_t pcb_head_quantize(const void* weight_dev, int32_t dtype, uint32_t cats, uint32_t features, uint32_t group,
+                          int32_t scale_dtype, uint8_t* codes_dev, void* scales_dev, pcb_stream s);
+int32_t pcb_head_pack(const uint8_t* codes_dev, const void* scales_dev, uint32_t cats, uint32_t features, uint32_t group,
+                      void* packed_dev, pcb_stream s);
+int32_t pcb_head_weight(const void* packed_dev, int32_t scale_dtype, uint32_t cats, uint32_t features, uint32_t group,
+                        float* weight_dev, pcb_stream s);
+/* y_dev [rows, cats] contiguous in y_dtype = x_dev [rows, features] (dtype, rows at x_row_stride) times the weights,
+ * plus bias_dev [cats] (f32, may be NULL).  Codes and features are multiplied exactly, summed in f32. */
+int32_t pcb_head_logits(const void* packed_dev, int32_t scale_dtype, uint32_t cats, uint32_t features, uint32_t group,
+                        const void* x_dev, int32_t dtype, uint64_t rows, uint64_t x_row_stride, const float* bias_dev,
+                        void* y_dev, int32_t y_dtype, pcb_stream s);
+
 /* ---- multi-GPU ---------------------------------------------------------------------- */
 /* One NCCL communicator per process; pcb_em_step then sums [edge_aggr | leaf flows | LL]
  * over ranks before the replicated update.  The reference has no counterpart (it runs one

@@ -76,6 +76,16 @@ SIGNATURES = {
     "pcb_sample_soft_rows": [_vp, _vp, _vp, _u32, _vp, _f32, _u32, _vp, _vp],
     "pcb_cond_td_prob": [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _vp, _vp],
     "pcb_pairwise_mi": [_vp, _u64, _u32, _u32, _f32, _vp, _vp],
+    "pcb_token_logprobs": [_vp, _i32, _u64, _u32, _u64, _f32, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp],
+    "pcb_token_logprobs_backward": [_vp, _i32, _u64, _u32, _u64, _f32, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _u64, _vp, _u64,
+                                    _vp, _vp, _vp],
+    "pcb_soft_evidence": [_vp, _i32, _u64, _u32, _u32, _u64, _u64, _vp, _u64, _u64, _f32, _vp, _vp, _vp],
+    "pcb_soft_evidence_backward": [_vp, _i32, _u64, _u32, _u32, _u64, _u64, _vp, _u64, _u64, _f32, _vp, _vp, _vp, _vp],
+    "pcb_head_packed_bytes": [_u32, _u32, _u32, C.POINTER(_u64)],
+    "pcb_head_quantize": [_vp, _i32, _u32, _u32, _u32, _i32, _vp, _vp, _vp],
+    "pcb_head_pack": [_vp, _vp, _u32, _u32, _u32, _vp, _vp],
+    "pcb_head_weight": [_vp, _i32, _u32, _u32, _u32, _vp, _vp],
+    "pcb_head_logits": [_vp, _i32, _u32, _u32, _u32, _vp, _i32, _u64, _u64, _vp, _vp, _i32, _vp],
     "pcb_comm_unique_id": [_vp],
     "pcb_comm_init": [_vp, _vp, _i32, _i32],
     "pcb_comm_destroy": [_vp],

@@ -18,6 +18,8 @@ forwards to libpcb200.so through the C ABI of include/pcb200.h:
   gumbel_sample (soft) / sample (hard Gumbel-max)                queries/sample.jl:349-383
   gumbel_sample_preallocation / gumbel_sample_with_prealloc      utils/cuda_preallocation.jl:150-203
 
+and, for the network on the other side of soft evidence, `token_logprobs`, `soft_evidence` and `QuantHead` (heads.py).
+
 torch is used for device buffers and streams only.
 """
 from __future__ import annotations
@@ -30,6 +32,7 @@ import torch
 
 from . import _lib
 from .circuit import FlatCircuit, PCNode, compile_circuit, compile_multihead
+from .heads import QuantHead, TokenLogprobs, soft_evidence, token_logprobs   # noqa: F401 (part of the public surface)
 
 ArrayLike = Union[np.ndarray, torch.Tensor]
 

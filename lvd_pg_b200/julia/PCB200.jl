@@ -479,6 +479,108 @@ function pairwise_MI(data::CuMatrix{UInt8}; num_cats = Int(maximum(data)) + 1, p
     mi
 end
 
+# ---- categorical heads: what a network's logits are scored with, and made into soft evidence ---------------
+logits_type(::Type{Float32}) = Int32(0)
+logits_type(::Type{Core.BFloat16}) = Int32(1)
+logits_type(::Type{Float16}) = Int32(2)
+ptr_or_null(x) = x === nothing ? CU_NULL : reinterpret(CuPtr{Cvoid}, pointer(x))
+
+"""
+token_logprobs(logits, tokens; top_k, temperature) — logits (cats, rows), tokens 0-based Int32 / Int64 (negative: none
+given); returns (logp, entropy, top_ids (top_k, rows) 0-based, top_logp, stats); `stats` is for token_logprobs_backward.
+"""
+function token_logprobs(logits::CuMatrix, tokens::Union{Nothing,CuVector{Int32},CuVector{Int64}} = nothing; top_k = 0, temperature = 1f0)
+    C, n = size(logits)
+    logp = CUDA.zeros(Float32, n); entropy = CUDA.zeros(Float32, n); stats = CUDA.zeros(Float32, 2, n)
+    ids = CUDA.zeros(Int64, top_k, n); top = CUDA.zeros(Float32, top_k, n)
+    check(ccall((:pcb_token_logprobs, libpcb200), Int32,
+                (CuPtr{Cvoid}, Int32, UInt64, UInt32, UInt64, Cfloat, CuPtr{Cvoid}, UInt32, UInt32, CuPtr{Cfloat}, CuPtr{Cfloat},
+                 CuPtr{Cfloat}, CuPtr{Int64}, CuPtr{Cfloat}, Ptr{Cvoid}),
+                ptr_or_null(logits), logits_type(eltype(logits)), n, C, C, temperature, ptr_or_null(tokens),
+                tokens === nothing ? 0 : sizeof(eltype(tokens)), top_k, logp, entropy, stats, ids, top, stream()))
+    (logp = logp, entropy = entropy, top_ids = ids, top_logp = top, stats = stats)
+end
+
+"gradient of the logits from those of `logp`, `entropy` and `top_logp` of `out = token_logprobs(logits, tokens; ...)` (nothing: none)"
+function token_logprobs_backward(logits::CuMatrix, tokens, out; g_logp = nothing, g_entropy = nothing, g_top = nothing, temperature = 1f0)
+    C, n = size(logits)
+    dx = similar(logits)
+    check(ccall((:pcb_token_logprobs_backward, libpcb200), Int32,
+                (CuPtr{Cvoid}, Int32, UInt64, UInt32, UInt64, Cfloat, CuPtr{Cvoid}, UInt32, UInt32, CuPtr{Int64}, CuPtr{Cfloat},
+                 CuPtr{Cfloat}, CuPtr{Cvoid}, UInt64, CuPtr{Cvoid}, UInt64, CuPtr{Cvoid}, CuPtr{Cvoid}, Ptr{Cvoid}),
+                ptr_or_null(logits), logits_type(eltype(logits)), n, C, C, temperature, ptr_or_null(tokens),
+                tokens === nothing ? 0 : sizeof(eltype(tokens)), size(out.top_ids, 1), out.top_ids, out.stats, out.entropy,
+                ptr_or_null(g_logp), 1, ptr_or_null(g_entropy), 1, ptr_or_null(g_top), ptr_or_null(dx), stream()))
+    dx
+end
+
+"""
+soft_evidence(logits; miss, temperature) — logits (cats, vars, rows) of a network as the (rows, vars, cats) log-weights that
+forward_ex and mini_batch_em take; `miss` (rows, vars) UInt8, nonzero = missing.  Returns (soft, stats).
+"""
+function soft_evidence(logits::CuArray{T,3}; miss = nothing, temperature = 1f0) where {T}
+    C, V, n = size(logits)
+    soft = CuArray{Float32}(undef, n, V, C); stats = CuArray{Float32}(undef, 2, V, n)
+    check(ccall((:pcb_soft_evidence, libpcb200), Int32,
+                (CuPtr{Cvoid}, Int32, UInt64, UInt32, UInt32, UInt64, UInt64, CuPtr{Cvoid}, UInt64, UInt64, Cfloat, CuPtr{Cfloat},
+                 CuPtr{Cfloat}, Ptr{Cvoid}),
+                ptr_or_null(logits), logits_type(T), n, V, C, C * V, C, ptr_or_null(miss), 1, n, temperature, soft, stats, stream()))
+    soft, stats
+end
+
+"gradient of the logits from that of the evidence, `g` (rows, vars, cats)"
+function soft_evidence_backward(logits::CuArray{T,3}, stats, g::CuArray{Float32,3}; miss = nothing, temperature = 1f0) where {T}
+    C, V, n = size(logits)
+    dx = similar(logits)
+    check(ccall((:pcb_soft_evidence_backward, libpcb200), Int32,
+                (CuPtr{Cvoid}, Int32, UInt64, UInt32, UInt32, UInt64, UInt64, CuPtr{Cvoid}, UInt64, UInt64, Cfloat, CuPtr{Cfloat},
+                 CuPtr{Cfloat}, CuPtr{Cvoid}, Ptr{Cvoid}),
+                ptr_or_null(logits), logits_type(T), n, V, C, C * V, C, ptr_or_null(miss), 1, n, temperature, stats, g, ptr_or_null(dx), stream()))
+    dx
+end
+
+"A head whose weights are held in 4 bits with group scales (pcb200.h); weight (features, cats)."
+struct QuantHead
+    packed::CuVector{UInt8}
+    bias::Union{Nothing,CuVector{Float32}}
+    cats::Int; features::Int; group::Int; scale_type::Int32
+end
+"codes (ceil(features / 2), cats) UInt8, two a byte; scales (ceil(features / group), cats) Float16 or BFloat16"
+function QuantHead(codes::CuMatrix{UInt8}, scales::CuMatrix, features::Integer; group = 64, bias = nothing)
+    cats = size(codes, 2)
+    bytes = Ref{UInt64}(0)
+    check(ccall((:pcb_head_packed_bytes, libpcb200), Int32, (UInt32, UInt32, UInt32, Ptr{UInt64}), cats, features, group, bytes))
+    packed = CuVector{UInt8}(undef, bytes[])
+    check(ccall((:pcb_head_pack, libpcb200), Int32, (CuPtr{UInt8}, CuPtr{Cvoid}, UInt32, UInt32, UInt32, CuPtr{UInt8}, Ptr{Cvoid}),
+                codes, ptr_or_null(scales), cats, features, group, packed, stream()))
+    QuantHead(packed, bias, cats, features, group, logits_type(eltype(scales)))
+end
+function QuantHead(weight::CuMatrix{T}; group = 64, bias = nothing) where {T}
+    K, N = size(weight)
+    S = T == Float16 ? Float16 : Core.BFloat16
+    codes = CuMatrix{UInt8}(undef, cld(K, 2), N); scales = CuMatrix{S}(undef, cld(K, group), N)
+    check(ccall((:pcb_head_quantize, libpcb200), Int32,
+                (CuPtr{Cvoid}, Int32, UInt32, UInt32, UInt32, Int32, CuPtr{UInt8}, CuPtr{Cvoid}, Ptr{Cvoid}),
+                ptr_or_null(weight), logits_type(T), N, K, group, logits_type(S), codes, ptr_or_null(scales), stream()))
+    QuantHead(codes, scales, K; group, bias)
+end
+"the weights that the codes stand for, (features, cats)"
+function head_weight(h::QuantHead)
+    w = CuMatrix{Float32}(undef, h.features, h.cats)
+    check(ccall((:pcb_head_weight, libpcb200), Int32, (CuPtr{UInt8}, Int32, UInt32, UInt32, UInt32, CuPtr{Cfloat}, Ptr{Cvoid}),
+                h.packed, h.scale_type, h.cats, h.features, h.group, w, stream()))
+    w
+end
+"logits (cats, rows) of features (features, rows)"
+function head_logits(h::QuantHead, x::CuMatrix; out_type = eltype(x))
+    y = CuMatrix{out_type}(undef, h.cats, size(x, 2))
+    check(ccall((:pcb_head_logits, libpcb200), Int32,
+                (CuPtr{UInt8}, Int32, UInt32, UInt32, UInt32, CuPtr{Cvoid}, Int32, UInt64, UInt64, CuPtr{Cvoid}, CuPtr{Cvoid}, Int32, Ptr{Cvoid}),
+                h.packed, h.scale_type, h.cats, h.features, h.group, ptr_or_null(x), logits_type(eltype(x)), size(x, 2), h.features,
+                ptr_or_null(h.bias), ptr_or_null(y), logits_type(out_type), stream()))
+    y
+end
+
 # ---- multi-head circuits (src-jl/multi_head_pc) ---------------------------------------------------------
 """
 CuMultiHeadBitsProbCircuit(pcs) — bit_circuit.jl:4-56: the heads under a fake root whose edges carry
