@@ -84,6 +84,51 @@ __device__ __forceinline__ void put(Stat& s, float x, float c) {
   s.A += e * d;
 }
 
+// 16-byte granules: VEC elements, in fp32 and back
+template <typename T> struct Vec { static constexpr uint32_t N = 16 / sizeof(T); };
+__device__ __forceinline__ uint4 load16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+template <typename T> __device__ __forceinline__ void unpack(uint4 v, float* f);
+template <> __device__ __forceinline__ void unpack<float>(uint4 v, float* f) {
+  f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+}
+template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(uint4 v, float* f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+template <> __device__ __forceinline__ void unpack<__half>(uint4 v, float* f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = p.x; f[2 * i + 1] = p.y;
+  }
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
 __device__ __forceinline__ int64_t token_at(const void* tokens, uint32_t bytes, uint64_t r) {
   return bytes == 8 ? static_cast<const int64_t*>(tokens)[r] : static_cast<const int32_t*>(tokens)[r];
 }
@@ -103,58 +148,523 @@ __device__ __forceinline__ float logp_of(float x, float m, float lnS, float invT
   return m == -INFINITY && !(lnS != lnS) ? -INFINITY : (x - m) * invT - lnS;
 }
 
-// the row's results but for the alternatives
+// ---- long rows: a block, or the blocks of a cluster, per row -------------------------------------------------------
+// One pass over the row.  A thread takes tiles of 128 (fp32) or 64 bytes, keeps a running (max, S, A) that is rescaled
+// once per tile whose maximum is new, and notes every tile's maximum in shared memory.
+//
+// Alternatives without a second pass: the k-th largest of the maxima of 32 groups of threads is a lower bound of the
+// k-th largest value (the groups hold different elements), so only tiles whose noted maximum reaches it are read
+// again: a few more than k of them.  What reaches the bound is collected and ordered by counting.  More than CAND of
+// those (rows of few different values, or large ones side by side in few groups) raise the bound to the k-th of what
+// was collected, as long as that helps; what is left then (mostly ties) goes by rounds over what lies above the bound and
+// one walk in index order over what equals it.
+constexpr uint32_t ROW_THREADS = 256, SLOTS = 16, CAND = 256, MAX_CLUSTER = 8;
+
+template <typename T> struct Tile { static constexpr uint32_t U = sizeof(T) == 4 ? 8 : 4; };   // granules per thread
+
+// The part of a row that a block reads: granules [g0, g1) counted from the 16-byte boundary at or below the row's start.
 template <typename T>
-__device__ void write_row(const LogprobArgs& a, uint64_t row, const T* x, Stat s) {
-  const float lnS = s.m == -INFINITY && s.S == 0.0f ? 0.0f : logf(s.S);
-  if (a.tokens) {
-    const int64_t t = token_at(a.tokens, a.token_bytes, row);
-    a.logp[row] = t < 0 ? 0.0f : t >= (int64_t)a.cats ? NAN : logp_of(to_f32(x[t]), s.m, lnS, a.invT);
+struct Part {
+  const T* base;        // that boundary
+  uint32_t off, end;    // the row's elements are base[off .. end)
+  uint32_t g0, g1, shift;
+  __device__ __forceinline__ bool whole(uint32_t g) const { return g * Vec<T>::N >= off && (g + 1) * Vec<T>::N <= end; }
+  // the granule's elements in fp32; -inf outside of the row
+  __device__ __forceinline__ void read(uint32_t g, float* f) const {
+    if (whole(g)) {
+      unpack<T>(load16(base + (size_t)g * Vec<T>::N), f);
+    } else {
+#pragma unroll
+      for (uint32_t v = 0; v < Vec<T>::N; ++v) {
+        const uint32_t j = g * Vec<T>::N + v;
+        f[v] = j >= off && j < end ? to_f32(base[j]) : -INFINITY;
+      }
+    }
   }
-  a.entropy[row] = s.m == -INFINITY && s.S == 0.0f ? 0.0f : lnS - LN2 * s.A / s.S;
-  a.stats[2 * row] = s.m;
-  a.stats[2 * row + 1] = s.S;
+  __device__ __forceinline__ bool inside(uint32_t g, uint32_t v) const {
+    const uint32_t j = g * Vec<T>::N + v;
+    return j >= off && j < end;
+  }
+  __device__ __forceinline__ uint32_t index(uint32_t g, uint32_t v) const { return g * Vec<T>::N + v - off; }
+};
+
+struct RowShared {
+  float slot[SLOTS][ROW_THREADS];
+  uint64_t cand[CAND];
+  uint64_t best[MAX_TOP];            // this block's alternatives, in order
+  uint64_t all[MAX_CLUSTER][MAX_TOP];   // first block of a cluster: every block's
+  Stat part[8], joined[MAX_CLUSTER];
+  float group[32];
+  uint64_t round[8];
+  uint32_t count, warp_count[8];
+};
+
+__device__ __forceinline__ float value_of(uint64_t key) {   // inverse of order_bits, but for NaN
+  const uint32_t u = (uint32_t)(key >> 32);
+  return u == 0xffffffffu ? NAN : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
-// One block per row: the statistics of the threads' values joined, then one pass per alternative.
+// lanes' statistics joined over `width` neighbouring lanes
+template <int width>
+__device__ __forceinline__ Stat lanes_join(Stat s, float c) {
+  float m = s.m;
+#pragma unroll
+  for (int o = width / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float d = s.m == -INFINITY ? 0.0f : max_nan((s.m - m) * c, NO_MASS), f = ex2_ftz(d);
+  s.A = f * (s.A + d * s.S);
+  s.S *= f;
+#pragma unroll
+  for (int o = width / 2; o; o >>= 1) {
+    s.S += __shfl_xor_sync(0xffffffffu, s.S, o);
+    s.A += __shfl_xor_sync(0xffffffffu, s.A, o);
+  }
+  s.m = m;
+  return s;
+}
+
+// f(granule) for the granules of the thread's tiles whose noted maximum passes `pick`
+template <typename T, typename P, typename F>
+__device__ __forceinline__ void picked_granules(const Part<T>& p, const RowShared& sh, P pick, F f) {
+  constexpr uint32_t U = Tile<T>::U, STEP = ROW_THREADS * U;
+  const uint32_t tiles = (p.g1 - p.g0 + STEP - 1) / STEP, slots = (tiles + (1u << p.shift) - 1) >> p.shift;
+  for (uint32_t s = 0; s < slots; ++s) {
+    if (!pick(sh.slot[s][threadIdx.x])) continue;
+    const uint32_t t1 = min(tiles, (s + 1) << p.shift);
+    for (uint32_t t = s << p.shift; t < t1; ++t)
+      for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t g = p.g0 + t * STEP + u * ROW_THREADS + threadIdx.x;
+        if (g < p.g1) f(g);
+      }
+  }
+}
+
+// The block's `top_k` largest, in order, into sh.best (0: there is no further one).  `mine`: the thread's largest value;
+// `wild`: the part holds NaN, which no noted maximum shows.
 template <typename T>
-__global__ void __launch_bounds__(256) logprob_row_kernel(LogprobArgs a) {
-  __shared__ Stat part[8];
-  __shared__ uint64_t best[8];
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T* x = static_cast<const T*>(a.x) + row * a.stride;
-    Stat s{-INFINITY, 0.0f, 0.0f};
-    for (uint32_t j = threadIdx.x; j < a.cats; j += blockDim.x) put(s, to_f32(x[j]), a.c);
-    s = warp_join(s, a.c);
-    if (lane == 0) part[warp] = s;
+__device__ void block_top(const Part<T>& p, RowShared& sh, uint32_t top_k, float mine, bool wild) {
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid < MAX_TOP) sh.best[tid] = 0;
+  float gm = mine;
+#pragma unroll
+  for (int o = 4; o; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+  if ((lane & 7) == 0) sh.group[warp * 4 + (lane >> 3)] = gm;
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  float bound;
+  {
+    const float v = sh.group[lane];
+    uint32_t above = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 32; ++j) {
+      const float w = sh.group[j];
+      above += w > v || (w == v && j < lane);
+    }
+    bound = __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, above == top_k - 1)) - 1);
+  }
+  bool raised = !wild;
+  for (uint32_t tries = 0; raised && tries < 8; ++tries) {
+    picked_granules<T>(p, sh, [&](float m) { return m >= bound; }, [&](uint32_t g) {
+      float f[Vec<T>::N];
+      p.read(g, f);
+#pragma unroll
+      for (uint32_t v = 0; v < Vec<T>::N; ++v)
+        if (f[v] >= bound && p.inside(g, v)) {
+          const uint32_t at = atomicAdd(&sh.count, 1u);
+          if (at < CAND) sh.cand[at] = order_key(f[v], p.index(g, v));
+        }
+    });
     __syncthreads();
-    s = part[0];
-    for (uint32_t w = 1; w < 8; ++w) s = join(s, part[w], a.c);
-    if (threadIdx.x == 0) write_row(a, row, x, s);
-    const float lnS = s.m == -INFINITY && s.S == 0.0f ? 0.0f : logf(s.S);
-    uint64_t last = ~0ull;
-    for (uint32_t k = 0; k < a.top_k; ++k) {
-      uint64_t key = 0;
-      for (uint32_t j = threadIdx.x; j < a.cats; j += blockDim.x) {
-        const uint64_t o = order_key(to_f32(x[j]), j);
-        if (o < last && o > key) key = o;
+    const uint32_t found = sh.count, n = min(found, CAND);
+    uint32_t above = 0;
+    const uint64_t key = tid < n ? sh.cand[tid] : 0;
+    for (uint32_t j = 0; j < n; ++j) above += sh.cand[j] > key;
+    if (tid < n && above < top_k) sh.best[above] = key;
+    __syncthreads();
+    if (found <= CAND) return;
+    const float better = value_of(sh.best[top_k - 1]);
+    raised = better > bound;
+    bound = raised ? better : bound;
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    if (tid < MAX_TOP) sh.best[tid] = 0;
+  }
+  // rounds over what lies above the bound (with NaN in the row: over everything)
+  uint32_t have = 0;
+  uint64_t last = ~0ull;
+  __syncthreads();
+  while (have < top_k) {
+    uint64_t key = 0;
+    picked_granules<T>(p, sh, [&](float m) { return wild || m > bound; }, [&](uint32_t g) {
+      float f[Vec<T>::N];
+      p.read(g, f);
+#pragma unroll
+      for (uint32_t v = 0; v < Vec<T>::N; ++v)
+        if ((wild || f[v] > bound) && p.inside(g, v)) {
+          const uint64_t k = order_key(f[v], p.index(g, v));
+          if (k < last && k > key) key = k;
+        }
+    });
+#pragma unroll
+    for (int o = 16; o; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+    if (lane == 0) sh.round[warp] = key;
+    __syncthreads();
+    for (uint32_t w = 0; w < 8; ++w) key = max(key, sh.round[w]);
+    __syncthreads();
+    if (key == 0) break;
+    if (tid == 0) sh.best[have] = key;
+    ++have;
+    last = key;
+  }
+  // what equals the bound, in index order
+  for (uint32_t g0 = p.g0; g0 < p.g1 && have < top_k && !wild; g0 += ROW_THREADS) {
+    const uint32_t g = g0 + tid;
+    float f[Vec<T>::N];
+    uint32_t hits = 0;
+    if (g < p.g1) {
+      p.read(g, f);
+#pragma unroll
+      for (uint32_t v = 0; v < Vec<T>::N; ++v) hits |= (uint32_t)(f[v] == bound && p.inside(g, v)) << v;
+    }
+    uint32_t before = __popc(hits);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= (uint32_t)o) before += x;
+    }
+    if (lane == 31) sh.warp_count[warp] = before;
+    before -= __popc(hits);
+    __syncthreads();
+    uint32_t total = 0;
+    for (uint32_t w = 0; w < 8; ++w) {
+      if (w < warp) before += sh.warp_count[w];
+      total += sh.warp_count[w];
+    }
+    for (uint32_t at = have + before; hits && at < top_k; hits &= hits - 1, ++at)
+      sh.best[at] = order_key(bound, p.index(g, __ffs(hits) - 1));
+    have += total;
+    __syncthreads();
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// the address of `p` in the first block of the cluster, and stores to it
+__device__ __forceinline__ uint32_t in_first_block(const void* p) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(pcbtc::smem_u32(p)));
+  return r;
+}
+__device__ __forceinline__ void store_there(uint32_t at, uint64_t v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
+__device__ __forceinline__ void store_there(uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
+
+// `split` blocks (a cluster; 1: no cluster) per row, split = the cluster's size; joined through distributed shared memory,
+// so that no call needs a workspace.
+template <typename T>
+__global__ void __launch_bounds__(ROW_THREADS) logprob_row_kernel(LogprobArgs a, uint32_t split) {
+  constexpr uint32_t N = Vec<T>::N, U = Tile<T>::U, STEP = ROW_THREADS * U;
+  __shared__ RowShared sh;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x % split;
+  for (uint64_t row = blockIdx.x / split; row < a.rows; row += gridDim.x / split) {
+    if (split > 1) cluster_arrive();   // the others run: their shared memory may be written from the wait on
+    const T* x = static_cast<const T*>(a.x) + row * a.stride;
+    // asked for early: the row's token and its logit
+    int64_t token = -1;
+    float x_token = 0.0f;
+    if (tid == 0 && rank == 0 && a.tokens) {
+      token = token_at(a.tokens, a.token_bytes, row);
+      if (token >= 0 && token < (int64_t)a.cats) x_token = to_f32(x[token]);
+    }
+    Part<T> p;
+    p.off = (uint32_t)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+    p.base = x - p.off;
+    p.end = p.off + a.cats;
+    const uint32_t granules = (uint32_t)(((uint64_t)p.end + N - 1) / N), each = (granules + split - 1) / split;
+    p.g0 = min(granules, rank * each);
+    p.g1 = min(granules, p.g0 + each);
+    p.shift = 0;
+    while ((((p.g1 - p.g0 + STEP - 1) / STEP) >> p.shift) >= SLOTS) ++p.shift;
+
+    Stat s{-INFINITY, 0.0f, 0.0f};
+    float2 S2 = {0.0f, 0.0f}, A2 = {0.0f, 0.0f};
+    float slot = -INFINITY;
+    uint32_t tile = 0;
+    for (uint32_t g0 = p.g0; g0 < p.g1; g0 += STEP, ++tile) {
+      uint4 raw[U];
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t g = g0 + u * ROW_THREADS + tid;
+        if (g < p.g1 && p.whole(g)) raw[u] = load16(p.base + (size_t)g * N);
       }
-      for (int o = 16; o; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
-      if (lane == 0) best[warp] = key;
-      __syncthreads();
-      key = best[0];
-      for (uint32_t w = 1; w < 8; ++w) key = max(key, best[w]);
-      if (threadIdx.x == 0) {
-        const uint32_t j = ~(uint32_t)key;
-        a.top_ids[row * a.top_k + k] = j;
-        a.top_logp[row * a.top_k + k] = logp_of(to_f32(x[j]), s.m, lnS, a.invT);
+      float f[U][N];
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t g = g0 + u * ROW_THREADS + tid;
+        if (g < p.g1 && p.whole(g)) {
+          unpack<T>(raw[u], f[u]);
+        } else if (g < p.g1) {
+          p.read(g, f[u]);
+        } else {
+#pragma unroll
+          for (uint32_t v = 0; v < N; ++v) f[u][v] = -INFINITY;
+        }
       }
-      last = key;
-      __syncthreads();
+      float most = -INFINITY;
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+        for (uint32_t v = 0; v < N; ++v) most = fmaxf(most, f[u][v]);
+      if (most > s.m) {
+        if (s.m != -INFINITY) {   // else: the sums are 0, or NaN
+          const float d = max_nan((s.m - most) * a.c, NO_MASS), e = ex2_ftz(d);
+          A2 = mul2({e, e}, fma2({d, d}, S2, A2));
+          S2 = mul2({e, e}, S2);
+        }
+        s.m = most;
+      }
+      const float shift = -finite_shift(s.m);
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+        for (uint32_t v = 0; v < N; v += 2) {
+          float2 d = mul2(add2({f[u][v], f[u][v + 1]}, {shift, shift}), {a.c, a.c});
+          d.x = max_nan(d.x, NO_MASS);
+          d.y = max_nan(d.y, NO_MASS);
+          const float2 e = {ex2_ftz(d.x), ex2_ftz(d.y)};
+          S2 = add2(S2, e);
+          A2 = fma2(e, d, A2);
+        }
+      slot = fmaxf(slot, most);
+      if (a.top_k && ((tile + 1) & ((1u << p.shift) - 1)) == 0) {
+        sh.slot[tile >> p.shift][tid] = slot;
+        slot = -INFINITY;
+      }
+    }
+    if (a.top_k && (tile & ((1u << p.shift) - 1)) != 0) sh.slot[tile >> p.shift][tid] = slot;
+    s.S = S2.x + S2.y;
+    s.A = A2.x + A2.y;
+    const float mine = s.m;
+    s = lanes_join<32>(s, a.c);
+    if (lane == 0) sh.part[warp] = s;
+    __syncthreads();
+    s = lanes_join<8>(sh.part[lane & 7], a.c);
+    if (a.top_k) block_top<T>(p, sh, a.top_k, mine, s.S != s.S);
+    if (split > 1) {
+      cluster_wait();
+      if (tid == 0) {
+        const uint32_t at = in_first_block(&sh.joined[rank]);
+        store_there(at, s.m);
+        store_there(at + 4, s.S);
+        store_there(at + 8, s.A);
+      }
+      if (tid < a.top_k) store_there(in_first_block(&sh.all[rank][tid]), sh.best[tid]);
+      cluster_arrive();
+      cluster_wait();
+      if (rank == 0) {
+        s = lanes_join<8>((lane & 7) < split ? sh.joined[lane & 7] : Stat{-INFINITY, 0.0f, 0.0f}, a.c);
+        if (a.top_k) {
+          const uint64_t key = tid < split * a.top_k ? sh.all[tid / a.top_k][tid % a.top_k] : 0;
+          uint32_t above = 0;
+          for (uint32_t r = 0; r < split; ++r)
+            for (uint32_t k = 0; k < a.top_k; ++k) above += sh.all[r][k] > key;
+          if (key && above < a.top_k) sh.best[above] = key;
+          __syncthreads();
+        }
+      }
+    }
+    if (rank == 0) {
+      const float lnS = s.S == 0.0f ? 0.0f : logf(s.S);
+      if (tid == 0) {
+        if (a.tokens) a.logp[row] = token < 0 ? 0.0f : token >= (int64_t)a.cats ? NAN : logp_of(x_token, s.m, lnS, a.invT);
+        a.entropy[row] = s.S == 0.0f ? 0.0f : lnS - LN2 * s.A / s.S;
+        a.stats[2 * row] = s.m;
+        a.stats[2 * row + 1] = s.S;
+      }
+      if (tid < a.top_k) {
+        const uint64_t key = sh.best[tid];
+        a.top_ids[row * a.top_k + tid] = (uint32_t)~key;
+        a.top_logp[row * a.top_k + tid] = logp_of(value_of(key), s.m, lnS, a.invT);
+      }
     }
     __syncthreads();
   }
+}
+
+// ---- short rows: L = 2^lg lanes of a warp per row, the whole row in registers -------------------------------------------
+// E elements per lane; element (i, v) of lane l is (l + i L) N + v in rows that are read as granules, l + i L otherwise.
+constexpr uint32_t SHORT_CATS = 1024;
+
+template <typename T, int E, bool GRANULES>
+struct ShortRow {
+  static constexpr uint32_t N = GRANULES ? Vec<T>::N : 1;
+  float f[E];
+  uint32_t sub, lg, cats;
+  __device__ __forceinline__ uint32_t index(int e) const { return (sub + ((uint32_t)(e / N) << lg)) * N + e % N; }
+  __device__ __forceinline__ void load(const T* x) {
+    if constexpr (GRANULES) {
+#pragma unroll
+      for (int i = 0; i < E / (int)N; ++i) {
+        const uint32_t g = sub + ((uint32_t)i << lg);
+        if (g * N < cats) {
+          unpack<T>(load16(x + g * N), f + i * N);
+        } else {
+#pragma unroll
+          for (uint32_t v = 0; v < N; ++v) f[i * N + v] = -INFINITY;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = index(e) < cats ? to_f32(x[index(e)]) : -INFINITY;
+    }
+  }
+};
+template <typename V, typename F>
+__device__ __forceinline__ V over_lanes(V v, uint32_t lg, F f) {   // f over the 2^lg lanes of a row
+  for (uint32_t o = 1u << lg >> 1; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+template <typename T, int E, bool GRANULES>
+__global__ void __launch_bounds__(256) logprob_short_kernel(LogprobArgs a, uint32_t lg) {
+  const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg;
+  ShortRow<T, E, GRANULES> r;
+  r.sub = lane & ((1u << lg) - 1);
+  r.lg = lg;
+  r.cats = a.cats;
+  const auto most_of = [](float x, float y) { return fmaxf(x, y); };
+  const auto sum_of = [](float x, float y) { return x + y; };
+  const uint64_t step = (uint64_t)gridDim.x * 8 * per_warp;
+  for (uint64_t r0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * per_warp; r0 < a.rows; r0 += step) {
+    const uint64_t mine = r0 + (lane >> lg);
+    const bool writes = mine < a.rows && r.sub == 0;
+    const uint64_t row = mine < a.rows ? mine : a.rows - 1;
+    const T* x = static_cast<const T*>(a.x) + row * a.stride;
+    r.load(x);
+    int64_t token = -1;
+    float x_token = 0.0f;
+    if (writes && a.tokens) {
+      token = token_at(a.tokens, a.token_bytes, row);
+      if (token >= 0 && token < (int64_t)a.cats) x_token = to_f32(x[token]);
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmaxf(m, r.f[e]);
+    m = over_lanes(m, lg, most_of);
+    const float shift = -finite_shift(m);
+    float2 S2 = {0.0f, 0.0f}, A2 = {0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      float2 d = mul2(add2({r.f[e], r.f[e + 1]}, {shift, shift}), {a.c, a.c});
+      d.x = max_nan(d.x, NO_MASS);
+      d.y = max_nan(d.y, NO_MASS);
+      const float2 p = {ex2_ftz(d.x), ex2_ftz(d.y)};
+      S2 = add2(S2, p);
+      A2 = fma2(p, d, A2);
+    }
+    const float S = over_lanes(S2.x + S2.y, lg, sum_of), A = over_lanes(A2.x + A2.y, lg, sum_of);
+    const float lnS = S == 0.0f ? 0.0f : logf(S);
+    if (writes) {
+      if (a.tokens) a.logp[row] = token < 0 ? 0.0f : token >= (int64_t)a.cats ? NAN : logp_of(x_token, m, lnS, a.invT);
+      a.entropy[row] = S == 0.0f ? 0.0f : lnS - LN2 * A / S;
+      reinterpret_cast<float2*>(a.stats)[row] = {m, S};
+    }
+    if (a.top_k == 0) continue;
+    if (__any_sync(0xffffffffu, S != S)) {   // NaN or inf somewhere: by keys, which order them too
+      uint64_t last = ~0ull;
+      for (uint32_t k = 0; k < a.top_k; ++k) {
+        uint64_t key = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const uint64_t o = r.index(e) < a.cats ? order_key(r.f[e], r.index(e)) : 0;
+          if (o < last && o > key) key = o;
+        }
+        key = over_lanes(key, lg, [](uint64_t x, uint64_t y) { return x > y ? x : y; });
+        if (writes) {
+          a.top_ids[row * a.top_k + k] = (uint32_t)~key;
+          a.top_logp[row * a.top_k + k] = logp_of(value_of(key), m, lnS, a.invT);
+        }
+        last = key;
+      }
+      continue;
+    }
+    // one alternative a round: the largest value that is left, then the lowest index that holds it
+    uint32_t taken = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) taken |= (uint32_t)(r.index(e) >= a.cats) << e;
+    float best = m;
+    for (uint32_t k = 0; k < a.top_k; ++k) {
+      if (k) {
+        best = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; ++e) best = taken >> e & 1 ? best : fmaxf(best, r.f[e]);
+        best = over_lanes(best, lg, most_of);
+      }
+      uint32_t own = 0xffffffffu;   // the lane's first place that holds it
+#pragma unroll
+      for (int e = E - 1; e >= 0; --e) own = r.f[e] == best && !(taken >> e & 1) ? (uint32_t)e : own;
+      const uint32_t at = own == 0xffffffffu ? own : (r.sub + ((own / r.N) << lg)) * r.N + own % r.N;
+      const uint32_t first = over_lanes(at, lg, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
+      if (at == first) taken |= 1u << (own & 31);
+      if (writes) {
+        a.top_ids[row * a.top_k + k] = first;
+        a.top_logp[row * a.top_k + k] = logp_of(best, m, lnS, a.invT);
+      }
+    }
+  }
+}
+
+// Lanes per row so that each holds about eight elements (all 32 from 129 categories on).
+uint32_t short_lanes_log2(uint32_t cats) {
+  uint32_t lg = 0;
+  while (lg < 5 && cats > (8u << lg)) ++lg;
+  return lg;
+}
+
+template <typename T>
+void launch_short(const LogprobArgs& a, uint32_t sms, cudaStream_t st) {
+  const uint32_t lg = short_lanes_log2(a.cats), each = (a.cats + (1u << lg) - 1) >> lg, per_block = 8u * (32u >> lg);
+  // rows that begin on 16 bytes and end on them are read in granules
+  const bool granules = ((reinterpret_cast<uintptr_t>(a.x) | a.stride * sizeof(T) | a.cats * sizeof(T)) & 15) == 0;
+  const uint64_t blocks = (a.rows + per_block - 1) / per_block;
+  const uint32_t grid = (uint32_t)(blocks < 8ull * sms ? blocks : 8ull * sms);
+  if (granules) {
+    if (each <= 8) logprob_short_kernel<T, 8, true><<<grid, 256, 0, st>>>(a, lg);
+    else if (each <= 16) logprob_short_kernel<T, 16, true><<<grid, 256, 0, st>>>(a, lg);
+    else logprob_short_kernel<T, 32, true><<<grid, 256, 0, st>>>(a, lg);
+  } else {
+    if (each <= 8) logprob_short_kernel<T, 8, false><<<grid, 256, 0, st>>>(a, lg);
+    else if (each <= 16) logprob_short_kernel<T, 16, false><<<grid, 256, 0, st>>>(a, lg);
+    else logprob_short_kernel<T, 32, false><<<grid, 256, 0, st>>>(a, lg);
+  }
+}
+
+// The blocks that share a long row: as many as keep the launch within two blocks per SM, and each with a tile of the row at
+// least.
+template <typename T>
+uint32_t row_split(uint64_t rows, uint32_t cats, uint32_t sms) {
+  uint32_t split = 1;
+  while (split < MAX_CLUSTER && rows * split * 2 <= 2 * (uint64_t)sms && cats >= split * 2 * ROW_THREADS * Vec<T>::N) split *= 2;
+  return split;
+}
+
+template <typename T>
+cudaError_t launch_rows(const LogprobArgs& a, uint32_t sms, cudaStream_t st) {
+  if (a.cats <= SHORT_CATS) {
+    launch_short<T>(a, sms, st);
+    return cudaGetLastError();
+  }
+  const uint32_t split = row_split<T>(a.rows, a.cats, sms);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((uint32_t)(a.rows < (1u << 24) ? a.rows : 1u << 24) * split);
+  cfg.blockDim = dim3(ROW_THREADS);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, logprob_row_kernel<T>, a, split);
 }
 
 struct LogprobGradArgs {
@@ -277,6 +787,16 @@ __global__ void __launch_bounds__(256) evidence_grad_kernel(EvidenceArgs a) {
   }
 }
 
+uint32_t sm_count() {   // of the current device, looked up once
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if ((n = known[dev & 63].load(std::memory_order_relaxed)) > 0) return (uint32_t)n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  known[dev & 63].store(n, std::memory_order_relaxed);
+  return (uint32_t)n;
+}
+
 int32_t check_logits(const void* x, int32_t dtype, uint32_t cats, float temperature) {
   PCB_REQUIRE(x, "null logits");
   PCB_REQUIRE(dtype == PCB_F32 || dtype == PCB_BF16 || dtype == PCB_F16, "logits are f32, bf16 or f16");
@@ -301,15 +821,16 @@ extern "C" int32_t pcb_token_logprobs(const void* x_dev, int32_t dtype, uint64_t
                                       float* top_logp_dev, pcb_stream s) {
   if (rows == 0) return PCB_OK;
   if (int32_t rc = check_logits(x_dev, dtype, cats, temperature)) return rc;
-  PCB_REQUIRE(entropy_dev && stats_dev, "null argument");
+  PCB_REQUIRE(entropy_dev && stats_dev && ((uintptr_t)stats_dev & 7) == 0, "null argument, or statistics that are not 8-byte aligned");
   PCB_REQUIRE(!tokens_dev || (logp_out_dev && (token_bytes == 4 || token_bytes == 8)), "tokens are int32 or int64 and need an output");
   PCB_REQUIRE(top_k <= MAX_TOP && top_k <= cats, "at most 32 alternatives, and no more than there are categories");
   PCB_REQUIRE(top_k == 0 || (top_ids_dev && top_logp_dev), "alternatives need their outputs");
   LogprobArgs a{x_dev, rows, row_stride, cats, top_k, token_bytes, 1.0f / temperature, LOG2E / temperature, tokens_dev,
                 logp_out_dev, entropy_dev, stats_dev, top_logp_dev, top_ids_dev};
-  const uint32_t grid = (uint32_t)(rows < 0x7fffffffull ? rows : 0x7fffffffull);
-  PCB_BY_DTYPE(dtype, logprob_row_kernel, grid, 256, 0, (cudaStream_t)s, a);
-  PCB_CUDA(cudaGetLastError());
+  const uint32_t sms = sm_count();
+  if (sms == 0) return pcb_fail(PCB_ERR_CUDA, "no CUDA device");
+  PCB_CUDA(dtype == PCB_F32 ? launch_rows<float>(a, sms, (cudaStream_t)s) : dtype == PCB_BF16 ? launch_rows<__nv_bfloat16>(a, sms, (cudaStream_t)s)
+                                                                                          : launch_rows<__half>(a, sms, (cudaStream_t)s));
   return PCB_OK;
 }
 
