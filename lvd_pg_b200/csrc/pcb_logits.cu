@@ -1,17 +1,21 @@
 // pcb_logits.cu — categorical distributions given by logits: log-probabilities of given categories with entropy and
 // best alternatives, their gradient, and soft evidence made of logits, with its gradient.
 //
-// With s = x / T, m = max x and c = log2(e) / T every kernel works on d_j = (x_j - m) c, so that exp(s_j - max s) =
-// 2^d_j: the difference is taken before the scaling, which keeps a row of the type's lowest values (a mask) finite where
-// x c would overflow.  S = sum 2^d, A = sum 2^d d:
-//   logp_j = (x_j - m) / T - ln S          H = ln S - ln2 A / S          p_j = 2^d_j / S
-// Terms of impossible categories (d = -inf) are clamped at -200, where 2^d is zero in fp32: 0 * inf stays out of A, and
-// NaN still passes (max.NaN).  A row without any possible category has S = 0, logp -inf, H = 0 and gradient 0.
+// With s = x / T, m = max x, c = log2(e) / T and d_j = (x_j - m) c every kernel works on 2^d_j = exp(s_j - max s).  With
+// S = sum 2^d, A = sum 2^d d:
+//   logp_j = ln2 d_j - ln S          H = ln S - ln2 A / S          p_j = 2^d_j / S
+// d is formed in one of two ways.  Near: fma(x, c, -round(m c)) with x raised to a floor first, so that impossible
+// categories (-inf) have 2^d = 0 and a finite d: 0 * inf stays out of A, one instruction per two elements; what rounding
+// m c leaves off is the same in every d of the row, in S and in A, and cancels.  Far, where m c could overflow (a row of
+// the type's lowest values, as masks leave it) or the floor would still weigh: (x - m) c, clamped at -200.  NaN passes
+// both (max.NaN).  A row without any possible category has S = 0, logp -inf, H = 0 and gradient 0.
 #include "pcb_internal.h"
 #include "pcb_tc.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 namespace {
 
@@ -47,67 +51,76 @@ __device__ __forceinline__ uint32_t order_bits(float v) {
 }
 __device__ __forceinline__ uint64_t order_key(float v, uint32_t j) { return (uint64_t)order_bits(v) << 32 | (uint32_t)~j; }
 
-struct Stat { float m, S, A; };   // running maximum, sum of 2^d, sum of 2^d d
+// Words of 4 bytes as they lie in memory: one fp32 element or two of 16 bits.
+template <typename T> struct Word;
+template <> struct Word<float> {
+  static constexpr uint32_t NONE = 0xff800000u;   // -inf
+  static constexpr float FLOOR = -1e30f;
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+  static __device__ __forceinline__ float top(uint32_t a) { return __uint_as_float(a); }
+};
+template <> struct Word<__nv_bfloat16> {
+  static constexpr uint32_t NONE = 0xff80ff80u;
+  static constexpr float FLOOR = -1e30f;
+  static __device__ __forceinline__ __nv_bfloat162 of(uint32_t a) { return *reinterpret_cast<const __nv_bfloat162*>(&a); }
+  static __device__ __forceinline__ uint32_t bits(__nv_bfloat162 a) { return *reinterpret_cast<const uint32_t*>(&a); }
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) { return bits(__hmax2(of(a), of(b))); }
+  static __device__ __forceinline__ uint32_t raised(uint32_t a) { return bits(__hmax2_nan(of(a), __float2bfloat162_rn(FLOOR))); }
+  static __device__ __forceinline__ float2 floats(uint32_t a) { return {__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u)}; }
+  static __device__ __forceinline__ float top(uint32_t a) { const float2 f = floats(a); return fmaxf(f.x, f.y); }
+  static __device__ __forceinline__ uint32_t equal(uint32_t a, float v) { return __heq2_mask(of(a), __float2bfloat162_rn(v)); }
+};
+template <> struct Word<__half> {
+  static constexpr uint32_t NONE = 0xfc00fc00u;
+  static constexpr float FLOOR = -65504.0f;
+  static __device__ __forceinline__ __half2 of(uint32_t a) { return *reinterpret_cast<const __half2*>(&a); }
+  static __device__ __forceinline__ uint32_t bits(__half2 a) { return *reinterpret_cast<const uint32_t*>(&a); }
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) { return bits(__hmax2(of(a), of(b))); }
+  static __device__ __forceinline__ uint32_t raised(uint32_t a) { return bits(__hmax2_nan(of(a), __float2half2_rn(FLOOR))); }
+  static __device__ __forceinline__ float2 floats(uint32_t a) { return __half22float2(of(a)); }
+  static __device__ __forceinline__ float top(uint32_t a) { const float2 f = floats(a); return fmaxf(f.x, f.y); }
+  static __device__ __forceinline__ uint32_t equal(uint32_t a, float v) { return __heq2_mask(of(a), __float2half2_rn(v)); }
+};
+template <typename T> constexpr uint32_t PER_WORD = 4 / sizeof(T);
 
-__device__ __forceinline__ Stat join(Stat a, Stat b, float c) {
-  Stat r;
-  r.m = fmaxf(a.m, b.m);
-  // a side without a possible value has S = 0 (or NaN, which has to pass): taken as it is
-  const float da = a.m == -INFINITY ? 0.0f : max_nan((a.m - r.m) * c, NO_MASS);
-  const float db = b.m == -INFINITY ? 0.0f : max_nan((b.m - r.m) * c, NO_MASS);
-  const float fa = ex2_ftz(da), fb = ex2_ftz(db);
-  r.S = a.S * fa + b.S * fb;
-  r.A = fa * (a.A + da * a.S) + fb * (b.A + db * b.S);
-  return r;
+// Where the powers of a row count from.
+struct Shift {
+  float m, c, mc;   // mc: m c, rounded
+  bool near;
+};
+template <typename T>
+__device__ __forceinline__ Shift shift_of(float m, float c) {
+  return {m, c, m * c, fabsf(m) < 1e29f && (m - Word<T>::FLOOR) * c > 200.0f && c < 1e8f};
 }
-__device__ __forceinline__ Stat warp_join(Stat s, float c) {
+__device__ __forceinline__ float scaled(const Shift& s, float x) {   // d, clamped; x finite or not
+  return max_nan(s.near ? fmaf(x, s.c, -s.mc) : (x - s.m) * s.c, NO_MASS);
+}
+// log2 of the factor between powers counted from a and from b
+__device__ __forceinline__ float between(const Shift& a, const Shift& b) {
+  return max_nan(a.near && b.near ? a.mc - b.mc : (a.m - b.m) * a.c, NO_MASS);
+}
+
+struct Stat { float m, S, A; };   // maximum, sum of 2^d, sum of 2^d d
+
+// lanes' statistics joined over `width` neighbouring lanes.  Where a side has no possible value, S is 0 (or NaN, which has
+// to pass): it is taken as it is.
+template <typename T, int width>
+__device__ __forceinline__ Stat lanes_join(Stat s, float c) {
+  float m = s.m;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    Stat t;
-    t.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-    t.S = __shfl_xor_sync(0xffffffffu, s.S, o);
-    t.A = __shfl_xor_sync(0xffffffffu, s.A, o);
-    s = join(s, t, c);
+  for (int o = width / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float d = s.m == -INFINITY || s.m == m ? 0.0f : between(shift_of<T>(s.m, c), shift_of<T>(m, c)), f = ex2_ftz(d);
+  s.A = f * (s.A + d * s.S);
+  s.S *= f;
+#pragma unroll
+  for (int o = width / 2; o; o >>= 1) {
+    s.S += __shfl_xor_sync(0xffffffffu, s.S, o);
+    s.A += __shfl_xor_sync(0xffffffffu, s.A, o);
   }
+  s.m = m;
   return s;
 }
-// one more value into a running statistic
-__device__ __forceinline__ void put(Stat& s, float x, float c) {
-  if (x > s.m) {
-    const float d = max_nan((s.m - x) * c, NO_MASS), f = ex2_ftz(d);   // s.m may be -inf: d = -200, f = 0
-    s.A = f * (s.A + d * s.S);
-    s.S *= f;
-    s.m = x;
-  }
-  const float d = max_nan((x - finite_shift(s.m)) * c, NO_MASS), e = ex2_ftz(d);
-  s.S += e;
-  s.A += e * d;
-}
 
-// 16-byte granules: VEC elements, in fp32 and back
-template <typename T> struct Vec { static constexpr uint32_t N = 16 / sizeof(T); };
-__device__ __forceinline__ uint4 load16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-template <typename T> __device__ __forceinline__ void unpack(uint4 v, float* f);
-template <> __device__ __forceinline__ void unpack<float>(uint4 v, float* f) {
-  f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
-}
-template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(uint4 v, float* f) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-}
-template <> __device__ __forceinline__ void unpack<__half>(uint4 v, float* f) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    f[2 * i] = p.x; f[2 * i + 1] = p.y;
-  }
-}
 // two fp32 operations in one instruction
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 r;
@@ -129,6 +142,59 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
+// 16-byte granules
+template <typename T> struct Vec { static constexpr uint32_t N = 16 / sizeof(T); };
+__device__ __forceinline__ uint4 load16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+// elements e and e + 1 (e even) of words
+template <typename T>
+__device__ __forceinline__ float2 pair_of(const uint32_t* w, int e) {
+  if constexpr (sizeof(T) == 4) return {__uint_as_float(w[e]), __uint_as_float(w[e + 1])};
+  else return Word<T>::floats(w[e / 2]);
+}
+template <typename T>
+__device__ __forceinline__ float element_of(const uint32_t* w, int e) {
+  const float2 p = pair_of<T>(w, e & ~1);
+  return e & 1 ? p.y : p.x;
+}
+template <typename T, int W>
+__device__ __forceinline__ float most_of_words(const uint32_t* w) {   // NaN does not count
+  uint32_t m = w[0];
+#pragma unroll
+  for (int i = 1; i < W; ++i) m = Word<T>::most(m, w[i]);
+  return fmaxf(Word<T>::top(m), -INFINITY);
+}
+// 2^d and 2^d d of W words (an even number of elements) added to S and A
+template <typename T, int W>
+__device__ __forceinline__ void add_words(const uint32_t* w, const Shift& s, float2& S, float2& A) {
+  constexpr int E = W * (int)PER_WORD<T>;
+  if (s.near) {
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      float2 x;
+      if constexpr (sizeof(T) == 4) x = {max_nan(__uint_as_float(w[e]), Word<T>::FLOOR), max_nan(__uint_as_float(w[e + 1]), Word<T>::FLOOR)};
+      else x = Word<T>::floats(Word<T>::raised(w[e / 2]));
+      const float2 d = fma2(x, {s.c, s.c}, {-s.mc, -s.mc});
+      const float2 p = {ex2_ftz(d.x), ex2_ftz(d.y)};
+      S = add2(S, p);
+      A = fma2(p, d, A);
+    }
+  } else {
+    const float m = finite_shift(s.m);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 x = pair_of<T>(w, e);
+      const float2 d = {max_nan((x.x - m) * s.c, NO_MASS), max_nan((x.y - m) * s.c, NO_MASS)};
+      const float2 p = {ex2_ftz(d.x), ex2_ftz(d.y)};
+      S = add2(S, p);
+      A = fma2(p, d, A);
+    }
+  }
+}
+
 __device__ __forceinline__ int64_t token_at(const void* tokens, uint32_t bytes, uint64_t r) {
   return bytes == 8 ? static_cast<const int64_t*>(tokens)[r] : static_cast<const int32_t*>(tokens)[r];
 }
@@ -143,9 +209,21 @@ struct LogprobArgs {
   int64_t* top_ids;
 };
 
-// log-probability of the value x in a row of statistics (m, ln S)
-__device__ __forceinline__ float logp_of(float x, float m, float lnS, float invT) {
-  return m == -INFINITY && !(lnS != lnS) ? -INFINITY : (x - m) * invT - lnS;
+// Log-probability of the value x in a row that counts from s; impossible ones are -inf, not the clamp's value.
+__device__ __forceinline__ float logp_of(float x, const Shift& s, float lnS) {
+  if (x == -INFINITY) return lnS != lnS ? lnS : -INFINITY;
+  const float d = s.near ? fmaf(x, s.c, -s.mc) : (x - s.m) * s.c;
+  if (d < -1e30f) {   // a mask's value: finite in natural units where d may not be
+    const float k = s.c * LN2;
+    return ((x < 0.0f) == (s.m < 0.0f) ? (x - s.m) * k : x * k - s.m * k) - lnS;
+  }
+  return fmaf(d, LN2, -lnS);
+}
+__device__ __forceinline__ float ln_of(float S) { return S == 0.0f ? 0.0f : logf(S); }
+__device__ __forceinline__ float entropy_of(float S, float A, float lnS) { return S == 0.0f ? 0.0f : lnS - LN2 * __fdividef(A, S); }
+__device__ __forceinline__ bool is_category(const LogprobArgs& a, int64_t token) { return token >= 0 && token < (int64_t)a.cats; }
+__device__ __forceinline__ float token_logp(const LogprobArgs& a, int64_t token, float x, const Shift& s, float lnS) {
+  return token < 0 ? 0.0f : token >= (int64_t)a.cats ? NAN : logp_of(x, s, lnS);
 }
 
 // ---- long rows: a block, or the blocks of a cluster, per row -------------------------------------------------------
@@ -169,17 +247,24 @@ struct Part {
   uint32_t off, end;    // the row's elements are base[off .. end)
   uint32_t g0, g1, shift;
   __device__ __forceinline__ bool whole(uint32_t g) const { return g * Vec<T>::N >= off && (g + 1) * Vec<T>::N <= end; }
-  // the granule's elements in fp32; -inf outside of the row
-  __device__ __forceinline__ void read(uint32_t g, float* f) const {
-    if (whole(g)) {
-      unpack<T>(load16(base + (size_t)g * Vec<T>::N), f);
-    } else {
+  // the granule as it lies in memory, -inf outside of the row
+  __device__ __forceinline__ uint4 read(uint32_t g) const {
+    if (whole(g)) return load16(base + (size_t)g * Vec<T>::N);
+    uint32_t w[4] = {Word<T>::NONE, Word<T>::NONE, Word<T>::NONE, Word<T>::NONE};
 #pragma unroll
-      for (uint32_t v = 0; v < Vec<T>::N; ++v) {
-        const uint32_t j = g * Vec<T>::N + v;
-        f[v] = j >= off && j < end ? to_f32(base[j]) : -INFINITY;
-      }
+    for (uint32_t v = 0; v < Vec<T>::N; ++v) {
+      const uint32_t j = g * Vec<T>::N + v;
+      if (j < off || j >= end) continue;
+      if constexpr (sizeof(T) == 4) w[v] = reinterpret_cast<const uint32_t*>(base)[j];
+      else w[v / 2] = (w[v / 2] & (v & 1 ? 0xffffu : 0xffff0000u)) | (uint32_t)reinterpret_cast<const uint16_t*>(base)[j] << (16 * (v & 1));
     }
+    return {w[0], w[1], w[2], w[3]};
+  }
+  __device__ __forceinline__ void read(uint32_t g, float* f) const {   // its elements in fp32
+    const uint4 q = read(g);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (uint32_t v = 0; v < Vec<T>::N; ++v) f[v] = element_of<T>(w, v);
   }
   __device__ __forceinline__ bool inside(uint32_t g, uint32_t v) const {
     const uint32_t j = g * Vec<T>::N + v;
@@ -202,24 +287,6 @@ struct RowShared {
 __device__ __forceinline__ float value_of(uint64_t key) {   // inverse of order_bits, but for NaN
   const uint32_t u = (uint32_t)(key >> 32);
   return u == 0xffffffffu ? NAN : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
-}
-
-// lanes' statistics joined over `width` neighbouring lanes
-template <int width>
-__device__ __forceinline__ Stat lanes_join(Stat s, float c) {
-  float m = s.m;
-#pragma unroll
-  for (int o = width / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float d = s.m == -INFINITY ? 0.0f : max_nan((s.m - m) * c, NO_MASS), f = ex2_ftz(d);
-  s.A = f * (s.A + d * s.S);
-  s.S *= f;
-#pragma unroll
-  for (int o = width / 2; o; o >>= 1) {
-    s.S += __shfl_xor_sync(0xffffffffu, s.S, o);
-    s.A += __shfl_xor_sync(0xffffffffu, s.A, o);
-  }
-  s.m = m;
-  return s;
 }
 
 // f(granule) for the granules of the thread's tiles whose noted maximum passes `pick`
@@ -361,7 +428,7 @@ __device__ __forceinline__ void store_there(uint32_t at, float v) { asm volatile
 // `split` blocks (a cluster; 1: no cluster) per row, split = the cluster's size; joined through distributed shared memory,
 // so that no call needs a workspace.
 template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS) logprob_row_kernel(LogprobArgs a, uint32_t split) {
+__global__ void __launch_bounds__(ROW_THREADS, 4) logprob_row_kernel(LogprobArgs a, uint32_t split) {
   constexpr uint32_t N = Vec<T>::N, U = Tile<T>::U, STEP = ROW_THREADS * U;
   __shared__ RowShared sh;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x % split;
@@ -373,7 +440,7 @@ __global__ void __launch_bounds__(ROW_THREADS) logprob_row_kernel(LogprobArgs a,
     float x_token = 0.0f;
     if (tid == 0 && rank == 0 && a.tokens) {
       token = token_at(a.tokens, a.token_bytes, row);
-      if (token >= 0 && token < (int64_t)a.cats) x_token = to_f32(x[token]);
+      if (is_category(a, token)) x_token = to_f32(x[token]);
     }
     Part<T> p;
     p.off = (uint32_t)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
@@ -386,54 +453,40 @@ __global__ void __launch_bounds__(ROW_THREADS) logprob_row_kernel(LogprobArgs a,
     while ((((p.g1 - p.g0 + STEP - 1) / STEP) >> p.shift) >= SLOTS) ++p.shift;
 
     Stat s{-INFINITY, 0.0f, 0.0f};
+    Shift from = shift_of<T>(-INFINITY, a.c);
     float2 S2 = {0.0f, 0.0f}, A2 = {0.0f, 0.0f};
     float slot = -INFINITY;
     uint32_t tile = 0;
     for (uint32_t g0 = p.g0; g0 < p.g1; g0 += STEP, ++tile) {
-      uint4 raw[U];
+      uint32_t w[U * 4];
+      if (g0 * N >= p.off && g0 + STEP <= p.g1 && (g0 + STEP) * N <= p.end) {   // every granule lies in the row
+        const T* at = p.base + (size_t)(g0 + tid) * N;
 #pragma unroll
-      for (uint32_t u = 0; u < U; ++u) {
-        const uint32_t g = g0 + u * ROW_THREADS + tid;
-        if (g < p.g1 && p.whole(g)) raw[u] = load16(p.base + (size_t)g * N);
-      }
-      float f[U][N];
+        for (uint32_t u = 0; u < U; ++u) {
+          const uint4 q = load16(at + (size_t)u * ROW_THREADS * N);
+          w[4 * u] = q.x; w[4 * u + 1] = q.y; w[4 * u + 2] = q.z; w[4 * u + 3] = q.w;
+        }
+      } else {
 #pragma unroll
-      for (uint32_t u = 0; u < U; ++u) {
-        const uint32_t g = g0 + u * ROW_THREADS + tid;
-        if (g < p.g1 && p.whole(g)) {
-          unpack<T>(raw[u], f[u]);
-        } else if (g < p.g1) {
-          p.read(g, f[u]);
-        } else {
-#pragma unroll
-          for (uint32_t v = 0; v < N; ++v) f[u][v] = -INFINITY;
+        for (uint32_t u = 0; u < U; ++u) {
+          const uint32_t g = g0 + u * ROW_THREADS + tid;
+          uint4 q = {Word<T>::NONE, Word<T>::NONE, Word<T>::NONE, Word<T>::NONE};
+          if (g < p.g1) q = p.read(g);
+          w[4 * u] = q.x; w[4 * u + 1] = q.y; w[4 * u + 2] = q.z; w[4 * u + 3] = q.w;
         }
       }
-      float most = -INFINITY;
-#pragma unroll
-      for (uint32_t u = 0; u < U; ++u)
-#pragma unroll
-        for (uint32_t v = 0; v < N; ++v) most = fmaxf(most, f[u][v]);
+      const float most = most_of_words<T, U * 4>(w);
       if (most > s.m) {
+        const Shift to = shift_of<T>(most, a.c);
         if (s.m != -INFINITY) {   // else: the sums are 0, or NaN
-          const float d = max_nan((s.m - most) * a.c, NO_MASS), e = ex2_ftz(d);
+          const float d = between(from, to), e = ex2_ftz(d);
           A2 = mul2({e, e}, fma2({d, d}, S2, A2));
           S2 = mul2({e, e}, S2);
         }
         s.m = most;
+        from = to;
       }
-      const float shift = -finite_shift(s.m);
-#pragma unroll
-      for (uint32_t u = 0; u < U; ++u)
-#pragma unroll
-        for (uint32_t v = 0; v < N; v += 2) {
-          float2 d = mul2(add2({f[u][v], f[u][v + 1]}, {shift, shift}), {a.c, a.c});
-          d.x = max_nan(d.x, NO_MASS);
-          d.y = max_nan(d.y, NO_MASS);
-          const float2 e = {ex2_ftz(d.x), ex2_ftz(d.y)};
-          S2 = add2(S2, e);
-          A2 = fma2(e, d, A2);
-        }
+      add_words<T, U * 4>(w, from, S2, A2);
       slot = fmaxf(slot, most);
       if (a.top_k && ((tile + 1) & ((1u << p.shift) - 1)) == 0) {
         sh.slot[tile >> p.shift][tid] = slot;
@@ -444,10 +497,10 @@ __global__ void __launch_bounds__(ROW_THREADS) logprob_row_kernel(LogprobArgs a,
     s.S = S2.x + S2.y;
     s.A = A2.x + A2.y;
     const float mine = s.m;
-    s = lanes_join<32>(s, a.c);
+    s = lanes_join<T, 32>(s, a.c);
     if (lane == 0) sh.part[warp] = s;
     __syncthreads();
-    s = lanes_join<8>(sh.part[lane & 7], a.c);
+    s = lanes_join<T, 8>(sh.part[lane & 7], a.c);
     if (a.top_k) block_top<T>(p, sh, a.top_k, mine, s.S != s.S);
     if (split > 1) {
       cluster_wait();
@@ -461,7 +514,7 @@ __global__ void __launch_bounds__(ROW_THREADS) logprob_row_kernel(LogprobArgs a,
       cluster_arrive();
       cluster_wait();
       if (rank == 0) {
-        s = lanes_join<8>((lane & 7) < split ? sh.joined[lane & 7] : Stat{-INFINITY, 0.0f, 0.0f}, a.c);
+        s = lanes_join<T, 8>((lane & 7) < split ? sh.joined[lane & 7] : Stat{-INFINITY, 0.0f, 0.0f}, a.c);
         if (a.top_k) {
           const uint64_t key = tid < split * a.top_k ? sh.all[tid / a.top_k][tid % a.top_k] : 0;
           uint32_t above = 0;
@@ -473,17 +526,17 @@ __global__ void __launch_bounds__(ROW_THREADS) logprob_row_kernel(LogprobArgs a,
       }
     }
     if (rank == 0) {
-      const float lnS = s.S == 0.0f ? 0.0f : logf(s.S);
+      const Shift at = shift_of<T>(s.m, a.c);
+      const float lnS = ln_of(s.S);
       if (tid == 0) {
-        if (a.tokens) a.logp[row] = token < 0 ? 0.0f : token >= (int64_t)a.cats ? NAN : logp_of(x_token, s.m, lnS, a.invT);
-        a.entropy[row] = s.S == 0.0f ? 0.0f : lnS - LN2 * s.A / s.S;
-        a.stats[2 * row] = s.m;
-        a.stats[2 * row + 1] = s.S;
+        if (a.tokens) a.logp[row] = token_logp(a, token, x_token, at, lnS);
+        a.entropy[row] = entropy_of(s.S, s.A, lnS);
+        reinterpret_cast<float2*>(a.stats)[row] = {s.m, s.S};
       }
       if (tid < a.top_k) {
         const uint64_t key = sh.best[tid];
         a.top_ids[row * a.top_k + tid] = (uint32_t)~key;
-        a.top_logp[row * a.top_k + tid] = logp_of(value_of(key), s.m, lnS, a.invT);
+        a.top_logp[row * a.top_k + tid] = logp_of(value_of(key), at, lnS);
       }
     }
     __syncthreads();
@@ -491,33 +544,15 @@ __global__ void __launch_bounds__(ROW_THREADS) logprob_row_kernel(LogprobArgs a,
 }
 
 // ---- short rows: L = 2^lg lanes of a warp per row, the whole row in registers -------------------------------------------
-// E elements per lane; element (i, v) of lane l is (l + i L) N + v in rows that are read as granules, l + i L otherwise.
-constexpr uint32_t SHORT_CATS = 1024;
+// E elements per lane, kept as they came; element (i, v) of lane l is (l + i L) N + v in rows that are read as granules,
+// l + i L otherwise.  Few lanes per row make few shuffles: one shuffle serves all rows of the warp.
+template <typename T> struct Most;   // elements a lane holds at most: 64 bytes
+template <> struct Most<float> { static constexpr uint32_t E = 16; };
+template <> struct Most<__nv_bfloat16> { static constexpr uint32_t E = 32; };
+template <> struct Most<__half> { static constexpr uint32_t E = 32; };
 
-template <typename T, int E, bool GRANULES>
-struct ShortRow {
-  static constexpr uint32_t N = GRANULES ? Vec<T>::N : 1;
-  float f[E];
-  uint32_t sub, lg, cats;
-  __device__ __forceinline__ uint32_t index(int e) const { return (sub + ((uint32_t)(e / N) << lg)) * N + e % N; }
-  __device__ __forceinline__ void load(const T* x) {
-    if constexpr (GRANULES) {
-#pragma unroll
-      for (int i = 0; i < E / (int)N; ++i) {
-        const uint32_t g = sub + ((uint32_t)i << lg);
-        if (g * N < cats) {
-          unpack<T>(load16(x + g * N), f + i * N);
-        } else {
-#pragma unroll
-          for (uint32_t v = 0; v < N; ++v) f[i * N + v] = -INFINITY;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = index(e) < cats ? to_f32(x[index(e)]) : -INFINITY;
-    }
-  }
-};
+__device__ __forceinline__ float most_of(float x, float y) { return fmaxf(x, y); }
+__device__ __forceinline__ float sum_of(float x, float y) { return x + y; }
 template <typename V, typename F>
 __device__ __forceinline__ V over_lanes(V v, uint32_t lg, F f) {   // f over the 2^lg lanes of a row
   for (uint32_t o = 1u << lg >> 1; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -525,117 +560,255 @@ __device__ __forceinline__ V over_lanes(V v, uint32_t lg, F f) {   // f over the
 }
 
 template <typename T, int E, bool GRANULES>
-__global__ void __launch_bounds__(256) logprob_short_kernel(LogprobArgs a, uint32_t lg) {
-  const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg;
-  ShortRow<T, E, GRANULES> r;
-  r.sub = lane & ((1u << lg) - 1);
-  r.lg = lg;
-  r.cats = a.cats;
-  const auto most_of = [](float x, float y) { return fmaxf(x, y); };
-  const auto sum_of = [](float x, float y) { return x + y; };
+struct ShortRow {
+  static constexpr uint32_t N = GRANULES ? Vec<T>::N : 1;
+  static constexpr int W = E / (int)PER_WORD<T>;
+  uint32_t w[W];
+
+  static __device__ __forceinline__ uint32_t index(int e, uint32_t sub, uint32_t lg) { return (sub + ((uint32_t)(e / N) << lg)) * N + e % N; }
+  __device__ __forceinline__ void load(const T* x, uint32_t sub, uint32_t lg, uint32_t cats) {
+    if constexpr (GRANULES) {
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        const uint32_t g = sub + ((uint32_t)i << lg);
+        uint4 v = {Word<T>::NONE, Word<T>::NONE, Word<T>::NONE, Word<T>::NONE};
+        if (g * N < cats) v = load16(x + g * N);
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) w[e] = index(e, sub, lg) < cats ? __float_as_uint(x[index(e, sub, lg)]) : Word<T>::NONE;
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const uint32_t lo = index(e, sub, lg) < cats ? h[index(e, sub, lg)] : Word<T>::NONE & 0xffffu;
+        const uint32_t hi = index(e + 1, sub, lg) < cats ? h[index(e + 1, sub, lg)] : Word<T>::NONE & 0xffffu;
+        w[e / 2] = lo | hi << 16;
+      }
+    }
+  }
+  // NaN in its place: counts no more in the lane's maximum and equals nothing
+  __device__ __forceinline__ void strike(uint32_t e, bool yes) {
+    const uint32_t place = yes ? e / PER_WORD<T> : 0xffffffffu, bits = sizeof(T) == 4 ? 0x7fffffffu : e & 1 ? 0x7fff0000u : 0x7fffu;
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] |= place == (uint32_t)i ? bits : 0u;
+  }
+  // the first place that holds v, 0xffffffff if none does
+  __device__ __forceinline__ uint32_t find(float v) const {
+    uint32_t hits = 0;   // fp32: bit e; else bit i for element 2 i, 16 + i for 2 i + 1
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) hits |= __uint_as_float(w[e]) == v ? 1u << e : 0u;
+      return hits ? __ffs(hits) - 1 : 0xffffffffu;
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) hits |= Word<T>::equal(w[i], v) & (0x10001u << i);
+      const uint32_t lo = hits & 0xffffu, hi = hits >> 16;
+      return min(lo ? 2 * (uint32_t)__ffs(lo) - 2 : 0xffffffffu, hi ? 2 * (uint32_t)__ffs(hi) - 1 : 0xffffffffu);
+    }
+  }
+};
+
+// A row's results, by the lanes that hold it; `writes` in one of them.  x_token: the token's logit, where `writes` holds.
+template <typename T, int E, bool GRANULES>
+__device__ __forceinline__ void short_results(const LogprobArgs& a, ShortRow<T, E, GRANULES>& r, uint64_t row, bool writes, int64_t token,
+                                              float x_token, uint32_t sub, uint32_t lg) {
+  using Row = ShortRow<T, E, GRANULES>;
+  const float m = over_lanes(most_of_words<T, Row::W>(r.w), lg, most_of);
+  const Shift from = shift_of<T>(m, a.c);
+  float2 S2 = {0.0f, 0.0f}, A2 = {0.0f, 0.0f};
+  add_words<T, Row::W>(r.w, from, S2, A2);
+  const float S = over_lanes(S2.x + S2.y, lg, sum_of), A = over_lanes(A2.x + A2.y, lg, sum_of);
+  const float lnS = ln_of(S);
+  if (writes) {
+    if (a.tokens) a.logp[row] = token_logp(a, token, x_token, from, lnS);
+    a.entropy[row] = entropy_of(S, A, lnS);
+    reinterpret_cast<float2*>(a.stats)[row] = {m, S};
+  }
+  if (a.top_k == 0) return;
+  if (__any_sync(0xffffffffu, S != S)) {   // NaN or inf somewhere: by keys, which order them too
+    uint64_t last = ~0ull;
+    for (uint32_t k = 0; k < a.top_k; ++k) {
+      uint64_t key = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t j = Row::index(e, sub, lg);
+        const uint64_t o = j < a.cats ? order_key(element_of<T>(r.w, e), j) : 0;
+        if (o < last && o > key) key = o;
+      }
+      key = over_lanes(key, lg, [](uint64_t x, uint64_t y) { return x > y ? x : y; });
+      if (writes) {
+        a.top_ids[row * a.top_k + k] = (uint32_t)~key;
+        a.top_logp[row * a.top_k + k] = logp_of(value_of(key), from, lnS);
+      }
+      last = key;
+    }
+    return;
+  }
+  // one alternative a round: the largest value that is left, then the lowest index that holds it.  (Places past the last
+  // category hold -inf at indices above every category's: they are never the lowest while a category is left.)
+  float best = m;
+  for (uint32_t k = 0; k < a.top_k; ++k) {
+    if (k) best = over_lanes(most_of_words<T, Row::W>(r.w), lg, most_of);
+    const uint32_t own = r.find(best), at = own == 0xffffffffu ? own : Row::index(0, sub, lg) + (((own / Row::N) << lg) * Row::N) + own % Row::N;
+    const uint32_t first = over_lanes(at, lg, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
+    if (writes) {
+      a.top_ids[row * a.top_k + k] = first;
+      a.top_logp[row * a.top_k + k] = logp_of(best, from, lnS);
+    }
+    if (k + 1 < a.top_k) r.strike(own, at == first);
+  }
+}
+
+// Rows in 16-byte granules: the next row is on its way while this one is worked on.
+template <typename T, int E>
+__global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_short_kernel(LogprobArgs a, uint32_t lg) {
+  using Row = ShortRow<T, E, true>;
+  const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1);
+  const uint64_t step = (uint64_t)gridDim.x * 8 * per_warp;
+  uint64_t r0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * per_warp;
+  const auto row_of = [&](uint64_t first) { const uint64_t r = first + (lane >> lg); return r < a.rows ? r : a.rows - 1; };
+  const auto fetch = [&](uint64_t first, Row& r, int64_t& token) {
+    const uint64_t row = row_of(first);
+    r.load(static_cast<const T*>(a.x) + row * a.stride, sub, lg, a.cats);
+    token = a.tokens ? token_at(a.tokens, a.token_bytes, row) : -1;
+  };
+  Row next;
+  int64_t next_token = -1;
+  if (r0 < a.rows) fetch(r0, next, next_token);
+  for (; r0 < a.rows; r0 += step) {
+    Row r = next;
+    const int64_t token = next_token;
+    if (r0 + step < a.rows) fetch(r0 + step, next, next_token);
+    // (from memory again: cheaper than picking it out of the lanes' registers)
+    const bool writes = r0 + (lane >> lg) < a.rows && sub == 0;
+    const float x_token = writes && is_category(a, token) ? to_f32((static_cast<const T*>(a.x) + row_of(r0) * a.stride)[token]) : 0.0f;
+    short_results<T, E, true>(a, r, row_of(r0), writes, token, x_token, sub, lg);
+  }
+}
+
+// Rows of any length and alignment, one behind the other (stride = cats): every warp stages the bytes of `rows_staged` of
+// them, from the 16-byte boundary below their beginning on, with asynchronous copies, two stages deep, and its lanes read
+// their elements there.
+constexpr uint32_t STAGE = 2048 + 32;   // bytes: 32 lanes' 64, and the granules that the rows share with others
+
+template <typename T, int E>
+__global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_staged_kernel(LogprobArgs a, uint32_t lg, uint32_t rows_staged) {
+  using Row = ShortRow<T, E, false>;
+  __shared__ __align__(16) uint8_t stage[8][2][STAGE];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1);
+  const uintptr_t x0 = reinterpret_cast<uintptr_t>(a.x), x1 = x0 + a.rows * a.cats * sizeof(T);
+  const uint64_t step = (uint64_t)gridDim.x * 8 * rows_staged;
+  const auto fetch = [&](uint64_t first, uint32_t buf) {   // the rows from `first` on
+    const uintptr_t lo = x0 + first * a.cats * sizeof(T), hi = min((uint64_t)x1, (uint64_t)(lo + (uint64_t)rows_staged * a.cats * sizeof(T)));
+    uint8_t* dst = stage[warp][buf];
+    for (uintptr_t at = (lo & ~(uintptr_t)15) + 16 * lane; at < hi; at += 512, dst += 512) {
+      if (at >= x0 && at + 16 <= x1) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(pcbtc::smem_u32(dst + 16 * lane)), "l"(at) : "memory");
+      } else {   // the granule reaches over an end of the tensor
+        for (uint32_t i = 0; i < 16; i += sizeof(T))
+          if (at + i >= x0 && at + i < x1) *reinterpret_cast<T*>(dst + 16 * lane + i) = *reinterpret_cast<const T*>(at + i);
+      }
+    }
+  };
+  uint64_t q0 = ((uint64_t)blockIdx.x * 8 + warp) * rows_staged;
+  if (q0 < a.rows) fetch(q0, 0);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  for (uint32_t buf = 0; q0 < a.rows; q0 += step, buf ^= 1) {
+    if (q0 + step < a.rows) fetch(q0 + step, buf ^ 1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    const uintptr_t lo = x0 + q0 * a.cats * sizeof(T);
+    const T* rows = reinterpret_cast<const T*>(stage[warp][buf] + (lo & 15));
+    const uint64_t q1 = min(a.rows, q0 + rows_staged);
+    for (uint64_t r0 = q0; r0 < q1; r0 += per_warp) {
+      const bool valid = r0 + (lane >> lg) < q1;
+      const uint64_t row = valid ? r0 + (lane >> lg) : q1 - 1;
+      const T* x = rows + (uint32_t)(row - q0) * a.cats;
+      const int64_t token = a.tokens ? token_at(a.tokens, a.token_bytes, row) : -1;
+      Row r;
+      r.load(x, sub, lg, a.cats);
+      const float x_token = is_category(a, token) ? to_f32(x[token]) : 0.0f;
+      short_results<T, E, false>(a, r, row, valid && sub == 0, token, x_token, sub, lg);
+    }
+    __syncwarp();   // everybody has read this stage
+  }
+}
+
+// Rows of any length, alignment and distance, element by element.
+template <typename T, int E>
+__global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_spread_kernel(LogprobArgs a, uint32_t lg) {
+  using Row = ShortRow<T, E, false>;
+  const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1);
   const uint64_t step = (uint64_t)gridDim.x * 8 * per_warp;
   for (uint64_t r0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * per_warp; r0 < a.rows; r0 += step) {
-    const uint64_t mine = r0 + (lane >> lg);
-    const bool writes = mine < a.rows && r.sub == 0;
-    const uint64_t row = mine < a.rows ? mine : a.rows - 1;
+    const bool valid = r0 + (lane >> lg) < a.rows;
+    const uint64_t row = valid ? r0 + (lane >> lg) : a.rows - 1;
     const T* x = static_cast<const T*>(a.x) + row * a.stride;
-    r.load(x);
-    int64_t token = -1;
-    float x_token = 0.0f;
-    if (writes && a.tokens) {
-      token = token_at(a.tokens, a.token_bytes, row);
-      if (token >= 0 && token < (int64_t)a.cats) x_token = to_f32(x[token]);
-    }
-    float m = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < E; ++e) m = fmaxf(m, r.f[e]);
-    m = over_lanes(m, lg, most_of);
-    const float shift = -finite_shift(m);
-    float2 S2 = {0.0f, 0.0f}, A2 = {0.0f, 0.0f};
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      float2 d = mul2(add2({r.f[e], r.f[e + 1]}, {shift, shift}), {a.c, a.c});
-      d.x = max_nan(d.x, NO_MASS);
-      d.y = max_nan(d.y, NO_MASS);
-      const float2 p = {ex2_ftz(d.x), ex2_ftz(d.y)};
-      S2 = add2(S2, p);
-      A2 = fma2(p, d, A2);
-    }
-    const float S = over_lanes(S2.x + S2.y, lg, sum_of), A = over_lanes(A2.x + A2.y, lg, sum_of);
-    const float lnS = S == 0.0f ? 0.0f : logf(S);
-    if (writes) {
-      if (a.tokens) a.logp[row] = token < 0 ? 0.0f : token >= (int64_t)a.cats ? NAN : logp_of(x_token, m, lnS, a.invT);
-      a.entropy[row] = S == 0.0f ? 0.0f : lnS - LN2 * A / S;
-      reinterpret_cast<float2*>(a.stats)[row] = {m, S};
-    }
-    if (a.top_k == 0) continue;
-    if (__any_sync(0xffffffffu, S != S)) {   // NaN or inf somewhere: by keys, which order them too
-      uint64_t last = ~0ull;
-      for (uint32_t k = 0; k < a.top_k; ++k) {
-        uint64_t key = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint64_t o = r.index(e) < a.cats ? order_key(r.f[e], r.index(e)) : 0;
-          if (o < last && o > key) key = o;
-        }
-        key = over_lanes(key, lg, [](uint64_t x, uint64_t y) { return x > y ? x : y; });
-        if (writes) {
-          a.top_ids[row * a.top_k + k] = (uint32_t)~key;
-          a.top_logp[row * a.top_k + k] = logp_of(value_of(key), m, lnS, a.invT);
-        }
-        last = key;
-      }
-      continue;
-    }
-    // one alternative a round: the largest value that is left, then the lowest index that holds it
-    uint32_t taken = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) taken |= (uint32_t)(r.index(e) >= a.cats) << e;
-    float best = m;
-    for (uint32_t k = 0; k < a.top_k; ++k) {
-      if (k) {
-        best = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < E; ++e) best = taken >> e & 1 ? best : fmaxf(best, r.f[e]);
-        best = over_lanes(best, lg, most_of);
-      }
-      uint32_t own = 0xffffffffu;   // the lane's first place that holds it
-#pragma unroll
-      for (int e = E - 1; e >= 0; --e) own = r.f[e] == best && !(taken >> e & 1) ? (uint32_t)e : own;
-      const uint32_t at = own == 0xffffffffu ? own : (r.sub + ((own / r.N) << lg)) * r.N + own % r.N;
-      const uint32_t first = over_lanes(at, lg, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
-      if (at == first) taken |= 1u << (own & 31);
-      if (writes) {
-        a.top_ids[row * a.top_k + k] = first;
-        a.top_logp[row * a.top_k + k] = logp_of(best, m, lnS, a.invT);
-      }
-    }
+    const int64_t token = a.tokens ? token_at(a.tokens, a.token_bytes, row) : -1;
+    Row r;
+    r.load(x, sub, lg, a.cats);
+    const float x_token = is_category(a, token) ? to_f32(x[token]) : 0.0f;
+    short_results<T, E, false>(a, r, row, valid && sub == 0, token, x_token, sub, lg);
   }
 }
 
-// Lanes per row so that each holds about eight elements (all 32 from 129 categories on).
-uint32_t short_lanes_log2(uint32_t cats) {
-  uint32_t lg = 0;
-  while (lg < 5 && cats > (8u << lg)) ++lg;
-  return lg;
+enum RowForm { GRANULE_ROWS, STAGED_ROWS, SPREAD_ROWS };
+struct ShortShape {
+  RowForm form;
+  uint32_t lg, each;   // log2 of the lanes per row, elements per lane
+};
+// Few lanes per row; four at least where the row has as many granules (64 contiguous bytes per load), sixteen where it
+// is read from memory by elements.
+template <typename T>
+ShortShape short_shape(uint32_t cats, uint64_t stride, const void* x) {
+  ShortShape s;
+  s.form = ((reinterpret_cast<uintptr_t>(x) | stride * sizeof(T) | (uint64_t)cats * sizeof(T)) & 15) == 0 ? GRANULE_ROWS
+         : stride == cats ? STAGED_ROWS : SPREAD_ROWS;
+  const uint32_t units = s.form == GRANULE_ROWS ? cats / Vec<T>::N : cats;
+  const uint32_t wanted = s.form == GRANULE_ROWS ? 4 : s.form == STAGED_ROWS ? 1 : 16;
+  s.lg = 0;
+  while (s.lg < 5 && (cats > (Most<T>::E << s.lg) || (1u << s.lg) < (units < wanted ? units : wanted))) ++s.lg;
+  s.each = s.form == GRANULE_ROWS ? ((units + (1u << s.lg) - 1) >> s.lg) * Vec<T>::N : (cats + (1u << s.lg) - 1) >> s.lg;
+  return s;
 }
 
+// blocks of `kernel` (256 threads) that fill the GPU, at most `needed`
+template <auto kernel>
+uint32_t resident_blocks(uint32_t sms, uint64_t needed) {
+  static std::atomic<int> known[64];   // per device
+  int dev = 0, per_sm = 1;
+  if (cudaGetDevice(&dev) == cudaSuccess && (per_sm = known[dev & 63].load(std::memory_order_relaxed)) < 1) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, 256, 0) != cudaSuccess || per_sm < 1) per_sm = 1;
+    known[dev & 63].store(per_sm, std::memory_order_relaxed);
+  }
+  const uint64_t all = (uint64_t)per_sm * sms;
+  return (uint32_t)(needed < all ? needed : all);
+}
+
+template <typename T, int E>
+void launch_short_as(const LogprobArgs& a, const ShortShape& s, uint32_t sms, cudaStream_t st) {
+  const uint32_t per_warp = 32u >> s.lg;
+  const auto needed = [&](uint32_t rows_per_warp) { return (a.rows + 8 * rows_per_warp - 1) / (8 * rows_per_warp); };
+  if (s.form == GRANULE_ROWS) {
+    if constexpr (E >= (int)Vec<T>::N)
+      logprob_short_kernel<T, E><<<resident_blocks<logprob_short_kernel<T, E>>(sms, needed(per_warp)), 256, 0, st>>>(a, s.lg);
+  } else if (s.form == STAGED_ROWS) {
+    const uint32_t fit = 2048 / (a.cats * (uint32_t)sizeof(T)), staged = fit > per_warp ? fit / per_warp * per_warp : per_warp;
+    logprob_staged_kernel<T, E><<<resident_blocks<logprob_staged_kernel<T, E>>(sms, needed(staged)), 256, 0, st>>>(a, s.lg, staged);
+  } else {
+    logprob_spread_kernel<T, E><<<resident_blocks<logprob_spread_kernel<T, E>>(sms, needed(per_warp)), 256, 0, st>>>(a, s.lg);
+  }
+}
 template <typename T>
 void launch_short(const LogprobArgs& a, uint32_t sms, cudaStream_t st) {
-  const uint32_t lg = short_lanes_log2(a.cats), each = (a.cats + (1u << lg) - 1) >> lg, per_block = 8u * (32u >> lg);
-  // rows that begin on 16 bytes and end on them are read in granules
-  const bool granules = ((reinterpret_cast<uintptr_t>(a.x) | a.stride * sizeof(T) | a.cats * sizeof(T)) & 15) == 0;
-  const uint64_t blocks = (a.rows + per_block - 1) / per_block;
-  const uint32_t grid = (uint32_t)(blocks < 8ull * sms ? blocks : 8ull * sms);
-  if (granules) {
-    if (each <= 8) logprob_short_kernel<T, 8, true><<<grid, 256, 0, st>>>(a, lg);
-    else if (each <= 16) logprob_short_kernel<T, 16, true><<<grid, 256, 0, st>>>(a, lg);
-    else logprob_short_kernel<T, 32, true><<<grid, 256, 0, st>>>(a, lg);
-  } else {
-    if (each <= 8) logprob_short_kernel<T, 8, false><<<grid, 256, 0, st>>>(a, lg);
-    else if (each <= 16) logprob_short_kernel<T, 16, false><<<grid, 256, 0, st>>>(a, lg);
-    else logprob_short_kernel<T, 32, false><<<grid, 256, 0, st>>>(a, lg);
-  }
+  const ShortShape s = short_shape<T>(a.cats, a.stride, a.x);
+  if (s.each <= 4) launch_short_as<T, 4>(a, s, sms, st);
+  else if (s.each <= 8) launch_short_as<T, 8>(a, s, sms, st);
+  else if (s.each <= 16) launch_short_as<T, 16>(a, s, sms, st);
+  else launch_short_as<T, Most<T>::E>(a, s, sms, st);
 }
 
 // The blocks that share a long row: as many as keep the launch within two blocks per SM, and each with a tile of the row at
@@ -649,7 +822,7 @@ uint32_t row_split(uint64_t rows, uint32_t cats, uint32_t sms) {
 
 template <typename T>
 cudaError_t launch_rows(const LogprobArgs& a, uint32_t sms, cudaStream_t st) {
-  if (a.cats <= SHORT_CATS) {
+  if (a.cats <= 32 * Most<T>::E) {
     launch_short<T>(a, sms, st);
     return cudaGetLastError();
   }
@@ -681,12 +854,14 @@ struct LogprobGradArgs {
 // What a row's gradient is made of: dx_j = 2^d_j (alpha + beta d_j) + the parts of the token and the alternatives, with
 // alpha = -(gL + sum gK + gH (H - ln S)) / (T S), beta = -gH ln2 / (T S).
 struct RowGrad {
-  float m, S, alpha, beta, gl;
+  Shift from;
+  float S, alpha, beta, gl;
   int64_t token;   // negative: none
 };
+template <typename T>
 __device__ __forceinline__ RowGrad row_grad(const LogprobGradArgs& a, uint64_t row) {
   RowGrad g;
-  g.m = a.stats[2 * row];
+  g.from = shift_of<T>(a.stats[2 * row], a.c);
   g.S = a.stats[2 * row + 1];
   g.token = -1;
   g.gl = 0.0f;
@@ -703,15 +878,15 @@ __device__ __forceinline__ RowGrad row_grad(const LogprobGradArgs& a, uint64_t r
   g.beta = -gh * LN2 * scale;
   return g;
 }
-__device__ __forceinline__ float grad_of(const RowGrad& g, float x, float c) {
-  const float d = max_nan((x - g.m) * c, NO_MASS);
+__device__ __forceinline__ float grad_of(const RowGrad& g, float x) {
+  const float d = scaled(g.from, x);
   return ex2_ftz(d) * fmaf(g.beta, d, g.alpha);
 }
 __device__ __forceinline__ bool no_mass(const RowGrad& g) { return g.S == 0.0f; }
 // the whole gradient of an element that the token or an alternative may point to
 __device__ __forceinline__ float pointed_grad(const LogprobGradArgs& a, const RowGrad& g, uint64_t row, uint32_t j, float x) {
   if (no_mass(g)) return 0.0f;
-  float v = grad_of(g, x, a.c);
+  float v = grad_of(g, x);
   if (g.token == (int64_t)j) v += g.gl * a.invT;
   if (a.g_top)
     for (uint32_t k = 0; k < a.top_k; ++k)
@@ -724,7 +899,7 @@ __global__ void __launch_bounds__(256) logprob_grad_kernel(LogprobGradArgs a) {
   for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.stride;
     T* dx = static_cast<T*>(a.dx) + row * a.cats;
-    const RowGrad g = row_grad(a, row);
+    const RowGrad g = row_grad<T>(a, row);
     for (uint32_t j = threadIdx.x; j < a.cats; j += blockDim.x) dx[j] = from_f32<T>(pointed_grad(a, g, row, j, to_f32(x[j])));
   }
 }
@@ -752,14 +927,17 @@ __global__ void __launch_bounds__(256) evidence_kernel(EvidenceArgs a) {
     float* out = a.out + b + a.rows * v;
     const uint64_t step = a.rows * a.vars;
     const bool missing = a.miss && a.miss[b * a.miss_row_stride + v * a.miss_var_stride];
-    Stat s{-INFINITY, 0.0f, 0.0f};
-    for (uint32_t j = lane; j < a.cats; j += 32) put(s, to_f32(x[j]), a.c);
-    s = warp_join(s, a.c);
-    const float lnS = s.m == -INFINITY && s.S == 0.0f ? 0.0f : logf(s.S);
-    for (uint32_t j = lane; j < a.cats; j += 32) out[j * step] = missing ? 0.0f : logp_of(to_f32(x[j]), s.m, lnS, a.invT);
+    float m = -INFINITY, S = 0.0f;
+    for (uint32_t j = lane; j < a.cats; j += 32) m = fmaxf(m, to_f32(x[j]));
+    m = over_lanes(m, 5, most_of);
+    const Shift from = shift_of<T>(m, a.c);
+    for (uint32_t j = lane; j < a.cats; j += 32) S += m == -INFINITY && x[j] == x[j] ? 0.0f : ex2_ftz(scaled(from, to_f32(x[j])));
+    S = over_lanes(S, 5, sum_of);
+    const float lnS = ln_of(S);
+    for (uint32_t j = lane; j < a.cats; j += 32) out[j * step] = missing ? 0.0f : logp_of(to_f32(x[j]), from, lnS);
     if (a.stats_out && lane == 0) {
-      a.stats_out[2 * (b * a.vars + v)] = s.m;
-      a.stats_out[2 * (b * a.vars + v) + 1] = s.S;
+      a.stats_out[2 * (b * a.vars + v)] = m;
+      a.stats_out[2 * (b * a.vars + v) + 1] = S;
     }
   }
 }
@@ -775,13 +953,14 @@ __global__ void __launch_bounds__(256) evidence_grad_kernel(EvidenceArgs a) {
     const float* g = a.g + b + a.rows * v;
     T* dx = static_cast<T*>(a.dx) + (b * a.vars + v) * a.cats;
     const uint64_t step = a.rows * a.vars;
-    const float m = a.stats[2 * (b * a.vars + v)], S = a.stats[2 * (b * a.vars + v) + 1];
+    const Shift from = shift_of<T>(a.stats[2 * (b * a.vars + v)], a.c);
+    const float S = a.stats[2 * (b * a.vars + v) + 1];
     const bool none = (a.miss && a.miss[b * a.miss_row_stride + v * a.miss_var_stride]) || S == 0.0f;
     float sum = 0.0f;
     for (uint32_t j = lane; j < a.cats; j += 32) sum += g[j * step];
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     for (uint32_t j = lane; j < a.cats; j += 32) {
-      const float e = ex2_ftz(max_nan((to_f32(x[j]) - m) * a.c, NO_MASS));
+      const float e = ex2_ftz(scaled(from, to_f32(x[j])));
       dx[j] = from_f32<T>(none ? 0.0f : (g[j * step] - e * (sum / S)) * a.invT);
     }
   }
@@ -800,6 +979,7 @@ uint32_t sm_count() {   // of the current device, looked up once
 int32_t check_logits(const void* x, int32_t dtype, uint32_t cats, float temperature) {
   PCB_REQUIRE(x, "null logits");
   PCB_REQUIRE(dtype == PCB_F32 || dtype == PCB_BF16 || dtype == PCB_F16, "logits are f32, bf16 or f16");
+  PCB_REQUIRE(((uintptr_t)x & (dtype == PCB_F32 ? 3 : 1)) == 0, "logits that are not aligned to their own size");
   PCB_REQUIRE(cats >= 1 && cats <= 0x7fffffffu, "the number of categories must be between 1 and 2^31 - 1");
   PCB_REQUIRE(temperature > 0.0f && LOG2E / temperature < INFINITY && 1.0f / temperature > 0.0f, "the temperature must be positive and finite");
   return PCB_OK;
