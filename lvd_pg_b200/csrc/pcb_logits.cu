@@ -15,6 +15,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -236,7 +237,7 @@ __device__ __forceinline__ float token_logp(const LogprobArgs& a, int64_t token,
 // those (rows of few different values, or large ones side by side in few groups) raise the bound to the k-th of what
 // was collected, as long as that helps; what is left then (mostly ties) goes by rounds over what lies above the bound and
 // one walk in index order over what equals it.
-constexpr uint32_t ROW_THREADS = 256, SLOTS = 16, CAND = 256, MAX_CLUSTER = 8;
+constexpr uint32_t SLOTS = 16, CAND = 256, PAIRS = 256, MAX_CLUSTER = 8;
 
 template <typename T> struct Tile { static constexpr uint32_t U = sizeof(T) == 4 ? 8 : 4; };   // granules per thread
 
@@ -273,15 +274,17 @@ struct Part {
   __device__ __forceinline__ uint32_t index(uint32_t g, uint32_t v) const { return g * Vec<T>::N + v - off; }
 };
 
+template <uint32_t THREADS>
 struct RowShared {
-  float slot[SLOTS][ROW_THREADS];
+  float slot[SLOTS][THREADS];
   uint64_t cand[CAND];
-  uint64_t best[MAX_TOP];            // this block's alternatives, in order
-  uint64_t all[MAX_CLUSTER][MAX_TOP];   // first block of a cluster: every block's
+  uint64_t best[MAX_TOP];   // this block's alternatives, in order
+  uint64_t all[THREADS == 256 ? MAX_CLUSTER : 1][MAX_TOP];   // first block of a cluster: every block's
   Stat part[8], joined[MAX_CLUSTER];
   float group[32];
-  uint64_t round[8];
-  uint32_t count, warp_count[8];
+  uint64_t round[THREADS / 32];
+  uint32_t pair[PAIRS];   // slot * THREADS + thread
+  uint32_t pairs, count, warp_count[THREADS / 32];
 };
 
 __device__ __forceinline__ float value_of(uint64_t key) {   // inverse of order_bits, but for NaN
@@ -290,16 +293,16 @@ __device__ __forceinline__ float value_of(uint64_t key) {   // inverse of order_
 }
 
 // f(granule) for the granules of the thread's tiles whose noted maximum passes `pick`
-template <typename T, typename P, typename F>
-__device__ __forceinline__ void picked_granules(const Part<T>& p, const RowShared& sh, P pick, F f) {
-  constexpr uint32_t U = Tile<T>::U, STEP = ROW_THREADS * U;
+template <uint32_t THREADS, typename T, typename P, typename F>
+__device__ __forceinline__ void picked_granules(const Part<T>& p, const RowShared<THREADS>& sh, P pick, F f) {
+  constexpr uint32_t U = Tile<T>::U, STEP = THREADS * U;
   const uint32_t tiles = (p.g1 - p.g0 + STEP - 1) / STEP, slots = (tiles + (1u << p.shift) - 1) >> p.shift;
   for (uint32_t s = 0; s < slots; ++s) {
     if (!pick(sh.slot[s][threadIdx.x])) continue;
     const uint32_t t1 = min(tiles, (s + 1) << p.shift);
     for (uint32_t t = s << p.shift; t < t1; ++t)
       for (uint32_t u = 0; u < U; ++u) {
-        const uint32_t g = p.g0 + t * STEP + u * ROW_THREADS + threadIdx.x;
+        const uint32_t g = p.g0 + t * STEP + u * THREADS + threadIdx.x;
         if (g < p.g1) f(g);
       }
   }
@@ -307,15 +310,16 @@ __device__ __forceinline__ void picked_granules(const Part<T>& p, const RowShare
 
 // The block's `top_k` largest, in order, into sh.best (0: there is no further one).  `mine`: the thread's largest value;
 // `wild`: the part holds NaN, which no noted maximum shows.
-template <typename T>
-__device__ void block_top(const Part<T>& p, RowShared& sh, uint32_t top_k, float mine, bool wild) {
+template <uint32_t THREADS, typename T>
+__device__ void block_top(const Part<T>& p, RowShared<THREADS>& sh, uint32_t top_k, float mine, bool wild) {
+  constexpr uint32_t U = Tile<T>::U, STEP = THREADS * U, WARPS = THREADS / 32;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid < MAX_TOP) sh.best[tid] = 0;
   float gm = mine;
 #pragma unroll
-  for (int o = 4; o; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
-  if ((lane & 7) == 0) sh.group[warp * 4 + (lane >> 3)] = gm;
-  if (tid == 0) sh.count = 0;
+  for (uint32_t o = WARPS / 2; o; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+  if (lane % WARPS == 0) sh.group[tid / WARPS] = gm;
+  if (tid == 0) sh.pairs = sh.count = 0;
   __syncthreads();
   float bound;
   {
@@ -328,9 +332,23 @@ __device__ void block_top(const Part<T>& p, RowShared& sh, uint32_t top_k, float
     }
     bound = __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, above == top_k - 1)) - 1);
   }
-  bool raised = !wild;
-  for (uint32_t tries = 0; raised && tries < 8; ++tries) {
-    picked_granules<T>(p, sh, [&](float m) { return m >= bound; }, [&](uint32_t g) {
+  const uint32_t tiles = (p.g1 - p.g0 + STEP - 1) / STEP, slots = (tiles + (1u << p.shift) - 1) >> p.shift;
+  bool again = !wild;
+  for (uint32_t tries = 0; again && tries < 8; ++tries) {
+    // the slots that reach the bound, then their granules over all threads: one trip to memory
+    for (uint32_t s = 0; s < slots; ++s)
+      if (sh.slot[s][tid] >= bound) {
+        const uint32_t at = atomicAdd(&sh.pairs, 1u);
+        if (at < PAIRS) sh.pair[at] = s * THREADS + tid;
+      }
+    __syncthreads();
+    const uint32_t pairs = sh.pairs;
+    if (pairs > PAIRS) break;   // ties, mostly: by rounds
+    const uint32_t per_pair = U << p.shift;   // granules, a power of two
+    for (uint32_t i = tid; i < pairs * per_pair; i += THREADS) {
+      const uint32_t pr = sh.pair[i / per_pair], k = i % per_pair;
+      const uint32_t g = p.g0 + (((pr / THREADS) << p.shift) + k / U) * STEP + k % U * THREADS + pr % THREADS;
+      if (g >= p.g1) continue;
       float f[Vec<T>::N];
       p.read(g, f);
 #pragma unroll
@@ -339,19 +357,21 @@ __device__ void block_top(const Part<T>& p, RowShared& sh, uint32_t top_k, float
           const uint32_t at = atomicAdd(&sh.count, 1u);
           if (at < CAND) sh.cand[at] = order_key(f[v], p.index(g, v));
         }
-    });
+    }
     __syncthreads();
     const uint32_t found = sh.count, n = min(found, CAND);
-    uint32_t above = 0;
-    const uint64_t key = tid < n ? sh.cand[tid] : 0;
-    for (uint32_t j = 0; j < n; ++j) above += sh.cand[j] > key;
-    if (tid < n && above < top_k) sh.best[above] = key;
+    for (uint32_t i = tid; i < n; i += THREADS) {
+      const uint64_t key = sh.cand[i];
+      uint32_t above = 0;
+      for (uint32_t j = 0; j < n; ++j) above += sh.cand[j] > key;
+      if (above < top_k) sh.best[above] = key;
+    }
     __syncthreads();
     if (found <= CAND) return;
-    const float better = value_of(sh.best[top_k - 1]);
-    raised = better > bound;
-    bound = raised ? better : bound;
-    if (tid == 0) sh.count = 0;
+    const float better = value_of(sh.best[top_k - 1]);   // of CAND values that reach the bound
+    again = better > bound;
+    bound = again ? better : bound;
+    if (tid == 0) sh.pairs = sh.count = 0;
     __syncthreads();
     if (tid < MAX_TOP) sh.best[tid] = 0;
   }
@@ -361,7 +381,7 @@ __device__ void block_top(const Part<T>& p, RowShared& sh, uint32_t top_k, float
   __syncthreads();
   while (have < top_k) {
     uint64_t key = 0;
-    picked_granules<T>(p, sh, [&](float m) { return wild || m > bound; }, [&](uint32_t g) {
+    picked_granules<THREADS>(p, sh, [&](float m) { return wild || m > bound; }, [&](uint32_t g) {
       float f[Vec<T>::N];
       p.read(g, f);
 #pragma unroll
@@ -375,7 +395,7 @@ __device__ void block_top(const Part<T>& p, RowShared& sh, uint32_t top_k, float
     for (int o = 16; o; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
     if (lane == 0) sh.round[warp] = key;
     __syncthreads();
-    for (uint32_t w = 0; w < 8; ++w) key = max(key, sh.round[w]);
+    for (uint32_t w = 0; w < WARPS; ++w) key = max(key, sh.round[w]);
     __syncthreads();
     if (key == 0) break;
     if (tid == 0) sh.best[have] = key;
@@ -383,7 +403,7 @@ __device__ void block_top(const Part<T>& p, RowShared& sh, uint32_t top_k, float
     last = key;
   }
   // what equals the bound, in index order
-  for (uint32_t g0 = p.g0; g0 < p.g1 && have < top_k && !wild; g0 += ROW_THREADS) {
+  for (uint32_t g0 = p.g0; g0 < p.g1 && have < top_k && !wild; g0 += THREADS) {
     const uint32_t g = g0 + tid;
     float f[Vec<T>::N];
     uint32_t hits = 0;
@@ -402,7 +422,7 @@ __device__ void block_top(const Part<T>& p, RowShared& sh, uint32_t top_k, float
     before -= __popc(hits);
     __syncthreads();
     uint32_t total = 0;
-    for (uint32_t w = 0; w < 8; ++w) {
+    for (uint32_t w = 0; w < WARPS; ++w) {
       if (w < warp) before += sh.warp_count[w];
       total += sh.warp_count[w];
     }
@@ -427,13 +447,13 @@ __device__ __forceinline__ void store_there(uint32_t at, float v) { asm volatile
 
 // `split` blocks (a cluster; 1: no cluster) per row, split = the cluster's size; joined through distributed shared memory,
 // so that no call needs a workspace.
-template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS, 4) logprob_row_kernel(LogprobArgs a, uint32_t split) {
-  constexpr uint32_t N = Vec<T>::N, U = Tile<T>::U, STEP = ROW_THREADS * U;
-  __shared__ RowShared sh;
+template <typename T, uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_row_kernel(LogprobArgs a, uint32_t split) {
+  constexpr uint32_t N = Vec<T>::N, U = Tile<T>::U, STEP = THREADS * U, WARPS = THREADS / 32;
+  __shared__ RowShared<THREADS> sh;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x % split;
   for (uint64_t row = blockIdx.x / split; row < a.rows; row += gridDim.x / split) {
-    if (split > 1) cluster_arrive();   // the others run: their shared memory may be written from the wait on
+    if (THREADS == 256 && split > 1) cluster_arrive();   // the others run: their shared memory may be written from the wait on
     const T* x = static_cast<const T*>(a.x) + row * a.stride;
     // asked for early: the row's token and its logit
     int64_t token = -1;
@@ -463,13 +483,13 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) logprob_row_kernel(LogprobArgs
         const T* at = p.base + (size_t)(g0 + tid) * N;
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
-          const uint4 q = load16(at + (size_t)u * ROW_THREADS * N);
+          const uint4 q = load16(at + (size_t)u * THREADS * N);
           w[4 * u] = q.x; w[4 * u + 1] = q.y; w[4 * u + 2] = q.z; w[4 * u + 3] = q.w;
         }
       } else {
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
-          const uint32_t g = g0 + u * ROW_THREADS + tid;
+          const uint32_t g = g0 + u * THREADS + tid;
           uint4 q = {Word<T>::NONE, Word<T>::NONE, Word<T>::NONE, Word<T>::NONE};
           if (g < p.g1) q = p.read(g);
           w[4 * u] = q.x; w[4 * u + 1] = q.y; w[4 * u + 2] = q.z; w[4 * u + 3] = q.w;
@@ -500,9 +520,9 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) logprob_row_kernel(LogprobArgs
     s = lanes_join<T, 32>(s, a.c);
     if (lane == 0) sh.part[warp] = s;
     __syncthreads();
-    s = lanes_join<T, 8>(sh.part[lane & 7], a.c);
-    if (a.top_k) block_top<T>(p, sh, a.top_k, mine, s.S != s.S);
-    if (split > 1) {
+    s = lanes_join<T, WARPS>(sh.part[lane % WARPS], a.c);
+    if (a.top_k) block_top<THREADS>(p, sh, a.top_k, mine, s.S != s.S);
+    if (THREADS == 256 && split > 1) {
       cluster_wait();
       if (tid == 0) {
         const uint32_t at = in_first_block(&sh.joined[rank]);
@@ -510,16 +530,16 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) logprob_row_kernel(LogprobArgs
         store_there(at + 4, s.S);
         store_there(at + 8, s.A);
       }
-      if (tid < a.top_k) store_there(in_first_block(&sh.all[rank][tid]), sh.best[tid]);
+      if (tid < a.top_k) store_there(in_first_block(&sh.all[THREADS == 256 ? rank : 0][tid]), sh.best[tid]);
       cluster_arrive();
       cluster_wait();
       if (rank == 0) {
         s = lanes_join<T, 8>((lane & 7) < split ? sh.joined[lane & 7] : Stat{-INFINITY, 0.0f, 0.0f}, a.c);
         if (a.top_k) {
-          const uint64_t key = tid < split * a.top_k ? sh.all[tid / a.top_k][tid % a.top_k] : 0;
+          const uint64_t key = tid < split * a.top_k ? sh.all[THREADS == 256 ? tid / a.top_k : 0][tid % a.top_k] : 0;
           uint32_t above = 0;
           for (uint32_t r = 0; r < split; ++r)
-            for (uint32_t k = 0; k < a.top_k; ++k) above += sh.all[r][k] > key;
+            for (uint32_t k = 0; k < a.top_k; ++k) above += sh.all[THREADS == 256 ? r : 0][k] > key;
           if (key && above < a.top_k) sh.best[above] = key;
           __syncthreads();
         }
@@ -610,178 +630,211 @@ struct ShortRow {
   }
 };
 
-// A row's results, by the lanes that hold it; `writes` in one of them.  x_token: the token's logit, where `writes` holds.
+// What a row leaves for its results.
+struct Kept { float m, S, A, best; uint32_t at; };
+
+// A row's statistics, in all lanes that hold it, and its alternatives: a single one goes into `k`, several are written at
+// once (`valid`: there is such a row).
 template <typename T, int E, bool GRANULES>
-__device__ __forceinline__ void short_results(const LogprobArgs& a, ShortRow<T, E, GRANULES>& r, uint64_t row, bool writes, int64_t token,
-                                              float x_token, uint32_t sub, uint32_t lg) {
+__device__ __forceinline__ Kept short_row(const LogprobArgs& a, ShortRow<T, E, GRANULES>& r, uint64_t row, bool valid, uint32_t sub, uint32_t lg) {
   using Row = ShortRow<T, E, GRANULES>;
-  const float m = over_lanes(most_of_words<T, Row::W>(r.w), lg, most_of);
-  const Shift from = shift_of<T>(m, a.c);
+  Kept k;
+  k.m = over_lanes(most_of_words<T, Row::W>(r.w), lg, most_of);
+  const Shift from = shift_of<T>(k.m, a.c);
   float2 S2 = {0.0f, 0.0f}, A2 = {0.0f, 0.0f};
   add_words<T, Row::W>(r.w, from, S2, A2);
-  const float S = over_lanes(S2.x + S2.y, lg, sum_of), A = over_lanes(A2.x + A2.y, lg, sum_of);
-  const float lnS = ln_of(S);
-  if (writes) {
-    if (a.tokens) a.logp[row] = token_logp(a, token, x_token, from, lnS);
-    a.entropy[row] = entropy_of(S, A, lnS);
-    reinterpret_cast<float2*>(a.stats)[row] = {m, S};
-  }
-  if (a.top_k == 0) return;
-  if (__any_sync(0xffffffffu, S != S)) {   // NaN or inf somewhere: by keys, which order them too
-    uint64_t last = ~0ull;
-    for (uint32_t k = 0; k < a.top_k; ++k) {
-      uint64_t key = 0;
+  k.S = over_lanes(S2.x + S2.y, lg, sum_of);
+  k.A = over_lanes(A2.x + A2.y, lg, sum_of);
+  k.best = k.m;
+  k.at = 0;
+  if (a.top_k == 0) return k;
+  const float lnS = a.top_k > 1 ? ln_of(k.S) : 0.0f;
+  const uint32_t width = 1u << lg;
+  if (__any_sync(0xffffffffu, k.S != k.S)) {   // NaN or inf somewhere: by keys, which order them too
+    uint32_t w[Row::W];   // a copy to be indexed, so that the registers need not be
 #pragma unroll
+    for (int i = 0; i < Row::W; ++i) w[i] = r.w[i];
+    uint64_t last = ~0ull;
+    for (uint32_t n = 0; n < a.top_k; ++n) {
+      uint64_t key = 0;
+#pragma unroll 1
       for (int e = 0; e < E; ++e) {
         const uint32_t j = Row::index(e, sub, lg);
-        const uint64_t o = j < a.cats ? order_key(element_of<T>(r.w, e), j) : 0;
+        const uint64_t o = j < a.cats ? order_key(element_of<T>(w, e), j) : 0;
         if (o < last && o > key) key = o;
       }
       key = over_lanes(key, lg, [](uint64_t x, uint64_t y) { return x > y ? x : y; });
-      if (writes) {
-        a.top_ids[row * a.top_k + k] = (uint32_t)~key;
-        a.top_logp[row * a.top_k + k] = logp_of(value_of(key), from, lnS);
+      k.best = value_of(key);
+      k.at = (uint32_t)~key;
+      if (a.top_k > 1 && valid && sub == 0) {
+        a.top_ids[row * a.top_k + n] = k.at;
+        a.top_logp[row * a.top_k + n] = logp_of(k.best, from, lnS);
       }
       last = key;
     }
-    return;
+    return k;
   }
-  // one alternative a round: the largest value that is left, then the lowest index that holds it.  (Places past the last
-  // category hold -inf at indices above every category's: they are never the lowest while a category is left.)
-  float best = m;
-  for (uint32_t k = 0; k < a.top_k; ++k) {
-    if (k) best = over_lanes(most_of_words<T, Row::W>(r.w), lg, most_of);
+  // One alternative a round: the largest value that is left, then the lowest index that holds it.  (Places past the last
+  // category hold -inf at indices above every category's: they are never the lowest while a category is left.)  A lane
+  // keeps every 2^lg-th and writes it with the others' at the end of as many rounds.
+  float best = k.m, kept = 0.0f;
+  uint32_t kept_at = 0;
+  for (uint32_t n = 0; n < a.top_k; ++n) {
+    if (n) best = over_lanes(most_of_words<T, Row::W>(r.w), lg, most_of);
     const uint32_t own = r.find(best), at = own == 0xffffffffu ? own : Row::index(0, sub, lg) + (((own / Row::N) << lg) * Row::N) + own % Row::N;
     const uint32_t first = over_lanes(at, lg, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
-    if (writes) {
-      a.top_ids[row * a.top_k + k] = first;
-      a.top_logp[row * a.top_k + k] = logp_of(best, from, lnS);
+    if (a.top_k == 1) {
+      k.at = first;
+      break;
     }
-    if (k + 1 < a.top_k) r.strike(own, at == first);
-  }
-}
-
-// Rows in 16-byte granules: the next row is on its way while this one is worked on.
-template <typename T, int E>
-__global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_short_kernel(LogprobArgs a, uint32_t lg) {
-  using Row = ShortRow<T, E, true>;
-  const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1);
-  const uint64_t step = (uint64_t)gridDim.x * 8 * per_warp;
-  uint64_t r0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * per_warp;
-  const auto row_of = [&](uint64_t first) { const uint64_t r = first + (lane >> lg); return r < a.rows ? r : a.rows - 1; };
-  const auto fetch = [&](uint64_t first, Row& r, int64_t& token) {
-    const uint64_t row = row_of(first);
-    r.load(static_cast<const T*>(a.x) + row * a.stride, sub, lg, a.cats);
-    token = a.tokens ? token_at(a.tokens, a.token_bytes, row) : -1;
-  };
-  Row next;
-  int64_t next_token = -1;
-  if (r0 < a.rows) fetch(r0, next, next_token);
-  for (; r0 < a.rows; r0 += step) {
-    Row r = next;
-    const int64_t token = next_token;
-    if (r0 + step < a.rows) fetch(r0 + step, next, next_token);
-    // (from memory again: cheaper than picking it out of the lanes' registers)
-    const bool writes = r0 + (lane >> lg) < a.rows && sub == 0;
-    const float x_token = writes && is_category(a, token) ? to_f32((static_cast<const T*>(a.x) + row_of(r0) * a.stride)[token]) : 0.0f;
-    short_results<T, E, true>(a, r, row_of(r0), writes, token, x_token, sub, lg);
-  }
-}
-
-// Rows of any length and alignment, one behind the other (stride = cats): every warp stages the bytes of `rows_staged` of
-// them, from the 16-byte boundary below their beginning on, with asynchronous copies, two stages deep, and its lanes read
-// their elements there.
-constexpr uint32_t STAGE = 2048 + 32;   // bytes: 32 lanes' 64, and the granules that the rows share with others
-
-template <typename T, int E>
-__global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_staged_kernel(LogprobArgs a, uint32_t lg, uint32_t rows_staged) {
-  using Row = ShortRow<T, E, false>;
-  __shared__ __align__(16) uint8_t stage[8][2][STAGE];
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1);
-  const uintptr_t x0 = reinterpret_cast<uintptr_t>(a.x), x1 = x0 + a.rows * a.cats * sizeof(T);
-  const uint64_t step = (uint64_t)gridDim.x * 8 * rows_staged;
-  const auto fetch = [&](uint64_t first, uint32_t buf) {   // the rows from `first` on
-    const uintptr_t lo = x0 + first * a.cats * sizeof(T), hi = min((uint64_t)x1, (uint64_t)(lo + (uint64_t)rows_staged * a.cats * sizeof(T)));
-    uint8_t* dst = stage[warp][buf];
-    for (uintptr_t at = (lo & ~(uintptr_t)15) + 16 * lane; at < hi; at += 512, dst += 512) {
-      if (at >= x0 && at + 16 <= x1) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(pcbtc::smem_u32(dst + 16 * lane)), "l"(at) : "memory");
-      } else {   // the granule reaches over an end of the tensor
-        for (uint32_t i = 0; i < 16; i += sizeof(T))
-          if (at + i >= x0 && at + i < x1) *reinterpret_cast<T*>(dst + 16 * lane + i) = *reinterpret_cast<const T*>(at + i);
+    if ((n & (width - 1)) == sub) {
+      kept = best;
+      kept_at = first;
+    }
+    if (n + 1 < a.top_k) r.strike(own, at == first);
+    if ((n & (width - 1)) == width - 1 || n + 1 == a.top_k) {
+      const uint32_t place = (n & ~(width - 1)) + sub;
+      if (valid && place <= n) {
+        a.top_ids[row * a.top_k + place] = kept_at;
+        a.top_logp[row * a.top_k + place] = logp_of(kept, from, lnS);
       }
     }
-  };
-  uint64_t q0 = ((uint64_t)blockIdx.x * 8 + warp) * rows_staged;
-  if (q0 < a.rows) fetch(q0, 0);
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  for (uint32_t buf = 0; q0 < a.rows; q0 += step, buf ^= 1) {
-    if (q0 + step < a.rows) fetch(q0 + step, buf ^ 1);
+  }
+  return k;
+}
+
+// The results of up to 32 rows, one per lane.
+template <typename T>
+__device__ __forceinline__ void short_results(const LogprobArgs& a, const Kept& k, uint64_t row, int64_t token, float x_token) {
+  const Shift from = shift_of<T>(k.m, a.c);
+  const float lnS = ln_of(k.S);
+  if (a.tokens) a.logp[row] = token_logp(a, token, x_token, from, lnS);
+  a.entropy[row] = entropy_of(k.S, k.A, lnS);
+  reinterpret_cast<float2*>(a.stats)[row] = {k.m, k.S};
+  if (a.top_k == 1) {
+    a.top_ids[row] = k.at;
+    a.top_logp[row] = logp_of(k.best, from, lnS);
+  }
+}
+
+// Rows in memory: in 16-byte granules, or element by element, whatever their distance.  A warp takes `passes` times the rows
+// that its lanes hold at once, the next ones on their way while it works on these (granules), and writes the results of all
+// of them together: lane (g, j) those of the g-th row of pass j.
+template <typename T, int E, bool GRANULES>
+__global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_short_kernel(LogprobArgs a, uint32_t lg, uint32_t passes) {
+  using Row = ShortRow<T, E, GRANULES>;
+  const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1), group = lane >> lg;
+  const uint64_t step = (uint64_t)gridDim.x * 8 * per_warp * passes;
+  for (uint64_t r0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * per_warp * passes; r0 < a.rows; r0 += step) {
+    const auto row_of = [&](uint32_t pass) { return min(a.rows - 1, r0 + pass * per_warp + group); };
+    const auto row_at = [&](uint64_t row) { return static_cast<const T*>(a.x) + row * a.stride; };
+    Row next;
+    next.load(row_at(row_of(0)), sub, lg, a.cats);
+    const uint64_t mine = r0 + sub * per_warp + group;   // the row whose results this lane writes
+    const bool writes = sub < passes && mine < a.rows;
+    int64_t token = -1;
+    float x_token = 0.0f;
+    if (writes && a.tokens) {
+      token = token_at(a.tokens, a.token_bytes, mine);
+      if (is_category(a, token)) x_token = to_f32(row_at(mine)[token]);
+    }
+    Kept kept = {0.0f, 0.0f, 0.0f, 0.0f, 0};
+    for (uint32_t pass = 0; pass < passes && r0 + pass * per_warp < a.rows; ++pass) {
+      Row r = next;
+      if (GRANULES && pass + 1 < passes) next.load(row_at(row_of(pass + 1)), sub, lg, a.cats);
+      const Kept k = short_row<T, E, GRANULES>(a, r, row_of(pass), r0 + pass * per_warp + group < a.rows, sub, lg);
+      if (sub == pass) kept = k;
+      if (!GRANULES && pass + 1 < passes) next.load(row_at(row_of(pass + 1)), sub, lg, a.cats);
+    }
+    if (writes) short_results<T>(a, kept, mine, token, x_token);
+  }
+}
+
+// Rows one behind the other (stride = cats), of any length and alignment: every warp stages the bytes of `rows_staged` of
+// them, from the 16-byte boundary below their beginning on, with asynchronous copies, STAGES - 1 of them ahead of its work,
+// and its lanes read their elements there.
+constexpr uint32_t STAGES = 3, STAGED_THREADS = 128, STAGED_ROWS_MOST = 128;
+constexpr uint32_t STAGE_BYTES = 2048 + 32;   // 32 lanes' 64 bytes, and the granules that the rows share with others
+
+template <typename T, int E>
+__global__ void __launch_bounds__(STAGED_THREADS, 6) logprob_staged_kernel(LogprobArgs a, uint32_t lg, uint32_t rows_staged) {
+  using Row = ShortRow<T, E, false>;
+  constexpr uint32_t WARPS = STAGED_THREADS / 32;
+  __shared__ __align__(16) uint8_t stages[WARPS][STAGES][STAGE_BYTES];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1), group = lane >> lg;
+  const uintptr_t x0 = reinterpret_cast<uintptr_t>(a.x), x1 = x0 + a.rows * a.cats * sizeof(T);
+  const uint64_t step = (uint64_t)gridDim.x * WARPS * rows_staged;
+  const uint64_t first = ((uint64_t)blockIdx.x * WARPS + warp) * rows_staged;
+  const auto fetch = [&](uint64_t q0, uint8_t* stage) {   // the rows from q0 on
+    if (q0 < a.rows) {
+      const uint32_t n = (uint32_t)min((uint64_t)rows_staged, a.rows - q0);
+      const uintptr_t lo = x0 + q0 * a.cats * sizeof(T), hi = lo + (uintptr_t)n * a.cats * sizeof(T);
+      uint8_t* dst = stage + 16 * lane;
+      for (uintptr_t at = (lo & ~(uintptr_t)15) + 16 * lane; at < hi; at += 512, dst += 512) {
+        if (at >= x0 && at + 16 <= x1) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(pcbtc::smem_u32(dst)), "l"(at) : "memory");
+        } else {   // the granule reaches over an end of the tensor
+          for (uint32_t i = 0; i < 16; i += sizeof(T))
+            if (at + i >= x0 && at + i < x1) *reinterpret_cast<T*>(dst + i) = *reinterpret_cast<const T*>(at + i);
+        }
+      }
+    }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-    __syncwarp();
-    const uintptr_t lo = x0 + q0 * a.cats * sizeof(T);
-    const T* rows = reinterpret_cast<const T*>(stage[warp][buf] + (lo & 15));
-    const uint64_t q1 = min(a.rows, q0 + rows_staged);
-    for (uint64_t r0 = q0; r0 < q1; r0 += per_warp) {
-      const bool valid = r0 + (lane >> lg) < q1;
-      const uint64_t row = valid ? r0 + (lane >> lg) : q1 - 1;
-      const T* x = rows + (uint32_t)(row - q0) * a.cats;
-      const int64_t token = a.tokens ? token_at(a.tokens, a.token_bytes, row) : -1;
-      Row r;
-      r.load(x, sub, lg, a.cats);
-      const float x_token = is_category(a, token) ? to_f32(x[token]) : 0.0f;
-      short_results<T, E, false>(a, r, row, valid && sub == 0, token, x_token, sub, lg);
+  };
+  for (uint32_t i = 0; i + 1 < STAGES; ++i) fetch(first + i * step, stages[warp][i]);
+  uint32_t buf = 0;
+  for (uint64_t q0 = first; q0 < a.rows; q0 += step) {
+    fetch(q0 + (STAGES - 1) * step, stages[warp][buf == 0 ? STAGES - 1 : buf - 1]);   // the stage that was read last
+    const uint32_t n = (uint32_t)min((uint64_t)rows_staged, a.rows - q0);
+    // 32 rows at a time, so that every lane has one to write
+    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+      const uint32_t mine = i0 + sub * per_warp + group;
+      const int64_t token = a.tokens && mine < n ? token_at(a.tokens, a.token_bytes, q0 + mine) : -1;
+      if (i0 == 0) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        __syncwarp();
+      }
+      const T* rows = reinterpret_cast<const T*>(stages[warp][buf] + ((x0 + q0 * a.cats * sizeof(T)) & 15));
+      Kept kept = {0.0f, 0.0f, 0.0f, 0.0f, 0};
+      for (uint32_t pass = 0; pass < (1u << lg) && i0 + pass * per_warp < n; ++pass) {
+        const uint32_t i = i0 + pass * per_warp + group;
+        Row r;
+        r.load(rows + min(i, n - 1) * a.cats, sub, lg, a.cats);
+        const Kept k = short_row<T, E, false>(a, r, q0 + min(i, n - 1), i < n, sub, lg);
+        if (sub == pass) kept = k;
+      }
+      if (mine < n) short_results<T>(a, kept, q0 + mine, token, is_category(a, token) ? to_f32(rows[mine * a.cats + (uint32_t)token]) : 0.0f);
     }
     __syncwarp();   // everybody has read this stage
+    buf = buf + 1 == STAGES ? 0 : buf + 1;
   }
 }
 
-// Rows of any length, alignment and distance, element by element.
-template <typename T, int E>
-__global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_spread_kernel(LogprobArgs a, uint32_t lg) {
-  using Row = ShortRow<T, E, false>;
-  const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1);
-  const uint64_t step = (uint64_t)gridDim.x * 8 * per_warp;
-  for (uint64_t r0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * per_warp; r0 < a.rows; r0 += step) {
-    const bool valid = r0 + (lane >> lg) < a.rows;
-    const uint64_t row = valid ? r0 + (lane >> lg) : a.rows - 1;
-    const T* x = static_cast<const T*>(a.x) + row * a.stride;
-    const int64_t token = a.tokens ? token_at(a.tokens, a.token_bytes, row) : -1;
-    Row r;
-    r.load(x, sub, lg, a.cats);
-    const float x_token = is_category(a, token) ? to_f32(x[token]) : 0.0f;
-    short_results<T, E, false>(a, r, row, valid && sub == 0, token, x_token, sub, lg);
-  }
-}
-
-enum RowForm { GRANULE_ROWS, STAGED_ROWS, SPREAD_ROWS };
 struct ShortShape {
-  RowForm form;
-  uint32_t lg, each;   // log2 of the lanes per row, elements per lane
+  bool granules, staged;   // rows begin on 16 bytes and end on them; they lie one behind the other
+  uint32_t lg, each;       // log2 of the lanes per row, elements per lane
 };
 // Few lanes per row; four at least where the row has as many granules (64 contiguous bytes per load), sixteen where it
 // is read from memory by elements.
 template <typename T>
 ShortShape short_shape(uint32_t cats, uint64_t stride, const void* x) {
   ShortShape s;
-  s.form = ((reinterpret_cast<uintptr_t>(x) | stride * sizeof(T) | (uint64_t)cats * sizeof(T)) & 15) == 0 ? GRANULE_ROWS
-         : stride == cats ? STAGED_ROWS : SPREAD_ROWS;
-  const uint32_t units = s.form == GRANULE_ROWS ? cats / Vec<T>::N : cats;
-  const uint32_t wanted = s.form == GRANULE_ROWS ? 4 : s.form == STAGED_ROWS ? 1 : 16;
+  s.granules = ((reinterpret_cast<uintptr_t>(x) | stride * sizeof(T) | (uint64_t)cats * sizeof(T)) & 15) == 0;
+  s.staged = stride == cats;
+  const uint32_t units = s.granules ? cats / Vec<T>::N : cats, wanted = s.granules ? 4 : s.staged ? 1 : 16;
   s.lg = 0;
   while (s.lg < 5 && (cats > (Most<T>::E << s.lg) || (1u << s.lg) < (units < wanted ? units : wanted))) ++s.lg;
-  s.each = s.form == GRANULE_ROWS ? ((units + (1u << s.lg) - 1) >> s.lg) * Vec<T>::N : (cats + (1u << s.lg) - 1) >> s.lg;
+  s.each = s.granules ? ((units + (1u << s.lg) - 1) >> s.lg) * Vec<T>::N : (cats + (1u << s.lg) - 1) >> s.lg;
   return s;
 }
 
-// blocks of `kernel` (256 threads) that fill the GPU, at most `needed`
-template <auto kernel>
+// blocks of `kernel` that fill the GPU, at most `needed`
+template <auto kernel, int threads>
 uint32_t resident_blocks(uint32_t sms, uint64_t needed) {
   static std::atomic<int> known[64];   // per device
   int dev = 0, per_sm = 1;
   if (cudaGetDevice(&dev) == cudaSuccess && (per_sm = known[dev & 63].load(std::memory_order_relaxed)) < 1) {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, 256, 0) != cudaSuccess || per_sm < 1) per_sm = 1;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0) != cudaSuccess || per_sm < 1) per_sm = 1;
     known[dev & 63].store(per_sm, std::memory_order_relaxed);
   }
   const uint64_t all = (uint64_t)per_sm * sms;
@@ -789,18 +842,28 @@ uint32_t resident_blocks(uint32_t sms, uint64_t needed) {
 }
 
 template <typename T, int E>
+void launch_staged(const LogprobArgs& a, const ShortShape& s, uint32_t sms, cudaStream_t st) {
+  const uint32_t per_warp = 32u >> s.lg, fit = std::min(2048 / (a.cats * (uint32_t)sizeof(T)), STAGED_ROWS_MOST);
+  // whole passes of 32 rows where they fit, else whole rows of lanes
+  const uint32_t rows = fit >= 32 ? fit / 32 * 32 : fit > per_warp ? fit / per_warp * per_warp : per_warp, per_block = rows * (STAGED_THREADS / 32);
+  const uint32_t grid = resident_blocks<logprob_staged_kernel<T, E>, STAGED_THREADS>(sms, (a.rows + per_block - 1) / per_block);
+  logprob_staged_kernel<T, E><<<grid, STAGED_THREADS, 0, st>>>(a, s.lg, rows);
+}
+template <typename T, int E, bool GRANULES>
+void launch_passes(const LogprobArgs& a, const ShortShape& s, uint32_t sms, cudaStream_t st) {
+  // passes per warp: as many as results can be written together, while the launch is a few times what fits on the GPU
+  const uint32_t per_pass = 256u >> s.lg;
+  uint32_t passes = 1u << s.lg;
+  while (passes > 1 && a.rows < (uint64_t)per_pass * passes * 12 * sms) passes /= 2;
+  const uint64_t blocks = (a.rows + per_pass * passes - 1) / (per_pass * passes);
+  logprob_short_kernel<T, E, GRANULES><<<(uint32_t)std::min<uint64_t>(blocks, 0x7fffffff), 256, 0, st>>>(a, s.lg, passes);
+}
+template <typename T, int E>
 void launch_short_as(const LogprobArgs& a, const ShortShape& s, uint32_t sms, cudaStream_t st) {
-  const uint32_t per_warp = 32u >> s.lg;
-  const auto needed = [&](uint32_t rows_per_warp) { return (a.rows + 8 * rows_per_warp - 1) / (8 * rows_per_warp); };
-  if (s.form == GRANULE_ROWS) {
-    if constexpr (E >= (int)Vec<T>::N)
-      logprob_short_kernel<T, E><<<resident_blocks<logprob_short_kernel<T, E>>(sms, needed(per_warp)), 256, 0, st>>>(a, s.lg);
-  } else if (s.form == STAGED_ROWS) {
-    const uint32_t fit = 2048 / (a.cats * (uint32_t)sizeof(T)), staged = fit > per_warp ? fit / per_warp * per_warp : per_warp;
-    logprob_staged_kernel<T, E><<<resident_blocks<logprob_staged_kernel<T, E>>(sms, needed(staged)), 256, 0, st>>>(a, s.lg, staged);
-  } else {
-    logprob_spread_kernel<T, E><<<resident_blocks<logprob_spread_kernel<T, E>>(sms, needed(per_warp)), 256, 0, st>>>(a, s.lg);
-  }
+  if constexpr (E >= (int)Vec<T>::N)
+    if (s.granules) return launch_passes<T, E, true>(a, s, sms, st);
+  if (s.staged) return launch_staged<T, E>(a, s, sms, st);
+  launch_passes<T, E, false>(a, s, sms, st);
 }
 template <typename T>
 void launch_short(const LogprobArgs& a, uint32_t sms, cudaStream_t st) {
@@ -811,12 +874,12 @@ void launch_short(const LogprobArgs& a, uint32_t sms, cudaStream_t st) {
   else launch_short_as<T, Most<T>::E>(a, s, sms, st);
 }
 
-// The blocks that share a long row: as many as keep the launch within two blocks per SM, and each with a tile of the row at
-// least.
+// The blocks that share a long row: as many as keep the launch within two blocks per SM, and each with a granule of the row
+// per thread at least.
 template <typename T>
 uint32_t row_split(uint64_t rows, uint32_t cats, uint32_t sms) {
   uint32_t split = 1;
-  while (split < MAX_CLUSTER && rows * split * 2 <= 2 * (uint64_t)sms && cats >= split * 2 * ROW_THREADS * Vec<T>::N) split *= 2;
+  while (split < MAX_CLUSTER && rows * split * 2 <= 2 * (uint64_t)sms && cats >= split * 2 * 256 * Vec<T>::N) split *= 2;
   return split;
 }
 
@@ -826,18 +889,29 @@ cudaError_t launch_rows(const LogprobArgs& a, uint32_t sms, cudaStream_t st) {
     launch_short<T>(a, sms, st);
     return cudaGetLastError();
   }
+  const uint32_t grid = (uint32_t)(a.rows < (1u << 24) ? a.rows : 1u << 24);
+  const uint64_t bytes = (uint64_t)a.cats * sizeof(T);
+  // rows of few tiles by one warp or four, where there are enough of them to fill the GPU
+  if (bytes <= 16384 && a.rows >= 16 * (uint64_t)sms) {
+    logprob_row_kernel<T, 32><<<grid, 32, 0, st>>>(a, 1);
+    return cudaGetLastError();
+  }
+  if (bytes <= 65536 && a.rows >= 4 * (uint64_t)sms) {
+    logprob_row_kernel<T, 128><<<grid, 128, 0, st>>>(a, 1);
+    return cudaGetLastError();
+  }
   const uint32_t split = row_split<T>(a.rows, a.cats, sms);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = split;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((uint32_t)(a.rows < (1u << 24) ? a.rows : 1u << 24) * split);
-  cfg.blockDim = dim3(ROW_THREADS);
+  cfg.gridDim = dim3(grid * split);
+  cfg.blockDim = dim3(256);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = split > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, logprob_row_kernel<T>, a, split);
+  return cudaLaunchKernelEx(&cfg, logprob_row_kernel<T, 256>, a, split);
 }
 
 struct LogprobGradArgs {
