@@ -817,10 +817,10 @@ struct ShortShape {
 // Few lanes per row; four at least where the row has as many granules (64 contiguous bytes per load), sixteen where it
 // is read from memory by elements.
 template <typename T>
-ShortShape short_shape(uint32_t cats, uint64_t stride, const void* x) {
+ShortShape short_shape(uint32_t cats, uint64_t stride, const void* x, const void* y = nullptr) {
   ShortShape s;
-  s.granules = ((reinterpret_cast<uintptr_t>(x) | stride * sizeof(T) | (uint64_t)cats * sizeof(T)) & 15) == 0;
-  s.staged = stride == cats;
+  s.granules = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | stride * sizeof(T) | (uint64_t)cats * sizeof(T)) & 15) == 0;
+  s.staged = stride == cats && (!y || ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0);
   const uint32_t units = s.granules ? cats / Vec<T>::N : cats, wanted = s.granules ? 4 : s.staged ? 1 : 16;
   s.lg = 0;
   while (s.lg < 5 && (cats > (Most<T>::E << s.lg) || (1u << s.lg) < (units < wanted ? units : wanted))) ++s.lg;
@@ -841,11 +841,15 @@ uint32_t resident_blocks(uint32_t sms, uint64_t needed) {
   return (uint32_t)(needed < all ? needed : all);
 }
 
+// rows per stage: whole passes of 32 rows where they fit, else whole rows of lanes
+template <typename T>
+uint32_t staged_rows(uint32_t cats, uint32_t lg) {
+  const uint32_t per_warp = 32u >> lg, fit = std::min(2048 / (cats * (uint32_t)sizeof(T)), STAGED_ROWS_MOST);
+  return fit >= 32 ? fit / 32 * 32 : fit > per_warp ? fit / per_warp * per_warp : per_warp;
+}
 template <typename T, int E>
 void launch_staged(const LogprobArgs& a, const ShortShape& s, uint32_t sms, cudaStream_t st) {
-  const uint32_t per_warp = 32u >> s.lg, fit = std::min(2048 / (a.cats * (uint32_t)sizeof(T)), STAGED_ROWS_MOST);
-  // whole passes of 32 rows where they fit, else whole rows of lanes
-  const uint32_t rows = fit >= 32 ? fit / 32 * 32 : fit > per_warp ? fit / per_warp * per_warp : per_warp, per_block = rows * (STAGED_THREADS / 32);
+  const uint32_t rows = staged_rows<T>(a.cats, s.lg), per_block = rows * (STAGED_THREADS / 32);
   const uint32_t grid = resident_blocks<logprob_staged_kernel<T, E>, STAGED_THREADS>(sms, (a.rows + per_block - 1) / per_block);
   logprob_staged_kernel<T, E><<<grid, STAGED_THREADS, 0, st>>>(a, s.lg, rows);
 }
@@ -957,7 +961,7 @@ __device__ __forceinline__ float grad_of(const RowGrad& g, float x) {
   return ex2_ftz(d) * fmaf(g.beta, d, g.alpha);
 }
 __device__ __forceinline__ bool no_mass(const RowGrad& g) { return g.S == 0.0f; }
-// the whole gradient of an element that the token or an alternative may point to
+// the whole gradient of an element that the token or an alternative points to
 __device__ __forceinline__ float pointed_grad(const LogprobGradArgs& a, const RowGrad& g, uint64_t row, uint32_t j, float x) {
   if (no_mass(g)) return 0.0f;
   float v = grad_of(g, x);
@@ -967,15 +971,259 @@ __device__ __forceinline__ float pointed_grad(const LogprobGradArgs& a, const Ro
       if (a.top_ids[row * a.top_k + k] == (int64_t)j) v += a.g_top[row * a.top_k + k] * a.invT;
   return v;
 }
+// p_j (alpha + beta d) of W words, as words
+template <typename T, int W>
+__device__ __forceinline__ void grad_words(const uint32_t* w, const RowGrad& g, uint32_t* out) {
+  constexpr int E = W * (int)PER_WORD<T>;
+  const float alpha = no_mass(g) ? 0.0f : g.alpha, beta = no_mass(g) ? 0.0f : g.beta;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) {
+    float2 d;
+    if (g.from.near) {
+      float2 x;
+      if constexpr (sizeof(T) == 4) x = {max_nan(__uint_as_float(w[e]), Word<T>::FLOOR), max_nan(__uint_as_float(w[e + 1]), Word<T>::FLOOR)};
+      else x = Word<T>::floats(Word<T>::raised(w[e / 2]));
+      d = fma2(x, {g.from.c, g.from.c}, {-g.from.mc, -g.from.mc});
+    } else {
+      const float2 x = pair_of<T>(w, e);
+      const float m = finite_shift(g.from.m);
+      d = {max_nan((x.x - m) * g.from.c, NO_MASS), max_nan((x.y - m) * g.from.c, NO_MASS)};
+    }
+    const float2 v = mul2({ex2_ftz(d.x), ex2_ftz(d.y)}, fma2({beta, beta}, d, {alpha, alpha}));
+    if constexpr (sizeof(T) == 4) {
+      out[e] = __float_as_uint(v.x);
+      out[e + 1] = __float_as_uint(v.y);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      out[e / 2] = Word<T>::bits(__floats2half2_rn(v.x, v.y));
+    } else {
+      out[e / 2] = Word<T>::bits(__floats2bfloat162_rn(v.x, v.y));
+    }
+  }
+}
 
+// A block takes GRAD_TILE bytes of a row: 64 per thread.  Granules are those of dx; x is read in them where it lies alike
+// towards 16-byte boundaries, by elements otherwise.  What the token and the alternatives point to is written again at the
+// end.  The last rows come first: the forward pass read them last, and some of them are still in the L2 cache.
+constexpr uint32_t GRAD_THREADS = 256, GRAD_TILE = 64 * GRAD_THREADS;
 template <typename T>
-__global__ void __launch_bounds__(256) logprob_grad_kernel(LogprobGradArgs a) {
-  for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+__global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(LogprobGradArgs a, uint32_t chunks) {
+  constexpr uint32_t N = Vec<T>::N, STEP = GRAD_TILE / 16;
+  const uint32_t tid = threadIdx.x;
+  for (uint64_t i = blockIdx.x; i < a.rows * chunks; i += gridDim.x) {
+    const uint64_t row = a.rows - 1 - i / chunks;
+    const uint32_t chunk = (uint32_t)(i % chunks);
     const T* x = static_cast<const T*>(a.x) + row * a.stride;
     T* dx = static_cast<T*>(a.dx) + row * a.cats;
+    Part<T> p;   // of dx
+    p.off = (uint32_t)((reinterpret_cast<uintptr_t>(dx) & 15) / sizeof(T));
+    p.base = dx - p.off;
+    p.end = p.off + a.cats;
+    const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
+    const uint32_t g0 = chunk * STEP, g1 = min((uint32_t)(((uint64_t)p.end + N - 1) / N), g0 + STEP);
+    const T* xs = x - p.off;   // x's element for place j of the granules
+    uint32_t w[4][4];
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t at = g0 + u * GRAD_THREADS + tid;
+      if (at >= g1) continue;
+      if (alike && p.whole(at)) {
+        const uint4 q = load16(xs + (size_t)at * N);
+        w[u][0] = q.x; w[u][1] = q.y; w[u][2] = q.z; w[u][3] = q.w;
+      } else {
+#pragma unroll
+        for (uint32_t v = 0; v < N; v += PER_WORD<T>) {
+          uint32_t word = 0;
+#pragma unroll
+          for (uint32_t h = 0; h < PER_WORD<T>; ++h) {
+            const uint32_t j = at * N + v + h;
+            if (j < p.off || j >= p.end) continue;
+            if constexpr (sizeof(T) == 4) word = reinterpret_cast<const uint32_t*>(xs)[j];
+            else word |= (uint32_t)reinterpret_cast<const uint16_t*>(xs)[j] << (16 * h);
+          }
+          w[u][v / PER_WORD<T>] = word;
+        }
+      }
+    }
     const RowGrad g = row_grad<T>(a, row);
-    for (uint32_t j = threadIdx.x; j < a.cats; j += blockDim.x) dx[j] = from_f32<T>(pointed_grad(a, g, row, j, to_f32(x[j])));
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t at = g0 + u * GRAD_THREADS + tid;
+      if (at >= g1) continue;
+      uint32_t out[4];
+      grad_words<T, 4>(w[u], g, out);
+      T* to = const_cast<T*>(p.base) + (size_t)at * N;
+      if (p.whole(at)) {
+        *reinterpret_cast<uint4*>(to) = {out[0], out[1], out[2], out[3]};
+      } else {
+#pragma unroll
+        for (uint32_t v = 0; v < N; ++v)
+          if (at * N + v >= p.off && at * N + v < p.end) {
+            if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(to)[v] = out[v];
+            else reinterpret_cast<uint16_t*>(to)[v] = (uint16_t)(out[v / 2] >> (16 * (v & 1)));
+          }
+      }
+    }
+    if (g.token >= 0 || a.g_top) {
+      __syncthreads();
+      const uint32_t first = max(g0 * N, p.off) - p.off, last = min(g1 * N, p.end) - p.off;   // the chunk's categories
+      if (tid <= (a.g_top ? a.top_k : 0)) {
+        const int64_t j = tid == 0 ? g.token : a.top_ids[row * a.top_k + tid - 1];
+        if (j >= (int64_t)first && j < (int64_t)last) dx[j] = from_f32<T>(pointed_grad(a, g, row, (uint32_t)j, to_f32(x[j])));
+      }
+    }
+    __syncthreads();
   }
+}
+
+// Short rows, 2^lg lanes each, as in logprob_short_kernel.
+template <typename T, int E, bool GRANULES>
+__global__ void __launch_bounds__(256, E >= 32 ? 3 : E >= 16 ? 4 : 6) logprob_grad_short_kernel(LogprobGradArgs a, uint32_t lg) {
+  using Row = ShortRow<T, E, GRANULES>;
+  const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1);
+  const uint64_t warps = (a.rows + per_warp - 1) / per_warp, step = (uint64_t)gridDim.x * 8;
+  for (uint64_t i = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < warps; i += step) {
+    const uint64_t r0 = (warps - 1 - i) * per_warp, mine = r0 + (lane >> lg), row = min(a.rows - 1, mine);   // the last rows first
+    const T* x = static_cast<const T*>(a.x) + row * a.stride;
+    T* dx = static_cast<T*>(a.dx) + row * a.cats;
+    Row r;
+    r.load(x, sub, lg, a.cats);
+    const RowGrad g = row_grad<T>(a, row);
+    uint32_t out[Row::W];
+    grad_words<T, Row::W>(r.w, g, out);
+    if (mine < a.rows) {
+      if constexpr (GRANULES) {
+#pragma unroll
+        for (int n = 0; n < Row::W / 4; ++n) {
+          const uint32_t at = (sub + ((uint32_t)n << lg)) * Row::N;
+          if (at < a.cats) *reinterpret_cast<uint4*>(dx + at) = {out[4 * n], out[4 * n + 1], out[4 * n + 2], out[4 * n + 3]};
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const uint32_t j = Row::index(e, sub, lg);
+          if (j >= a.cats) continue;
+          if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(dx)[j] = out[e];
+          else reinterpret_cast<uint16_t*>(dx)[j] = (uint16_t)(out[e / 2] >> (16 * (e & 1)));
+        }
+      }
+    }
+    if (a.g_logp || a.g_top) {
+      __syncwarp();   // the lanes' stores come before these
+      const uint32_t n = a.g_top ? a.top_k + 1 : 1;
+      for (uint32_t k = sub; k < n; k += 1u << lg) {
+        const int64_t j = k == 0 ? g.token : a.top_ids[row * a.top_k + k - 1];
+        if (mine < a.rows && j >= 0 && j < (int64_t)a.cats) dx[j] = from_f32<T>(pointed_grad(a, g, row, (uint32_t)j, to_f32(x[j])));
+      }
+    }
+  }
+}
+
+// Short rows one behind the other, of any length, staged as in logprob_staged_kernel: the gradient takes the place of the
+// logits in shared memory and leaves in granules, but for those that the stage shares with its neighbours.
+template <typename T, int E>
+__global__ void __launch_bounds__(STAGED_THREADS, 6) logprob_grad_staged_kernel(LogprobGradArgs a, uint32_t lg, uint32_t rows_staged) {
+  using Row = ShortRow<T, E, false>;
+  constexpr uint32_t WARPS = STAGED_THREADS / 32;
+  __shared__ __align__(16) uint8_t stages[WARPS][STAGE_BYTES];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1), group = lane >> lg;
+  const uint64_t all = (a.rows + rows_staged - 1) / rows_staged, step = (uint64_t)gridDim.x * WARPS;
+  uint8_t* stage = stages[warp];
+  for (uint64_t i = (uint64_t)blockIdx.x * WARPS + warp; i < all; i += step) {
+    const uint64_t q0 = (all - 1 - i) * rows_staged;   // the last rows first
+    const uint32_t n = (uint32_t)min((uint64_t)rows_staged, a.rows - q0);
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(a.x) + q0 * a.cats * sizeof(T), hi = lo + (uintptr_t)n * a.cats * sizeof(T);
+    const intptr_t to = reinterpret_cast<uintptr_t>(a.dx) - reinterpret_cast<uintptr_t>(a.x);   // a multiple of 16
+    for (uint32_t k = 16 * lane; (lo & ~(uintptr_t)15) + k < hi; k += 512) {
+      const uintptr_t at = (lo & ~(uintptr_t)15) + k;
+      if (at >= lo && at + 16 <= hi) {
+        *reinterpret_cast<uint4*>(stage + k) = load16(reinterpret_cast<const void*>(at));
+      } else {
+        for (uint32_t e = 0; e < 16; e += sizeof(T))
+          if (at + e >= lo && at + e < hi) *reinterpret_cast<T*>(stage + k + e) = *reinterpret_cast<const T*>(at + e);
+      }
+    }
+    __syncwarp();
+    T* rows = reinterpret_cast<T*>(stage + (lo & 15));
+    for (uint32_t i0 = 0; i0 < n; i0 += per_warp) {
+      const bool valid = i0 + group < n;
+      const uint32_t r = valid ? i0 + group : n - 1;
+      const uint64_t row = q0 + r;
+      T* x = rows + r * a.cats;
+      Row in;
+      in.load(x, sub, lg, a.cats);
+      const RowGrad g = row_grad<T>(a, row);
+      uint32_t out[Row::W];
+      grad_words<T, Row::W>(in.w, g, out);
+      // what is pointed to, from the logits, before they are gone
+      const uint32_t most = a.g_top ? a.top_k + 1 : a.g_logp ? 1 : 0;
+      for (uint32_t k0 = 0; k0 < most || k0 == 0; k0 += 1u << lg) {
+        const uint32_t k = k0 + sub;
+        int64_t j = -1;
+        T value = from_f32<T>(0.0f);
+        if (valid && k < most) {
+          j = k == 0 ? g.token : a.top_ids[row * a.top_k + k - 1];
+          if (j < 0 || j >= (int64_t)a.cats) j = -1;
+          else if (k0 == 0) value = from_f32<T>(pointed_grad(a, g, row, (uint32_t)j, to_f32(x[j])));
+          else value = from_f32<T>(pointed_grad(a, g, row, (uint32_t)j, to_f32(static_cast<const T*>(a.x)[row * a.cats + (uint32_t)j])));
+        }
+        __syncwarp();   // everybody has read the row
+        if (k0 == 0 && valid) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const uint32_t c = Row::index(e, sub, lg);
+            if (c >= a.cats) continue;
+            if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(x)[c] = out[e];
+            else reinterpret_cast<uint16_t*>(x)[c] = (uint16_t)(out[e / 2] >> (16 * (e & 1)));
+          }
+        }
+        __syncwarp();
+        if (j >= 0) x[j] = value;
+        __syncwarp();
+      }
+    }
+    for (uint32_t k = 16 * lane; (lo & ~(uintptr_t)15) + k < hi; k += 512) {
+      const uintptr_t at = (lo & ~(uintptr_t)15) + k;
+      if (at >= lo && at + 16 <= hi) {
+        *reinterpret_cast<uint4*>(at + to) = *reinterpret_cast<const uint4*>(stage + k);
+      } else {
+        for (uint32_t e = 0; e < 16; e += sizeof(T))
+          if (at + e >= lo && at + e < hi) *reinterpret_cast<T*>(at + e + to) = *reinterpret_cast<const T*>(stage + k + e);
+      }
+    }
+    __syncwarp();
+  }
+}
+
+template <typename T, int E>
+void launch_grad_short_as(const LogprobGradArgs& a, const ShortShape& s, cudaStream_t st) {
+  const uint32_t lg = s.lg;
+  if (s.staged && !s.granules) {
+    const uint32_t rows = staged_rows<T>(a.cats, lg), per_block = rows * (STAGED_THREADS / 32);
+    const uint64_t n = (a.rows + per_block - 1) / per_block;
+    logprob_grad_staged_kernel<T, E><<<(uint32_t)std::min<uint64_t>(n, 0x7fffffff), STAGED_THREADS, 0, st>>>(a, lg, rows);
+    return;
+  }
+  const uint64_t blocks = (a.rows + (256u >> lg) - 1) / (256u >> lg);
+  const uint32_t grid = (uint32_t)std::min<uint64_t>(blocks, 0x7fffffff);
+  if constexpr (E >= (int)Vec<T>::N)
+    if (s.granules) {
+      logprob_grad_short_kernel<T, E, true><<<grid, 256, 0, st>>>(a, lg);
+      return;
+    }
+  logprob_grad_short_kernel<T, E, false><<<grid, 256, 0, st>>>(a, lg);
+}
+template <typename T>
+void launch_grad(const LogprobGradArgs& a, cudaStream_t st) {
+  if (a.cats <= 32 * Most<T>::E) {
+    const ShortShape s = short_shape<T>(a.cats, a.stride, a.x, a.dx);
+    if (s.each <= 4) launch_grad_short_as<T, 4>(a, s, st);
+    else if (s.each <= 8) launch_grad_short_as<T, 8>(a, s, st);
+    else if (s.each <= 16) launch_grad_short_as<T, 16>(a, s, st);
+    else launch_grad_short_as<T, Most<T>::E>(a, s, st);
+    return;
+  }
+  const uint32_t chunks = (uint32_t)(((uint64_t)a.cats + 2 * Vec<T>::N) * sizeof(T) / GRAD_TILE + 1);
+  logprob_grad_kernel<T><<<(uint32_t)std::min<uint64_t>(a.rows * chunks, 0x7fffffff), GRAD_THREADS, 0, st>>>(a, chunks);
 }
 
 struct EvidenceArgs {
@@ -989,55 +1237,319 @@ struct EvidenceArgs {
   void* dx;
 };
 
-// One warp per (row, variable).
+// ---- soft evidence -----------------------------------------------------------------------------------------------------
+// Logits have the category fastest, evidence the row: a block transposes a tile of 32 rows and up to `cap` columns (the
+// categories of one variable, or of several short ones, which lie one behind the other) through shared memory in fp32.
+// Rows come and go in granules; from there on a lane is a row: it walks the categories of its (variable, part), so that
+// maxima and sums need no shuffles and every access to evidence moves 32 neighbouring rows, 128 bytes.  Element (column,
+// row) lies at column * 32 + (row + column / N) % 32 (granules of N; N = 1 where rows are read by elements): free of bank
+// conflicts both ways.  A distribution of more than `cap` categories passes twice, in chunks: once for its sum, once for its values.
+constexpr uint32_t EV_THREADS = 256, EV_WARPS = 8, EV_COLUMNS = 256;
+
+struct EvidenceTile {
+  uint32_t cap;         // columns of a tile
+  uint32_t vars;        // variables per tile (1 where a variable has more than cap categories)
+  uint32_t row_tiles;
+  bool granules;        // rows of a tile begin on 16 bytes
+};
+struct EvidenceJoin { float m[EV_WARPS][32], S[EV_WARPS][32]; };
+
 template <typename T>
-__global__ void __launch_bounds__(256) evidence_kernel(EvidenceArgs a) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t total = a.rows * a.vars;
-  for (uint64_t i = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; i < total; i += (uint64_t)gridDim.x * 8) {
-    const uint64_t b = i % a.rows;
-    const uint32_t v = (uint32_t)(i / a.rows);
-    const T* x = static_cast<const T*>(a.x) + b * a.row_stride + v * a.var_stride;
-    float* out = a.out + b + a.rows * v;
-    const uint64_t step = a.rows * a.vars;
-    const bool missing = a.miss && a.miss[b * a.miss_row_stride + v * a.miss_var_stride];
-    float m = -INFINITY, S = 0.0f;
-    for (uint32_t j = lane; j < a.cats; j += 32) m = fmaxf(m, to_f32(x[j]));
-    m = over_lanes(m, 5, most_of);
-    const Shift from = shift_of<T>(m, a.c);
-    for (uint32_t j = lane; j < a.cats; j += 32) S += m == -INFINITY && x[j] == x[j] ? 0.0f : ex2_ftz(scaled(from, to_f32(x[j])));
-    S = over_lanes(S, 5, sum_of);
-    const float lnS = ln_of(S);
-    for (uint32_t j = lane; j < a.cats; j += 32) out[j * step] = missing ? 0.0f : logp_of(to_f32(x[j]), from, lnS);
-    if (a.stats_out && lane == 0) {
-      a.stats_out[2 * (b * a.vars + v)] = m;
-      a.stats_out[2 * (b * a.vars + v) + 1] = S;
+struct EvidenceLayout {
+  static constexpr uint32_t LOG_N = sizeof(T) == 4 ? 2 : 3;
+  uint32_t log_n;   // 0 without granules
+  __device__ __forceinline__ uint32_t at(uint32_t column, uint32_t row) const { return column * 32 + ((row + (column >> log_n)) & 31); }
+};
+
+// `columns` columns of 32 rows, the first of them at x: into the tile, in fp32
+template <typename T>
+__device__ __forceinline__ void load_tile(float* tile, EvidenceLayout<T> lay, const T* x, uint64_t row_stride, uint32_t rows, uint32_t columns) {
+  constexpr uint32_t N = Vec<T>::N;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lay.log_n) {
+    for (uint32_t g = lane; g * N < columns; g += 32) {
+      uint4 q[4];
+      const bool whole = (g + 1) * N <= columns;
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t r = warp + EV_WARPS * i;
+        if (whole && r < rows) q[i] = load16(x + r * row_stride + g * N);
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t r = warp + EV_WARPS * i;
+        if (r >= rows) continue;
+        if (whole) {
+          const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+          for (uint32_t v = 0; v < N; ++v) tile[lay.at(g * N + v, r)] = element_of<T>(w, v);
+        } else {
+          for (uint32_t j = g * N; j < columns; ++j) tile[lay.at(j, r)] = to_f32(x[r * row_stride + j]);
+        }
+      }
+    }
+  } else {
+    for (uint32_t j = lane; j < columns; j += 32) {
+      float f[4];
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t r = warp + EV_WARPS * i;
+        f[i] = r < rows ? to_f32(x[r * row_stride + j]) : 0.0f;
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) tile[lay.at(j, warp + EV_WARPS * i)] = f[i];
     }
   }
 }
 
+// maximum and sum of the powers of columns [c0, c1) of a row, added to (m, S)
 template <typename T>
-__global__ void __launch_bounds__(256) evidence_grad_kernel(EvidenceArgs a) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t total = a.rows * a.vars;
-  for (uint64_t i = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; i < total; i += (uint64_t)gridDim.x * 8) {
-    const uint64_t b = i % a.rows;
-    const uint32_t v = (uint32_t)(i / a.rows);
-    const T* x = static_cast<const T*>(a.x) + b * a.row_stride + v * a.var_stride;
-    const float* g = a.g + b + a.rows * v;
-    T* dx = static_cast<T*>(a.dx) + (b * a.vars + v) * a.cats;
-    const uint64_t step = a.rows * a.vars;
-    const Shift from = shift_of<T>(a.stats[2 * (b * a.vars + v)], a.c);
-    const float S = a.stats[2 * (b * a.vars + v) + 1];
-    const bool none = (a.miss && a.miss[b * a.miss_row_stride + v * a.miss_var_stride]) || S == 0.0f;
-    float sum = 0.0f;
-    for (uint32_t j = lane; j < a.cats; j += 32) sum += g[j * step];
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    for (uint32_t j = lane; j < a.cats; j += 32) {
-      const float e = ex2_ftz(scaled(from, to_f32(x[j])));
-      dx[j] = from_f32<T>(none ? 0.0f : (g[j * step] - e * (sum / S)) * a.invT);
+__device__ __forceinline__ void add_columns(const float* tile, EvidenceLayout<T> lay, uint32_t c0, uint32_t c1, uint32_t row, float c, float& m, float& S) {
+  constexpr uint32_t RUN = 8;
+  for (uint32_t j = c0; j < c1; j += RUN) {
+    float x[RUN], most = -INFINITY;
+#pragma unroll
+    for (uint32_t i = 0; i < RUN; ++i) x[i] = j + i < c1 ? tile[lay.at(j + i, row)] : -INFINITY;
+#pragma unroll
+    for (uint32_t i = 0; i < RUN; ++i) most = fmaxf(most, x[i]);
+    if (most > m) {
+      if (m != -INFINITY) S *= ex2_ftz(between(shift_of<T>(m, c), shift_of<T>(most, c)));
+      m = most;
+    }
+    const Shift s = shift_of<T>(m, c);
+    if (s.near) {
+#pragma unroll
+      for (uint32_t i = 0; i < RUN; ++i) S += ex2_ftz(fmaf(x[i], s.c, -s.mc));
+    } else {
+      const float from = finite_shift(m);
+#pragma unroll
+      for (uint32_t i = 0; i < RUN; ++i) S += ex2_ftz(max_nan((x[i] - from) * c, NO_MASS));
     }
   }
+}
+template <typename T>
+__device__ __forceinline__ void join_columns(const EvidenceJoin& join, uint32_t first, uint32_t parts, uint32_t row, float c, float& m, float& S) {
+  m = -INFINITY;
+  for (uint32_t i = 0; i < parts; ++i) m = fmaxf(m, join.m[first + i][row]);
+  const Shift to = shift_of<T>(m, c);
+  S = 0.0f;
+  for (uint32_t i = 0; i < parts; ++i) {
+    const float mi = join.m[first + i][row];
+    S += join.S[first + i][row] * (mi == -INFINITY || mi == m ? 1.0f : ex2_ftz(between(shift_of<T>(mi, c), to)));
+  }
+}
+
+// What a warp works on: variable `v` of the tile and part `part` of its categories (all, where a tile has eight variables).
+struct EvidenceUnits {
+  uint32_t parts, units;
+  __device__ __forceinline__ explicit EvidenceUnits(uint32_t vars) : parts(vars >= EV_WARPS ? 1 : EV_WARPS / vars), units(vars * parts) {}
+  __device__ __forceinline__ uint32_t var(uint32_t u) const { return u / parts; }
+  __device__ __forceinline__ uint32_t begin(uint32_t u, uint32_t columns) const { return (uint32_t)((uint64_t)(u % parts) * columns / parts); }
+  __device__ __forceinline__ uint32_t end(uint32_t u, uint32_t columns) const { return (uint32_t)((uint64_t)(u % parts + 1) * columns / parts); }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(EV_THREADS, 4) evidence_kernel(EvidenceArgs a, EvidenceTile et) {
+  extern __shared__ __align__(16) float tile[];
+  __shared__ EvidenceJoin join;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const EvidenceLayout<T> lay{et.granules ? EvidenceLayout<T>::LOG_N : 0};
+  const uint64_t tiles = (uint64_t)et.row_tiles * ((a.vars + et.vars - 1) / et.vars);
+  for (uint64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
+    const uint64_t b0 = i % et.row_tiles * 32, b = b0 + lane;   // neighbouring blocks write neighbouring rows
+    const uint32_t v0 = (uint32_t)(i / et.row_tiles) * et.vars, nv = min(et.vars, a.vars - v0);
+    const uint32_t rows = (uint32_t)min((uint64_t)32, a.rows - b0), width = min(a.cats, et.cap);   // categories of a pass
+    const bool one = width == a.cats;
+    const T* x = static_cast<const T*>(a.x) + b0 * a.row_stride + (uint64_t)v0 * a.var_stride;
+    const EvidenceUnits un(nv);
+    float m = -INFINITY, S = 0.0f;   // of the one unit that a warp has where parts > 1
+    for (uint32_t c0 = 0; c0 < a.cats; c0 += width) {
+      const uint32_t n = min(width, a.cats - c0);
+      load_tile<T>(tile, lay, x + c0, a.row_stride, rows, one ? nv * a.cats : n);
+      __syncthreads();
+      if (un.parts > 1 && warp < un.units && lane < rows) add_columns<T>(tile, lay, un.var(warp) * a.cats + un.begin(warp, n), un.var(warp) * a.cats + un.end(warp, n), lane, a.c, m, S);
+      if (!one) __syncthreads();
+    }
+    if (un.parts > 1) {
+      join.m[warp][lane] = m;
+      join.S[warp][lane] = S;
+      __syncthreads();
+    }
+    for (uint32_t c0 = 0; c0 < a.cats; c0 += width) {
+      const uint32_t n = min(width, a.cats - c0);
+      if (!one) {
+        load_tile<T>(tile, lay, x + c0, a.row_stride, rows, n);
+        __syncthreads();
+      }
+      for (uint32_t u = warp; u < un.units; u += EV_WARPS) {
+        if (lane >= rows) continue;
+        const uint32_t v = v0 + un.var(u), first = un.var(u) * a.cats;
+        if (un.parts > 1) {
+          join_columns<T>(join, u - u % un.parts, un.parts, lane, a.c, m, S);
+        } else {
+          m = -INFINITY;
+          S = 0.0f;
+          add_columns<T>(tile, lay, first, first + n, lane, a.c, m, S);
+        }
+        const Shift from = shift_of<T>(m, a.c);
+        const float lnS = ln_of(S);
+        const bool missing = a.miss && a.miss[b * a.miss_row_stride + v * a.miss_var_stride];
+        if (a.stats_out && c0 == 0 && u % un.parts == 0) reinterpret_cast<float2*>(a.stats_out)[b * a.vars + v] = {m, S};
+        const uint32_t j1 = un.end(u, n);
+        float* out = a.out + b + a.rows * (v + (uint64_t)a.vars * (c0 + un.begin(u, n)));
+        const uint64_t step = a.rows * a.vars;
+#pragma unroll 4
+        for (uint32_t j = un.begin(u, n); j < j1; ++j, out += step) {
+          const float xj = tile[lay.at(first + j, lane)];
+          float value = fmaf(fmaf(xj, from.c, -from.mc), LN2, -lnS);   // near, and no mask's value: all but a few
+          if (!from.near || value < -1e30f) value = logp_of(xj, from, lnS);
+          *out = missing ? 0.0f : value;
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// columns of a tile back to rows at dx, in T
+template <typename T>
+__device__ __forceinline__ void store_tile(const float* tile, EvidenceLayout<T> lay, T* dx, uint64_t row_stride, uint32_t rows, uint32_t columns) {
+  constexpr uint32_t N = Vec<T>::N;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (uint32_t r = warp; r < rows; r += EV_WARPS) {
+    T* to = dx + r * row_stride;
+    if (lay.log_n) {
+      for (uint32_t g = lane; g * N < columns; g += 32) {
+        if ((g + 1) * N <= columns) {
+          uint32_t w[4];
+#pragma unroll
+          for (uint32_t v = 0; v < N; v += PER_WORD<T>) {
+            const float f = tile[lay.at(g * N + v, r)];
+            if constexpr (sizeof(T) == 4) w[v] = __float_as_uint(f);
+            else if constexpr (std::is_same<T, __half>::value) w[v / 2] = Word<T>::bits(__floats2half2_rn(f, tile[lay.at(g * N + v + 1, r)]));
+            else w[v / 2] = Word<T>::bits(__floats2bfloat162_rn(f, tile[lay.at(g * N + v + 1, r)]));
+          }
+          *reinterpret_cast<uint4*>(to + g * N) = {w[0], w[1], w[2], w[3]};
+        } else {
+          for (uint32_t j = g * N; j < columns; ++j) to[j] = from_f32<T>(tile[lay.at(j, r)]);
+        }
+      }
+    } else {
+      for (uint32_t j = lane; j < columns; j += 32) to[j] = from_f32<T>(tile[lay.at(j, r)]);
+    }
+  }
+}
+
+// dx_c = (g_c - p_c sum g) / T: the sum needs g alone; g waits in a second tile where the distribution fits into one.
+template <typename T>
+__global__ void __launch_bounds__(EV_THREADS, 3) evidence_grad_kernel(EvidenceArgs a, EvidenceTile et) {
+  extern __shared__ __align__(16) float tile[];
+  __shared__ EvidenceJoin join;
+  float* g_tile = tile + et.cap * 32;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const EvidenceLayout<T> lay{et.granules ? EvidenceLayout<T>::LOG_N : 0};
+  const uint64_t tiles = (uint64_t)et.row_tiles * ((a.vars + et.vars - 1) / et.vars), step = a.rows * a.vars;
+  for (uint64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
+    const uint64_t b0 = i % et.row_tiles * 32, b = b0 + lane;
+    const uint32_t v0 = (uint32_t)(i / et.row_tiles) * et.vars, nv = min(et.vars, a.vars - v0);
+    const uint32_t rows = (uint32_t)min((uint64_t)32, a.rows - b0), width = min(a.cats, et.cap);
+    const bool one = width == a.cats;
+    const T* x = static_cast<const T*>(a.x) + b0 * a.row_stride + (uint64_t)v0 * a.var_stride;
+    T* dx = static_cast<T*>(a.dx) + (b0 * a.vars + v0) * a.cats;
+    const EvidenceUnits un(nv);
+    if (one) load_tile<T>(tile, lay, x, a.row_stride, rows, nv * a.cats);
+    for (uint32_t u = warp; u < un.units; u += EV_WARPS) {
+      if (lane >= rows) continue;
+      const uint32_t v = v0 + un.var(u), first = un.var(u) * a.cats;
+      const float* g = a.g + b + a.rows * v;
+      const uint32_t j0 = un.begin(u, a.cats), j1 = un.end(u, a.cats);
+      float sum = 0.0f;
+#pragma unroll 8
+      for (uint32_t j = j0; j < j1; ++j) {
+        const float gj = g[step * j];
+        sum += gj;
+        if (one) g_tile[(first + j) * 32 + lane] = gj;
+      }
+      if (un.parts > 1) join.S[u][lane] = sum;
+      else g_tile[first * 32 + lane + 32 * et.cap] = sum;   // behind the tile: one sum per variable and row
+    }
+    __syncthreads();
+    for (uint32_t c0 = 0; c0 < a.cats; c0 += width) {
+      const uint32_t n = min(width, a.cats - c0);
+      if (!one) {
+        load_tile<T>(tile, lay, x + c0, a.row_stride, rows, n);
+        __syncthreads();
+      }
+      for (uint32_t u = warp; u < un.units; u += EV_WARPS) {
+        if (lane >= rows) continue;
+        const uint32_t v = v0 + un.var(u), first = un.var(u) * a.cats;
+        float sum = 0.0f;
+        if (un.parts > 1)
+          for (uint32_t k = 0; k < un.parts; ++k) sum += join.S[u - u % un.parts + k][lane];
+        else sum = g_tile[first * 32 + lane + 32 * et.cap];
+        const float2 st = reinterpret_cast<const float2*>(a.stats)[b * a.vars + v];
+        const Shift from = shift_of<T>(st.x, a.c);
+        const bool none = st.y == 0.0f || (a.miss && a.miss[b * a.miss_row_stride + v * a.miss_var_stride]);
+        const float k = sum / st.y;
+        const float* g = a.g + b + a.rows * v + step * c0;
+        const uint32_t j1 = un.end(u, n);
+#pragma unroll 4
+        for (uint32_t j = un.begin(u, n); j < j1; ++j) {
+          const uint32_t at = lay.at(first + j, lane);
+          const float gj = one ? g_tile[(first + j) * 32 + lane] : g[step * j];
+          tile[at] = none ? 0.0f : (gj - ex2_ftz(scaled(from, tile[at])) * k) * a.invT;
+        }
+      }
+      __syncthreads();
+      store_tile<T>(tile, lay, dx + c0, (uint64_t)a.vars * a.cats, rows, one ? nv * a.cats : n);
+      __syncthreads();
+    }
+  }
+}
+
+// Tiles of up to EV_COLUMNS columns; a variable of up to `most` categories is held whole.
+template <typename T>
+EvidenceTile evidence_tile(const EvidenceArgs& a, uint32_t most) {
+  EvidenceTile t;
+  const uint32_t n = Vec<T>::N;
+  t.vars = 1;
+  if (a.var_stride == a.cats && a.cats <= EV_COLUMNS / 2) {   // variables one behind the other
+    t.vars = EV_COLUMNS / a.cats;
+    while (t.vars > 1 && t.vars * a.cats % n) --t.vars;   // whole granules per tile where there is such a number
+    if (t.vars * a.cats % n) t.vars = EV_COLUMNS / a.cats;
+  }
+  if (t.vars > a.vars) t.vars = a.vars;
+  t.cap = t.vars > 1 ? t.vars * a.cats : a.cats <= most ? a.cats : EV_COLUMNS;
+  t.row_tiles = (uint32_t)((a.rows + 31) / 32);
+  // where rows of tiles begin: of x, and of dx, which is contiguous
+  const bool several = t.vars < a.vars;
+  uint64_t at = reinterpret_cast<uintptr_t>(a.x) | a.row_stride * sizeof(T) | (several ? t.vars * a.var_stride * sizeof(T) : 0);
+  if (a.dx) at |= reinterpret_cast<uintptr_t>(a.dx) | (uint64_t)a.vars * a.cats * sizeof(T) | (several ? (uint64_t)t.vars * a.cats * sizeof(T) : 0);
+  t.granules = (at & 15) == 0;
+  return t;
+}
+
+template <typename T>
+cudaError_t launch_evidence(const EvidenceArgs& a, cudaStream_t st) {
+  static PcbPerDeviceOnce once;
+  const cudaError_t e = once.run([] { return cudaFuncSetAttribute(evidence_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 768 * 128); });
+  if (e != cudaSuccess) return e;
+  const EvidenceTile t = evidence_tile<T>(a, 768);
+  const uint64_t tiles = (uint64_t)t.row_tiles * ((a.vars + t.vars - 1) / t.vars);
+  evidence_kernel<T><<<(uint32_t)std::min<uint64_t>(tiles, 0x7fffffff), EV_THREADS, t.cap * 128, st>>>(a, t);
+  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t launch_evidence_grad(const EvidenceArgs& a, cudaStream_t st) {
+  static PcbPerDeviceOnce once;
+  const cudaError_t e = once.run([] { return cudaFuncSetAttribute(evidence_grad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * 512 * 128); });
+  if (e != cudaSuccess) return e;
+  const EvidenceTile t = evidence_tile<T>(a, 512);
+  const uint64_t tiles = (uint64_t)t.row_tiles * ((a.vars + t.vars - 1) / t.vars);
+  // two tiles, and the first columns of every variable of a third for the sums where a warp may have several variables
+  const uint32_t smem = t.cap * 128 * (t.vars > EV_WARPS / 2 ? 3 : 2);
+  evidence_grad_kernel<T><<<(uint32_t)std::min<uint64_t>(tiles, 0x7fffffff), EV_THREADS, smem, st>>>(a, t);
+  return cudaGetLastError();
 }
 
 uint32_t sm_count() {   // of the current device, looked up once
@@ -1058,14 +1570,6 @@ int32_t check_logits(const void* x, int32_t dtype, uint32_t cats, float temperat
   PCB_REQUIRE(temperature > 0.0f && LOG2E / temperature < INFINITY && 1.0f / temperature > 0.0f, "the temperature must be positive and finite");
   return PCB_OK;
 }
-
-// kernel<T><<<...>>>(args) for the logits' type
-#define PCB_BY_DTYPE(dtype, kernel, grid, block, smem, st, args)                               \
-  do {                                                                                         \
-    if ((dtype) == PCB_F32) kernel<float><<<grid, block, smem, st>>>(args);                    \
-    else if ((dtype) == PCB_BF16) kernel<__nv_bfloat16><<<grid, block, smem, st>>>(args);      \
-    else kernel<__half><<<grid, block, smem, st>>>(args);                                      \
-  } while (0)
 
 }  // namespace
 
@@ -1101,8 +1605,9 @@ extern "C" int32_t pcb_token_logprobs_backward(const void* x_dev, int32_t dtype,
   PCB_REQUIRE(!g_top_dev || (top_k > 0 && top_ids_dev), "a gradient of the alternatives needs their indices");
   LogprobGradArgs a{x_dev, rows, row_stride, g_logp_stride, g_entropy_stride, cats, top_k, token_bytes, 1.0f / temperature,
                     LOG2E / temperature, tokens_dev, top_ids_dev, stats_dev, entropy_dev, g_logp_dev, g_entropy_dev, g_top_dev, dx_dev};
-  const uint32_t grid = (uint32_t)(rows < 0x7fffffffull ? rows : 0x7fffffffull);
-  PCB_BY_DTYPE(dtype, logprob_grad_kernel, grid, 256, 0, (cudaStream_t)s, a);
+  if (dtype == PCB_F32) launch_grad<float>(a, (cudaStream_t)s);
+  else if (dtype == PCB_BF16) launch_grad<__nv_bfloat16>(a, (cudaStream_t)s);
+  else launch_grad<__half>(a, (cudaStream_t)s);
   PCB_CUDA(cudaGetLastError());
   return PCB_OK;
 }
@@ -1115,10 +1620,10 @@ extern "C" int32_t pcb_soft_evidence(const void* x_dev, int32_t dtype, uint64_t 
   PCB_REQUIRE(out_dev, "null argument");
   EvidenceArgs a{x_dev, rows, row_stride, var_stride, miss_row_stride, miss_var_stride, vars, cats, 1.0f / temperature,
                  LOG2E / temperature, miss_dev, out_dev, stats_dev, nullptr, nullptr, nullptr};
-  const uint64_t blocks = (rows * vars + 7) / 8;
-  const uint32_t grid = (uint32_t)(blocks < 0x7fffffffull ? blocks : 0x7fffffffull);
-  PCB_BY_DTYPE(dtype, evidence_kernel, grid, 256, 0, (cudaStream_t)s, a);
-  PCB_CUDA(cudaGetLastError());
+  PCB_REQUIRE(!stats_dev || ((uintptr_t)stats_dev & 7) == 0, "statistics that are not 8-byte aligned");
+  PCB_REQUIRE(rows < (1ull << 36), "at most 2^36 rows");
+  cudaStream_t st = (cudaStream_t)s;
+  PCB_CUDA(dtype == PCB_F32 ? launch_evidence<float>(a, st) : dtype == PCB_BF16 ? launch_evidence<__nv_bfloat16>(a, st) : launch_evidence<__half>(a, st));
   return PCB_OK;
 }
 
@@ -1131,9 +1636,10 @@ extern "C" int32_t pcb_soft_evidence_backward(const void* x_dev, int32_t dtype, 
   PCB_REQUIRE(stats_dev && g_dev && dx_dev, "null argument");
   EvidenceArgs a{x_dev, rows, row_stride, var_stride, miss_row_stride, miss_var_stride, vars, cats, 1.0f / temperature,
                  LOG2E / temperature, miss_dev, nullptr, nullptr, stats_dev, g_dev, dx_dev};
-  const uint64_t blocks = (rows * vars + 7) / 8;
-  const uint32_t grid = (uint32_t)(blocks < 0x7fffffffull ? blocks : 0x7fffffffull);
-  PCB_BY_DTYPE(dtype, evidence_grad_kernel, grid, 256, 0, (cudaStream_t)s, a);
-  PCB_CUDA(cudaGetLastError());
+  PCB_REQUIRE(((uintptr_t)stats_dev & 7) == 0, "statistics that are not 8-byte aligned");
+  PCB_REQUIRE(rows < (1ull << 36), "at most 2^36 rows");
+  cudaStream_t st = (cudaStream_t)s;
+  PCB_CUDA(dtype == PCB_F32 ? launch_evidence_grad<float>(a, st) : dtype == PCB_BF16 ? launch_evidence_grad<__nv_bfloat16>(a, st)
+                                                                                    : launch_evidence_grad<__half>(a, st));
   return PCB_OK;
 }
