@@ -168,8 +168,8 @@ __device__ __forceinline__ float most_of_words(const uint32_t* w) {   // NaN doe
   for (int i = 1; i < W; ++i) m = Word<T>::most(m, w[i]);
   return fmaxf(Word<T>::top(m), -INFINITY);
 }
-// 2^d and 2^d d of W words (an even number of elements) added to S and A
-template <typename T, int W>
+// 2^d (and 2^d d) of W words (an even number of elements) added to S (and A)
+template <typename T, int W, bool WITH_A = true>
 __device__ __forceinline__ void add_words(const uint32_t* w, const Shift& s, float2& S, float2& A) {
   constexpr int E = W * (int)PER_WORD<T>;
   if (s.near) {
@@ -181,7 +181,7 @@ __device__ __forceinline__ void add_words(const uint32_t* w, const Shift& s, flo
       const float2 d = fma2(x, {s.c, s.c}, {-s.mc, -s.mc});
       const float2 p = {ex2_ftz(d.x), ex2_ftz(d.y)};
       S = add2(S, p);
-      A = fma2(p, d, A);
+      if (WITH_A) A = fma2(p, d, A);
     }
   } else {
     const float m = finite_shift(s.m);
@@ -191,7 +191,7 @@ __device__ __forceinline__ void add_words(const uint32_t* w, const Shift& s, flo
       const float2 d = {max_nan((x.x - m) * s.c, NO_MASS), max_nan((x.y - m) * s.c, NO_MASS)};
       const float2 p = {ex2_ftz(d.x), ex2_ftz(d.y)};
       S = add2(S, p);
-      A = fma2(p, d, A);
+      if (WITH_A) A = fma2(p, d, A);
     }
   }
 }
@@ -210,21 +210,20 @@ struct LogprobArgs {
   int64_t* top_ids;
 };
 
-// Log-probability of the value x in a row that counts from s; impossible ones are -inf, not the clamp's value.
-__device__ __forceinline__ float logp_of(float x, const Shift& s, float lnS) {
-  if (x == -INFINITY) return lnS != lnS ? lnS : -INFINITY;
-  const float d = s.near ? fmaf(x, s.c, -s.mc) : (x - s.m) * s.c;
-  if (d < -1e30f) {   // a mask's value: finite in natural units where d may not be
-    const float k = s.c * LN2;
-    return ((x < 0.0f) == (s.m < 0.0f) ? (x - s.m) * k : x * k - s.m * k) - lnS;
-  }
-  return fmaf(d, LN2, -lnS);
+// A row's log-probabilities: logp = (x - m) / T - ln S, where S counts from the rounded m c: what that is off by goes into
+// the logarithm.  No scaling by log2(e), which would take a mask's value out of range.
+struct LogScale { float m, invT, ln; };
+template <typename T>
+__device__ __forceinline__ LogScale log_scale(const Shift& s, float S, float invT) {
+  const float ln = S == 0.0f ? 0.0f : logf(S);
+  return {finite_shift(s.m), invT, s.near ? fmaf(-LN2, fmaf(s.m, s.c, -s.mc), ln) : ln};
 }
+__device__ __forceinline__ float logp_of(float x, const LogScale& l) { return fmaf(x - l.m, l.invT, -l.ln); }
 __device__ __forceinline__ float ln_of(float S) { return S == 0.0f ? 0.0f : logf(S); }
 __device__ __forceinline__ float entropy_of(float S, float A, float lnS) { return S == 0.0f ? 0.0f : lnS - LN2 * __fdividef(A, S); }
 __device__ __forceinline__ bool is_category(const LogprobArgs& a, int64_t token) { return token >= 0 && token < (int64_t)a.cats; }
-__device__ __forceinline__ float token_logp(const LogprobArgs& a, int64_t token, float x, const Shift& s, float lnS) {
-  return token < 0 ? 0.0f : token >= (int64_t)a.cats ? NAN : logp_of(x, s, lnS);
+__device__ __forceinline__ float token_logp(const LogprobArgs& a, int64_t token, float x, const LogScale& l) {
+  return token < 0 ? 0.0f : token >= (int64_t)a.cats ? NAN : logp_of(x, l);
 }
 
 // ---- long rows: a block, or the blocks of a cluster, per row -------------------------------------------------------
@@ -546,17 +545,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_row_kernel(Lo
       }
     }
     if (rank == 0) {
-      const Shift at = shift_of<T>(s.m, a.c);
-      const float lnS = ln_of(s.S);
+      const LogScale l = log_scale<T>(shift_of<T>(s.m, a.c), s.S, a.invT);
       if (tid == 0) {
-        if (a.tokens) a.logp[row] = token_logp(a, token, x_token, at, lnS);
-        a.entropy[row] = entropy_of(s.S, s.A, lnS);
+        if (a.tokens) a.logp[row] = token_logp(a, token, x_token, l);
+        a.entropy[row] = entropy_of(s.S, s.A, ln_of(s.S));
         reinterpret_cast<float2*>(a.stats)[row] = {s.m, s.S};
       }
       if (tid < a.top_k) {
         const uint64_t key = sh.best[tid];
         a.top_ids[row * a.top_k + tid] = (uint32_t)~key;
-        a.top_logp[row * a.top_k + tid] = logp_of(value_of(key), at, lnS);
+        a.top_logp[row * a.top_k + tid] = logp_of(value_of(key), l);
       }
     }
     __syncthreads();
@@ -648,7 +646,8 @@ __device__ __forceinline__ Kept short_row(const LogprobArgs& a, ShortRow<T, E, G
   k.best = k.m;
   k.at = 0;
   if (a.top_k == 0) return k;
-  const float lnS = a.top_k > 1 ? ln_of(k.S) : 0.0f;
+  LogScale l = {0.0f, 0.0f, 0.0f};
+  if (a.top_k > 1) l = log_scale<T>(from, k.S, a.invT);
   const uint32_t width = 1u << lg;
   if (__any_sync(0xffffffffu, k.S != k.S)) {   // NaN or inf somewhere: by keys, which order them too
     uint32_t w[Row::W];   // a copy to be indexed, so that the registers need not be
@@ -668,7 +667,7 @@ __device__ __forceinline__ Kept short_row(const LogprobArgs& a, ShortRow<T, E, G
       k.at = (uint32_t)~key;
       if (a.top_k > 1 && valid && sub == 0) {
         a.top_ids[row * a.top_k + n] = k.at;
-        a.top_logp[row * a.top_k + n] = logp_of(k.best, from, lnS);
+        a.top_logp[row * a.top_k + n] = logp_of(k.best, l);
       }
       last = key;
     }
@@ -696,7 +695,7 @@ __device__ __forceinline__ Kept short_row(const LogprobArgs& a, ShortRow<T, E, G
       const uint32_t place = (n & ~(width - 1)) + sub;
       if (valid && place <= n) {
         a.top_ids[row * a.top_k + place] = kept_at;
-        a.top_logp[row * a.top_k + place] = logp_of(kept, from, lnS);
+        a.top_logp[row * a.top_k + place] = logp_of(kept, l);
       }
     }
   }
@@ -706,14 +705,13 @@ __device__ __forceinline__ Kept short_row(const LogprobArgs& a, ShortRow<T, E, G
 // The results of up to 32 rows, one per lane.
 template <typename T>
 __device__ __forceinline__ void short_results(const LogprobArgs& a, const Kept& k, uint64_t row, int64_t token, float x_token) {
-  const Shift from = shift_of<T>(k.m, a.c);
-  const float lnS = ln_of(k.S);
-  if (a.tokens) a.logp[row] = token_logp(a, token, x_token, from, lnS);
-  a.entropy[row] = entropy_of(k.S, k.A, lnS);
+  const LogScale l = log_scale<T>(shift_of<T>(k.m, a.c), k.S, a.invT);
+  if (a.tokens) a.logp[row] = token_logp(a, token, x_token, l);
+  a.entropy[row] = entropy_of(k.S, k.A, ln_of(k.S));
   reinterpret_cast<float2*>(a.stats)[row] = {k.m, k.S};
   if (a.top_k == 1) {
     a.top_ids[row] = k.at;
-    a.top_logp[row] = logp_of(k.best, from, lnS);
+    a.top_logp[row] = logp_of(k.best, l);
   }
 }
 
@@ -1238,318 +1236,383 @@ struct EvidenceArgs {
 };
 
 // ---- soft evidence -----------------------------------------------------------------------------------------------------
-// Logits have the category fastest, evidence the row: a block transposes a tile of 32 rows and up to `cap` columns (the
-// categories of one variable, or of several short ones, which lie one behind the other) through shared memory in fp32.
-// Rows come and go in granules; from there on a lane is a row: it walks the categories of its (variable, part), so that
-// maxima and sums need no shuffles and every access to evidence moves 32 neighbouring rows, 128 bytes.  Element (column,
-// row) lies at column * 32 + (row + column / N) % 32 (granules of N; N = 1 where rows are read by elements): free of bank
-// conflicts both ways.  A distribution of more than `cap` categories passes twice, in chunks: once for its sum, once for its values.
-constexpr uint32_t EV_THREADS = 256, EV_WARPS = 8, EV_COLUMNS = 256;
+// Logits have the category fastest, evidence the row.  A block takes a tile of 32 rows and up to EV_COLUMNS columns (the
+// categories of one variable, or of several short ones that lie one behind the other).  Distributions are worked on where
+// they are contiguous: 2^lg lanes hold one, as in logprob_short_kernel.  Evidence and its gradient move by columns of 32
+// neighbouring rows, 128 bytes, a warp each; shared memory stands between the two orders.  Columns are 33 floats apart there;
+// for fp32 logits, where four neighbouring granules would share a bank, one more per row of a warp after every 32 columns
+// (37 x 192 x 500: 16.0 -> 15.0 us; 16-bit logits, two to a bank, lose more by the arithmetic than the conflicts cost:
+// 512 x 784 x 256 bf16 119 -> 125).  A distribution of more than `cap` categories passes twice, in chunks: once for its
+// sum, once for its values.
+constexpr uint32_t EV_THREADS = 256, EV_WARPS = 8, EV_COLUMNS = 256, EV_PITCH = 33;
 
 struct EvidenceTile {
   uint32_t cap;         // columns of a tile
   uint32_t vars;        // variables per tile (1 where a variable has more than cap categories)
-  uint32_t row_tiles;
-  bool granules;        // rows of a tile begin on 16 bytes
-};
-struct EvidenceJoin { float m[EV_WARPS][32], S[EV_WARPS][32]; };
-
-template <typename T>
-struct EvidenceLayout {
-  static constexpr uint32_t LOG_N = sizeof(T) == 4 ? 2 : 3;
-  uint32_t log_n;   // 0 without granules
-  __device__ __forceinline__ uint32_t at(uint32_t column, uint32_t row) const { return column * 32 + ((row + (column >> log_n)) & 31); }
+  uint32_t row_tiles, var_tiles, lg, each;   // tiles of rows and of variables; lanes per distribution (log2), elements per lane
+  bool granules;        // distributions begin on 16 bytes and end on them
 };
 
-// `columns` columns of 32 rows, the first of them at x: into the tile, in fp32
 template <typename T>
-__device__ __forceinline__ void load_tile(float* tile, EvidenceLayout<T> lay, const T* x, uint64_t row_stride, uint32_t rows, uint32_t columns) {
-  constexpr uint32_t N = Vec<T>::N;
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lay.log_n) {
-    for (uint32_t g = lane; g * N < columns; g += 32) {
-      uint4 q[4];
-      const bool whole = (g + 1) * N <= columns;
+__host__ __device__ __forceinline__ uint32_t tile_place(uint32_t column, uint32_t lg) {
+  return column * EV_PITCH + (sizeof(T) == 4 ? (column >> 5) << (5 - lg) : 0);
+}
+
+// The distributions of a tile: q = row * vars + variable.
+struct TileOrder {
+  uint32_t nv, magic;
+  __device__ __forceinline__ explicit TileOrder(uint32_t nv_) : nv(nv_), magic(0xffffffffu / nv_ + 1) {}
+  __device__ __forceinline__ uint32_t row(uint32_t q) const { return nv == 1 ? q : __umulhi(q, magic); }   // q < 2^13, nv <= 2^8
+};
+
+// Columns of the tile and rows-fastest memory from `at` on, a warp per column: f(place in the tile, pointer).
+template <typename P, typename F>
+__device__ __forceinline__ void tile_columns(uint32_t cats, uint32_t nv, uint64_t rows, uint32_t vars, P* at, F f) {
+  const uint32_t warp = threadIdx.x >> 5;
+  const uint64_t cat_step = rows * vars;
+  if (nv == 1) {
+    at += cat_step * warp;
+    const uint64_t step = cat_step * EV_WARPS;
+    uint32_t c = warp;
+    for (; c + 3 * EV_WARPS < cats; c += 4 * EV_WARPS) {
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t r = warp + EV_WARPS * i;
-        if (whole && r < rows) q[i] = load16(x + r * row_stride + g * N);
-      }
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t r = warp + EV_WARPS * i;
-        if (r >= rows) continue;
-        if (whole) {
-          const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
-#pragma unroll
-          for (uint32_t v = 0; v < N; ++v) tile[lay.at(g * N + v, r)] = element_of<T>(w, v);
-        } else {
-          for (uint32_t j = g * N; j < columns; ++j) tile[lay.at(j, r)] = to_f32(x[r * row_stride + j]);
-        }
-      }
+      for (uint32_t k = 0; k < 4; ++k, at += step) f(c + k * EV_WARPS, at);
     }
+    for (; c < cats; c += EV_WARPS, at += step) f(c, at);
   } else {
-    for (uint32_t j = lane; j < columns; j += 32) {
-      float f[4];
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t r = warp + EV_WARPS * i;
-        f[i] = r < rows ? to_f32(x[r * row_stride + j]) : 0.0f;
-      }
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) tile[lay.at(j, warp + EV_WARPS * i)] = f[i];
+    uint32_t v = warp / cats, c = warp % cats;
+    for (uint32_t column = warp; column < nv * cats; column += EV_WARPS) {
+      f(column, at + rows * v + cat_step * c);
+      c += EV_WARPS;
+      while (c >= cats) { c -= cats; ++v; }
     }
   }
 }
 
-// maximum and sum of the powers of columns [c0, c1) of a row, added to (m, S)
+// A warp's statistics of a whole row of any length and alignment, in all lanes.
 template <typename T>
-__device__ __forceinline__ void add_columns(const float* tile, EvidenceLayout<T> lay, uint32_t c0, uint32_t c1, uint32_t row, float c, float& m, float& S) {
-  constexpr uint32_t RUN = 8;
-  for (uint32_t j = c0; j < c1; j += RUN) {
-    float x[RUN], most = -INFINITY;
+__device__ float2 stream_row(const T* x, uint32_t cats, float c) {
+  const uint32_t lane = threadIdx.x & 31;
+  Part<T> p;
+  p.off = (uint32_t)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  p.base = x - p.off;
+  p.end = p.off + cats;
+  const uint32_t granules = (uint32_t)(((uint64_t)p.end + Vec<T>::N - 1) / Vec<T>::N);
+  float m = -INFINITY;
+  float2 S2 = {0.0f, 0.0f}, none = {0.0f, 0.0f};
+  for (uint32_t g0 = 0; g0 < granules; g0 += 128) {
+    uint32_t w[16];
 #pragma unroll
-    for (uint32_t i = 0; i < RUN; ++i) x[i] = j + i < c1 ? tile[lay.at(j + i, row)] : -INFINITY;
-#pragma unroll
-    for (uint32_t i = 0; i < RUN; ++i) most = fmaxf(most, x[i]);
+    for (uint32_t u = 0; u < 4; ++u) {
+      uint4 q = {Word<T>::NONE, Word<T>::NONE, Word<T>::NONE, Word<T>::NONE};
+      if (g0 + 32 * u + lane < granules) q = p.read(g0 + 32 * u + lane);
+      w[4 * u] = q.x; w[4 * u + 1] = q.y; w[4 * u + 2] = q.z; w[4 * u + 3] = q.w;
+    }
+    const float most = most_of_words<T, 16>(w);
     if (most > m) {
-      if (m != -INFINITY) S *= ex2_ftz(between(shift_of<T>(m, c), shift_of<T>(most, c)));
+      if (m != -INFINITY) {
+        const float f = ex2_ftz(between(shift_of<T>(m, c), shift_of<T>(most, c)));
+        S2 = mul2(S2, {f, f});
+      }
       m = most;
     }
-    const Shift s = shift_of<T>(m, c);
-    if (s.near) {
-#pragma unroll
-      for (uint32_t i = 0; i < RUN; ++i) S += ex2_ftz(fmaf(x[i], s.c, -s.mc));
-    } else {
-      const float from = finite_shift(m);
-#pragma unroll
-      for (uint32_t i = 0; i < RUN; ++i) S += ex2_ftz(max_nan((x[i] - from) * c, NO_MASS));
-    }
+    add_words<T, 16, false>(w, shift_of<T>(m, c), S2, none);
   }
-}
-template <typename T>
-__device__ __forceinline__ void join_columns(const EvidenceJoin& join, uint32_t first, uint32_t parts, uint32_t row, float c, float& m, float& S) {
-  m = -INFINITY;
-  for (uint32_t i = 0; i < parts; ++i) m = fmaxf(m, join.m[first + i][row]);
-  const Shift to = shift_of<T>(m, c);
-  S = 0.0f;
-  for (uint32_t i = 0; i < parts; ++i) {
-    const float mi = join.m[first + i][row];
-    S += join.S[first + i][row] * (mi == -INFINITY || mi == m ? 1.0f : ex2_ftz(between(shift_of<T>(mi, c), to)));
-  }
+  const Stat s = lanes_join<T, 32>(Stat{m, S2.x + S2.y, 0.0f}, c);
+  return {s.m, s.S};
 }
 
-// What a warp works on: variable `v` of the tile and part `part` of its categories (all, where a tile has eight variables).
-struct EvidenceUnits {
-  uint32_t parts, units;
-  __device__ __forceinline__ explicit EvidenceUnits(uint32_t vars) : parts(vars >= EV_WARPS ? 1 : EV_WARPS / vars), units(vars * parts) {}
-  __device__ __forceinline__ uint32_t var(uint32_t u) const { return u / parts; }
-  __device__ __forceinline__ uint32_t begin(uint32_t u, uint32_t columns) const { return (uint32_t)((uint64_t)(u % parts) * columns / parts); }
-  __device__ __forceinline__ uint32_t end(uint32_t u, uint32_t columns) const { return (uint32_t)((uint64_t)(u % parts + 1) * columns / parts); }
-};
-
-template <typename T>
-__global__ void __launch_bounds__(EV_THREADS, 4) evidence_kernel(EvidenceArgs a, EvidenceTile et) {
+template <typename T, int E, bool GRANULES>
+__global__ void __launch_bounds__(EV_THREADS, sizeof(T) == 4 ? 4 : 5) evidence_kernel(EvidenceArgs a, EvidenceTile et) {
+  using Row = ShortRow<T, E, GRANULES>;
   extern __shared__ __align__(16) float tile[];
-  __shared__ EvidenceJoin join;
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const EvidenceLayout<T> lay{et.granules ? EvidenceLayout<T>::LOG_N : 0};
-  const uint64_t tiles = (uint64_t)et.row_tiles * ((a.vars + et.vars - 1) / et.vars);
-  for (uint64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
-    const uint64_t b0 = i % et.row_tiles * 32, b = b0 + lane;   // neighbouring blocks write neighbouring rows
-    const uint32_t v0 = (uint32_t)(i / et.row_tiles) * et.vars, nv = min(et.vars, a.vars - v0);
+  __shared__ float2 streamed[32];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = et.lg, sub = lane & ((1u << lg) - 1), per_pass = EV_THREADS >> lg;
+  const uint64_t b0 = (uint64_t)blockIdx.x * 32;   // neighbouring blocks write neighbouring rows
+  for (uint32_t vt = blockIdx.y; vt < et.var_tiles; vt += gridDim.y) {
+    const uint32_t v0 = vt * et.vars, nv = min(et.vars, a.vars - v0);
     const uint32_t rows = (uint32_t)min((uint64_t)32, a.rows - b0), width = min(a.cats, et.cap);   // categories of a pass
     const bool one = width == a.cats;
+    const TileOrder order(nv);
     const T* x = static_cast<const T*>(a.x) + b0 * a.row_stride + (uint64_t)v0 * a.var_stride;
-    const EvidenceUnits un(nv);
-    float m = -INFINITY, S = 0.0f;   // of the one unit that a warp has where parts > 1
-    for (uint32_t c0 = 0; c0 < a.cats; c0 += width) {
-      const uint32_t n = min(width, a.cats - c0);
-      load_tile<T>(tile, lay, x + c0, a.row_stride, rows, one ? nv * a.cats : n);
-      __syncthreads();
-      if (un.parts > 1 && warp < un.units && lane < rows) add_columns<T>(tile, lay, un.var(warp) * a.cats + un.begin(warp, n), un.var(warp) * a.cats + un.end(warp, n), lane, a.c, m, S);
-      if (!one) __syncthreads();
-    }
-    if (un.parts > 1) {
-      join.m[warp][lane] = m;
-      join.S[warp][lane] = S;
-      __syncthreads();
-    }
-    for (uint32_t c0 = 0; c0 < a.cats; c0 += width) {
-      const uint32_t n = min(width, a.cats - c0);
-      if (!one) {
-        load_tile<T>(tile, lay, x + c0, a.row_stride, rows, n);
-        __syncthreads();
+    if (!one) {
+      for (uint32_t r = warp; r < rows; r += EV_WARPS) {
+        const float2 s = stream_row<T>(x + r * a.row_stride, a.cats, a.c);
+        if (lane == 0) streamed[r] = s;
       }
-      for (uint32_t u = warp; u < un.units; u += EV_WARPS) {
-        if (lane >= rows) continue;
-        const uint32_t v = v0 + un.var(u), first = un.var(u) * a.cats;
-        if (un.parts > 1) {
-          join_columns<T>(join, u - u % un.parts, un.parts, lane, a.c, m, S);
+      __syncthreads();
+    }
+    for (uint32_t c0 = 0; c0 < a.cats; c0 += width) {
+      const uint32_t n = min(width, a.cats - c0);
+      for (uint32_t q0 = 0; q0 < rows * nv; q0 += per_pass) {
+        const uint32_t q = q0 + (threadIdx.x >> lg), qq = min(q, rows * nv - 1), r = order.row(qq), v = qq - r * nv;
+        Row in;
+        in.load(x + r * a.row_stride + v * a.var_stride + c0, sub, lg, n);
+        const uint64_t b = b0 + r;
+        const bool missing = a.miss && a.miss[b * a.miss_row_stride + (v0 + v) * a.miss_var_stride];
+        float m, S;
+        if (one) {
+          m = over_lanes(most_of_words<T, Row::W>(in.w), lg, most_of);
+          float2 S2 = {0.0f, 0.0f}, none = {0.0f, 0.0f};
+          add_words<T, Row::W, false>(in.w, shift_of<T>(m, a.c), S2, none);
+          S = over_lanes(S2.x + S2.y, lg, sum_of);
         } else {
-          m = -INFINITY;
-          S = 0.0f;
-          add_columns<T>(tile, lay, first, first + n, lane, a.c, m, S);
+          m = streamed[r].x;
+          S = streamed[r].y;
         }
-        const Shift from = shift_of<T>(m, a.c);
-        const float lnS = ln_of(S);
-        const bool missing = a.miss && a.miss[b * a.miss_row_stride + v * a.miss_var_stride];
-        if (a.stats_out && c0 == 0 && u % un.parts == 0) reinterpret_cast<float2*>(a.stats_out)[b * a.vars + v] = {m, S};
-        const uint32_t j1 = un.end(u, n);
-        float* out = a.out + b + a.rows * (v + (uint64_t)a.vars * (c0 + un.begin(u, n)));
-        const uint64_t step = a.rows * a.vars;
-#pragma unroll 4
-        for (uint32_t j = un.begin(u, n); j < j1; ++j, out += step) {
-          const float xj = tile[lay.at(first + j, lane)];
-          float value = fmaf(fmaf(xj, from.c, -from.mc), LN2, -lnS);   // near, and no mask's value: all but a few
-          if (!from.near || value < -1e30f) value = logp_of(xj, from, lnS);
-          *out = missing ? 0.0f : value;
-        }
-      }
-      __syncthreads();
-    }
-  }
-}
-
-// columns of a tile back to rows at dx, in T
-template <typename T>
-__device__ __forceinline__ void store_tile(const float* tile, EvidenceLayout<T> lay, T* dx, uint64_t row_stride, uint32_t rows, uint32_t columns) {
-  constexpr uint32_t N = Vec<T>::N;
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (uint32_t r = warp; r < rows; r += EV_WARPS) {
-    T* to = dx + r * row_stride;
-    if (lay.log_n) {
-      for (uint32_t g = lane; g * N < columns; g += 32) {
-        if ((g + 1) * N <= columns) {
-          uint32_t w[4];
+        if (a.stats_out && c0 == 0 && sub == 0 && q == qq) reinterpret_cast<float2*>(a.stats_out)[b * a.vars + v0 + v] = {m, S};
+        const LogScale l = log_scale<T>(shift_of<T>(m, a.c), S, a.invT);
+        const uint32_t column = v * a.cats + sub * Row::N;
+        const uint32_t mine = q == qq ? n : 0;   // a place is written where it lies below
 #pragma unroll
-          for (uint32_t v = 0; v < N; v += PER_WORD<T>) {
-            const float f = tile[lay.at(g * N + v, r)];
-            if constexpr (sizeof(T) == 4) w[v] = __float_as_uint(f);
-            else if constexpr (std::is_same<T, __half>::value) w[v / 2] = Word<T>::bits(__floats2half2_rn(f, tile[lay.at(g * N + v + 1, r)]));
-            else w[v / 2] = Word<T>::bits(__floats2bfloat162_rn(f, tile[lay.at(g * N + v + 1, r)]));
-          }
-          *reinterpret_cast<uint4*>(to + g * N) = {w[0], w[1], w[2], w[3]};
-        } else {
-          for (uint32_t j = g * N; j < columns; ++j) to[j] = from_f32<T>(tile[lay.at(j, r)]);
+        for (int e = 0; e < E; e += Row::N) {
+          if (sub * Row::N + (((uint32_t)e) << lg) >= mine) continue;
+          float* at = tile + tile_place<T>(column + ((uint32_t)e << lg), lg) + r;
+#pragma unroll
+          for (uint32_t h = 0; h < Row::N; ++h) at[h * EV_PITCH] = missing ? 0.0f : logp_of(element_of<T>(in.w, e + h), l);
         }
       }
-    } else {
-      for (uint32_t j = lane; j < columns; j += 32) to[j] = from_f32<T>(tile[lay.at(j, r)]);
+      __syncthreads();
+      float* out = a.out + b0 + lane + a.rows * (v0 + (uint64_t)a.vars * c0);
+      if (lane < rows) tile_columns(n, nv, a.rows, a.vars, out, [&](uint32_t column, float* at) { *at = tile[tile_place<T>(column, lg) + lane]; });
+      __syncthreads();
     }
   }
 }
 
-// dx_c = (g_c - p_c sum g) / T: the sum needs g alone; g waits in a second tile where the distribution fits into one.
-template <typename T>
-__global__ void __launch_bounds__(EV_THREADS, 3) evidence_grad_kernel(EvidenceArgs a, EvidenceTile et) {
+// dx_c = (g_c - p_c sum g) / T
+template <typename T, int E, bool GRANULES>
+__global__ void __launch_bounds__(EV_THREADS, GRANULES ? 4 : 3) evidence_grad_kernel(EvidenceArgs a, EvidenceTile et) {
+  using Row = ShortRow<T, E, GRANULES>;
   extern __shared__ __align__(16) float tile[];
-  __shared__ EvidenceJoin join;
-  float* g_tile = tile + et.cap * 32;
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const EvidenceLayout<T> lay{et.granules ? EvidenceLayout<T>::LOG_N : 0};
-  const uint64_t tiles = (uint64_t)et.row_tiles * ((a.vars + et.vars - 1) / et.vars), step = a.rows * a.vars;
-  for (uint64_t i = blockIdx.x; i < tiles; i += gridDim.x) {
-    const uint64_t b0 = i % et.row_tiles * 32, b = b0 + lane;
-    const uint32_t v0 = (uint32_t)(i / et.row_tiles) * et.vars, nv = min(et.vars, a.vars - v0);
+  __shared__ float part[EV_WARPS][32];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = et.lg, sub = lane & ((1u << lg) - 1), per_pass = EV_THREADS >> lg;
+  const uint64_t b0 = (uint64_t)blockIdx.x * 32;
+  for (uint32_t vt = blockIdx.y; vt < et.var_tiles; vt += gridDim.y) {
+    const uint32_t v0 = vt * et.vars, nv = min(et.vars, a.vars - v0);
     const uint32_t rows = (uint32_t)min((uint64_t)32, a.rows - b0), width = min(a.cats, et.cap);
     const bool one = width == a.cats;
+    const TileOrder order(nv);
     const T* x = static_cast<const T*>(a.x) + b0 * a.row_stride + (uint64_t)v0 * a.var_stride;
     T* dx = static_cast<T*>(a.dx) + (b0 * a.vars + v0) * a.cats;
-    const EvidenceUnits un(nv);
-    if (one) load_tile<T>(tile, lay, x, a.row_stride, rows, nv * a.cats);
-    for (uint32_t u = warp; u < un.units; u += EV_WARPS) {
-      if (lane >= rows) continue;
-      const uint32_t v = v0 + un.var(u), first = un.var(u) * a.cats;
-      const float* g = a.g + b + a.rows * v;
-      const uint32_t j0 = un.begin(u, a.cats), j1 = un.end(u, a.cats);
+    const float* g = a.g + b0 + lane + a.rows * v0;
+    if (!one) {   // the sum of all chunks first
       float sum = 0.0f;
-#pragma unroll 8
-      for (uint32_t j = j0; j < j1; ++j) {
-        const float gj = g[step * j];
-        sum += gj;
-        if (one) g_tile[(first + j) * 32 + lane] = gj;
-      }
-      if (un.parts > 1) join.S[u][lane] = sum;
-      else g_tile[first * 32 + lane + 32 * et.cap] = sum;   // behind the tile: one sum per variable and row
+      if (lane < rows) tile_columns(a.cats, 1, a.rows, a.vars, g, [&](uint32_t, const float* at) { sum += *at; });
+      part[warp][lane] = sum;
     }
-    __syncthreads();
     for (uint32_t c0 = 0; c0 < a.cats; c0 += width) {
       const uint32_t n = min(width, a.cats - c0);
-      if (!one) {
-        load_tile<T>(tile, lay, x + c0, a.row_stride, rows, n);
-        __syncthreads();
-      }
-      for (uint32_t u = warp; u < un.units; u += EV_WARPS) {
-        if (lane >= rows) continue;
-        const uint32_t v = v0 + un.var(u), first = un.var(u) * a.cats;
-        float sum = 0.0f;
-        if (un.parts > 1)
-          for (uint32_t k = 0; k < un.parts; ++k) sum += join.S[u - u % un.parts + k][lane];
-        else sum = g_tile[first * 32 + lane + 32 * et.cap];
-        const float2 st = reinterpret_cast<const float2*>(a.stats)[b * a.vars + v];
+      const float* gc = g + a.rows * ((uint64_t)a.vars * c0);
+      if (lane < rows) tile_columns(n, nv, a.rows, a.vars, gc, [&](uint32_t column, const float* at) { tile[tile_place<T>(column, lg) + lane] = *at; });
+      __syncthreads();
+      for (uint32_t q0 = 0; q0 < rows * nv; q0 += per_pass) {
+        const uint32_t q = q0 + (threadIdx.x >> lg), qq = min(q, rows * nv - 1), r = order.row(qq), v = qq - r * nv;
+        Row in;
+        in.load(x + r * a.row_stride + v * a.var_stride + c0, sub, lg, n);
+        const uint64_t b = b0 + r;
+        const bool missing = a.miss && a.miss[b * a.miss_row_stride + (v0 + v) * a.miss_var_stride];
+        const float2 st = reinterpret_cast<const float2*>(a.stats)[b * a.vars + v0 + v];
+        const uint32_t column = v * a.cats + sub * Row::N;
+        float ge[E], sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e += Row::N) {
+          const bool there = sub * Row::N + ((uint32_t)e << lg) < n;
+          const float* at = tile + tile_place<T>(column + (there ? (uint32_t)e << lg : 0), lg) + r;
+#pragma unroll
+          for (uint32_t h = 0; h < Row::N; ++h) ge[e + h] = there ? at[h * EV_PITCH] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum += ge[e];
+        if (one) {
+          sum = over_lanes(sum, lg, sum_of);
+        } else {
+          sum = 0.0f;
+          for (uint32_t k = 0; k < EV_WARPS; ++k) sum += part[k][r];
+        }
         const Shift from = shift_of<T>(st.x, a.c);
-        const bool none = st.y == 0.0f || (a.miss && a.miss[b * a.miss_row_stride + v * a.miss_var_stride]);
-        const float k = sum / st.y;
-        const float* g = a.g + b + a.rows * v + step * c0;
-        const uint32_t j1 = un.end(u, n);
-#pragma unroll 4
-        for (uint32_t j = un.begin(u, n); j < j1; ++j) {
-          const uint32_t at = lay.at(first + j, lane);
-          const float gj = one ? g_tile[(first + j) * 32 + lane] : g[step * j];
-          tile[at] = none ? 0.0f : (gj - ex2_ftz(scaled(from, tile[at])) * k) * a.invT;
+        const float scale = missing || st.y == 0.0f ? 0.0f : a.invT, k = -sum / st.y * a.invT;
+        uint32_t out[Row::W];
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 xe = pair_of<T>(in.w, e);
+          float2 d = fma2(xe, {from.c, from.c}, {-from.mc, -from.mc});
+          if (!from.near) d = {scaled(from, xe.x), scaled(from, xe.y)};
+          float2 value = fma2({ex2_ftz(d.x), ex2_ftz(d.y)}, {k, k}, mul2({ge[e], ge[e + 1]}, {scale, scale}));
+          if (scale == 0.0f) value = {0.0f, 0.0f};
+          if constexpr (sizeof(T) == 4) {
+            out[e] = __float_as_uint(value.x);
+            out[e + 1] = __float_as_uint(value.y);
+          } else if constexpr (std::is_same<T, __half>::value) {
+            out[e / 2] = Word<T>::bits(__floats2half2_rn(value.x, value.y));
+          } else {
+            out[e / 2] = Word<T>::bits(__floats2bfloat162_rn(value.x, value.y));
+          }
+        }
+        T* to = dx + ((uint64_t)r * a.vars + v) * a.cats + c0;
+        if (q == qq) {
+          if constexpr (GRANULES) {
+#pragma unroll
+            for (int j = 0; j < Row::W / 4; ++j) {
+              const uint32_t at = (sub + ((uint32_t)j << lg)) * Row::N;
+              if (at < n) *reinterpret_cast<uint4*>(to + at) = {out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]};
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              const uint32_t j = Row::index(e, sub, lg);
+              if (j >= n) continue;
+              if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(to)[j] = out[e];
+              else reinterpret_cast<uint16_t*>(to)[j] = (uint16_t)(out[e / 2] >> (16 * (e & 1)));
+            }
+          }
         }
       }
-      __syncthreads();
-      store_tile<T>(tile, lay, dx + c0, (uint64_t)a.vars * a.cats, rows, one ? nv * a.cats : n);
       __syncthreads();
     }
   }
 }
 
-// Tiles of up to EV_COLUMNS columns; a variable of up to `most` categories is held whole.
-template <typename T>
-EvidenceTile evidence_tile(const EvidenceArgs& a, uint32_t most) {
-  EvidenceTile t;
-  const uint32_t n = Vec<T>::N;
-  t.vars = 1;
-  if (a.var_stride == a.cats && a.cats <= EV_COLUMNS / 2) {   // variables one behind the other
-    t.vars = EV_COLUMNS / a.cats;
-    while (t.vars > 1 && t.vars * a.cats % n) --t.vars;   // whole granules per tile where there is such a number
-    if (t.vars * a.cats % n) t.vars = EV_COLUMNS / a.cats;
+// Variables of at most 32 categories that lie one behind the other: a lane is a row, holds a distribution of at most C
+// categories, and needs no shuffles; rows come (and the gradient's go) by elements, 32 neighbouring ones at a time.
+template <typename T, int C, bool GRADIENT>
+__global__ void __launch_bounds__(EV_THREADS, GRADIENT ? 3 : 4) evidence_thin_kernel(EvidenceArgs a, EvidenceTile et) {
+  extern __shared__ __align__(16) float tile[];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint64_t step = a.rows * a.vars, b0 = (uint64_t)blockIdx.x * 32, b = b0 + lane;
+  for (uint32_t vt = blockIdx.y; vt < et.var_tiles; vt += gridDim.y) {
+    const uint32_t v0 = vt * et.vars, nv = min(et.vars, a.vars - v0), columns = nv * a.cats;
+    const uint32_t rows = (uint32_t)min((uint64_t)32, a.rows - b0);
+    const T* x = static_cast<const T*>(a.x) + b0 * a.row_stride + (uint64_t)v0 * a.var_stride;
+    for (uint32_t r = warp; r < rows; r += EV_WARPS) {
+      const T* from = x + r * a.row_stride;
+      T raw[EV_COLUMNS / 32];
+#pragma unroll
+      for (uint32_t k = 0; k < EV_COLUMNS / 32; ++k)
+        if (32 * k + lane < columns) raw[k] = from[32 * k + lane];
+#pragma unroll
+      for (uint32_t k = 0; k < EV_COLUMNS / 32; ++k)
+        if (32 * k + lane < columns) tile[(32 * k + lane) * EV_PITCH + r] = to_f32(raw[k]);
+    }
+    __syncthreads();
+    for (uint32_t v = warp; v < nv; v += EV_WARPS) {
+      if (lane >= rows) continue;
+      float* at = tile + v * a.cats * EV_PITCH + lane;
+      const bool missing = a.miss && a.miss[b * a.miss_row_stride + (v0 + v) * a.miss_var_stride];
+      const uint64_t memory = b + a.rows * (v0 + v);
+      float xc[C];
+#pragma unroll
+      for (int c = 0; c < C; ++c) xc[c] = c < (int)a.cats ? at[c * EV_PITCH] : -INFINITY;
+      if constexpr (!GRADIENT) {
+        float m = xc[0], S = 0.0f;
+#pragma unroll
+        for (int c = 1; c < C; ++c) m = fmaxf(m, xc[c]);
+        m = fmaxf(m, -INFINITY);
+        const Shift from = shift_of<T>(m, a.c);
+        if (from.near) {
+#pragma unroll
+          for (int c = 0; c < C; ++c) S += ex2_ftz(fmaf(xc[c], from.c, -from.mc));
+        } else {
+#pragma unroll
+          for (int c = 0; c < C; ++c) S += ex2_ftz(max_nan((xc[c] - finite_shift(m)) * from.c, NO_MASS));
+        }
+        const LogScale l = log_scale<T>(from, S, a.invT);
+        if (a.stats_out) reinterpret_cast<float2*>(a.stats_out)[b * a.vars + v0 + v] = {m, S};
+        float* out = a.out + memory;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          if (c < (int)a.cats) out[step * c] = missing ? 0.0f : logp_of(xc[c], l);
+      } else {
+        const float* g = a.g + memory;
+        float gc[C], sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) gc[c] = c < (int)a.cats ? g[step * c] : 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) sum += gc[c];
+        const float2 st = reinterpret_cast<const float2*>(a.stats)[b * a.vars + v0 + v];
+        const Shift from = shift_of<T>(st.x, a.c);
+        const bool none = missing || st.y == 0.0f;
+        const float k = sum / st.y;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          if (c < (int)a.cats) at[c * EV_PITCH] = none ? 0.0f : (gc[c] - ex2_ftz(scaled(from, xc[c])) * k) * a.invT;
+      }
+    }
+    __syncthreads();
+    if constexpr (GRADIENT) {
+      T* dx = static_cast<T*>(a.dx) + (b0 * a.vars + v0) * a.cats;
+      for (uint32_t r = warp; r < rows; r += EV_WARPS) {
+        T* to = dx + (uint64_t)r * a.vars * a.cats;
+        for (uint32_t j = lane; j < columns; j += 32) to[j] = from_f32<T>(tile[j * EV_PITCH + r]);
+      }
+      __syncthreads();
+    }
   }
-  if (t.vars > a.vars) t.vars = a.vars;
-  t.cap = t.vars > 1 ? t.vars * a.cats : a.cats <= most ? a.cats : EV_COLUMNS;
+}
+
+// Tiles of up to EV_COLUMNS columns; a variable of up to EV_MOST categories is held whole.
+template <typename T> constexpr uint32_t EV_MOST = 32 * Most<T>::E < 768 ? 32 * Most<T>::E : 768;
+template <typename T>
+EvidenceTile evidence_tile(const EvidenceArgs& a) {
+  EvidenceTile t;
+  t.vars = a.var_stride == a.cats && a.cats <= EV_COLUMNS / 2 ? std::min(EV_COLUMNS / a.cats, a.vars) : 1;
+  t.cap = t.vars > 1 ? t.vars * a.cats : a.cats <= EV_MOST<T> ? a.cats : EV_COLUMNS;
   t.row_tiles = (uint32_t)((a.rows + 31) / 32);
-  // where rows of tiles begin: of x, and of dx, which is contiguous
-  const bool several = t.vars < a.vars;
-  uint64_t at = reinterpret_cast<uintptr_t>(a.x) | a.row_stride * sizeof(T) | (several ? t.vars * a.var_stride * sizeof(T) : 0);
-  if (a.dx) at |= reinterpret_cast<uintptr_t>(a.dx) | (uint64_t)a.vars * a.cats * sizeof(T) | (several ? (uint64_t)t.vars * a.cats * sizeof(T) : 0);
+  t.var_tiles = (a.vars - 1) / t.vars + 1;
+  uint64_t at = reinterpret_cast<uintptr_t>(a.x) | (a.row_stride | (a.vars > 1 ? a.var_stride : 0) | a.cats) * sizeof(T);
+  if (a.dx) at |= reinterpret_cast<uintptr_t>(a.dx);   // contiguous: as the categories are
   t.granules = (at & 15) == 0;
+  // few lanes per distribution; four at least where it has as many granules, eight where it is read by elements
+  const uint32_t n = std::min(a.cats, t.cap), units = t.granules ? n / Vec<T>::N : n, wanted = t.granules ? 4 : 8;
+  t.lg = 0;
+  while (t.lg < 5 && (n > (Most<T>::E << t.lg) || (1u << t.lg) < std::min(units, wanted))) ++t.lg;
+  t.each = t.granules ? ((units + (1u << t.lg) - 1) >> t.lg) * Vec<T>::N : (n + (1u << t.lg) - 1) >> t.lg;
   return t;
 }
 
-template <typename T>
-cudaError_t launch_evidence(const EvidenceArgs& a, cudaStream_t st) {
+template <typename T, int E, bool GRANULES>
+cudaError_t launch_evidence_as(const EvidenceArgs& a, const EvidenceTile& t, cudaStream_t st) {
+  const dim3 grid(t.row_tiles, std::min(t.var_tiles, 65535u));
+  const uint32_t smem = (tile_place<T>(t.cap, t.lg) + 32) * (uint32_t)sizeof(float);
   static PcbPerDeviceOnce once;
-  const cudaError_t e = once.run([] { return cudaFuncSetAttribute(evidence_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 768 * 128); });
+  const cudaError_t e = once.run([] {
+    const int most = (int)((tile_place<T>(768, 0) + 32) * sizeof(float));
+    const cudaError_t f = cudaFuncSetAttribute(evidence_kernel<T, E, GRANULES>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    return f != cudaSuccess ? f : cudaFuncSetAttribute(evidence_grad_kernel<T, E, GRANULES>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  });
   if (e != cudaSuccess) return e;
-  const EvidenceTile t = evidence_tile<T>(a, 768);
-  const uint64_t tiles = (uint64_t)t.row_tiles * ((a.vars + t.vars - 1) / t.vars);
-  evidence_kernel<T><<<(uint32_t)std::min<uint64_t>(tiles, 0x7fffffff), EV_THREADS, t.cap * 128, st>>>(a, t);
+  if (a.dx) evidence_grad_kernel<T, E, GRANULES><<<grid, EV_THREADS, smem, st>>>(a, t);
+  else evidence_kernel<T, E, GRANULES><<<grid, EV_THREADS, smem, st>>>(a, t);
+  return cudaGetLastError();
+}
+template <typename T, int E>
+cudaError_t launch_evidence_of(const EvidenceArgs& a, const EvidenceTile& t, cudaStream_t st) {
+  if constexpr (E >= (int)Vec<T>::N)
+    if (t.granules) return launch_evidence_as<T, E, true>(a, t, st);
+  return launch_evidence_as<T, E, false>(a, t, st);
+}
+template <typename T, int C>
+cudaError_t launch_thin(const EvidenceArgs& a, const EvidenceTile& t, cudaStream_t st) {
+  const dim3 grid(t.row_tiles, std::min(t.var_tiles, 65535u));
+  const uint32_t smem = t.cap * EV_PITCH * (uint32_t)sizeof(float);
+  if (a.dx) evidence_thin_kernel<T, C, true><<<grid, EV_THREADS, smem, st>>>(a, t);
+  else evidence_thin_kernel<T, C, false><<<grid, EV_THREADS, smem, st>>>(a, t);
   return cudaGetLastError();
 }
 template <typename T>
-cudaError_t launch_evidence_grad(const EvidenceArgs& a, cudaStream_t st) {
-  static PcbPerDeviceOnce once;
-  const cudaError_t e = once.run([] { return cudaFuncSetAttribute(evidence_grad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * 512 * 128); });
-  if (e != cudaSuccess) return e;
-  const EvidenceTile t = evidence_tile<T>(a, 512);
-  const uint64_t tiles = (uint64_t)t.row_tiles * ((a.vars + t.vars - 1) / t.vars);
-  // two tiles, and the first columns of every variable of a third for the sums where a warp may have several variables
-  const uint32_t smem = t.cap * 128 * (t.vars > EV_WARPS / 2 ? 3 : 2);
-  evidence_grad_kernel<T><<<(uint32_t)std::min<uint64_t>(tiles, 0x7fffffff), EV_THREADS, smem, st>>>(a, t);
-  return cudaGetLastError();
+cudaError_t launch_evidence(const EvidenceArgs& a, cudaStream_t st) {   // the gradient where dx is given
+  const EvidenceTile t = evidence_tile<T>(a);
+  if (t.vars > 1 && a.cats <= 32) {
+    if (a.cats <= 2) return launch_thin<T, 2>(a, t, st);
+    if (a.cats <= 4) return launch_thin<T, 4>(a, t, st);
+    if (a.cats <= 8) return launch_thin<T, 8>(a, t, st);
+    if (a.cats <= 16) return launch_thin<T, 16>(a, t, st);
+    return launch_thin<T, 32>(a, t, st);
+  }
+  if (t.each <= 4) return launch_evidence_of<T, 4>(a, t, st);
+  if (t.each <= 8) return launch_evidence_of<T, 8>(a, t, st);
+  if (t.each <= 16) return launch_evidence_of<T, 16>(a, t, st);
+  return launch_evidence_of<T, Most<T>::E>(a, t, st);
 }
 
 uint32_t sm_count() {   // of the current device, looked up once
@@ -1621,7 +1684,7 @@ extern "C" int32_t pcb_soft_evidence(const void* x_dev, int32_t dtype, uint64_t 
   EvidenceArgs a{x_dev, rows, row_stride, var_stride, miss_row_stride, miss_var_stride, vars, cats, 1.0f / temperature,
                  LOG2E / temperature, miss_dev, out_dev, stats_dev, nullptr, nullptr, nullptr};
   PCB_REQUIRE(!stats_dev || ((uintptr_t)stats_dev & 7) == 0, "statistics that are not 8-byte aligned");
-  PCB_REQUIRE(rows < (1ull << 36), "at most 2^36 rows");
+  PCB_REQUIRE(rows < (1ull << 35), "at most 2^35 rows");
   cudaStream_t st = (cudaStream_t)s;
   PCB_CUDA(dtype == PCB_F32 ? launch_evidence<float>(a, st) : dtype == PCB_BF16 ? launch_evidence<__nv_bfloat16>(a, st) : launch_evidence<__half>(a, st));
   return PCB_OK;
@@ -1637,9 +1700,9 @@ extern "C" int32_t pcb_soft_evidence_backward(const void* x_dev, int32_t dtype, 
   EvidenceArgs a{x_dev, rows, row_stride, var_stride, miss_row_stride, miss_var_stride, vars, cats, 1.0f / temperature,
                  LOG2E / temperature, miss_dev, nullptr, nullptr, stats_dev, g_dev, dx_dev};
   PCB_REQUIRE(((uintptr_t)stats_dev & 7) == 0, "statistics that are not 8-byte aligned");
-  PCB_REQUIRE(rows < (1ull << 36), "at most 2^36 rows");
+  PCB_REQUIRE(rows < (1ull << 35), "at most 2^35 rows");
   cudaStream_t st = (cudaStream_t)s;
-  PCB_CUDA(dtype == PCB_F32 ? launch_evidence_grad<float>(a, st) : dtype == PCB_BF16 ? launch_evidence_grad<__nv_bfloat16>(a, st)
-                                                                                    : launch_evidence_grad<__half>(a, st));
+  PCB_CUDA(dtype == PCB_F32 ? launch_evidence<float>(a, st) : dtype == PCB_BF16 ? launch_evidence<__nv_bfloat16>(a, st)
+                                                                                    : launch_evidence<__half>(a, st));
   return PCB_OK;
 }
