@@ -347,7 +347,7 @@ int32_t pcb_soft_evidence_backward(const void* x_dev, int32_t dtype, uint64_t ro
                                    const float* stats_dev, const float* g_dev, void* dx_dev, pcb_stream s);
 
 /* A head of `cats` x `features` weights in 4 bits: weight (n, k) = scale[n, k / group] * (code[n, k] - 8), codes 0..15,
- * group 32, 64 or 128, scales bf16 or f16.  Codes come two a byte, [cats, (features + 1) / 2], the even column in the
+ * group 32, 64 or 128, scales bf16 or f16, at most 32768 features.  Codes come two a byte, [cats, (features + 1) / 2], the even column in the
  * low half; scales [cats, ceil(features / group)]; both contiguous.
  * pcb_head_quantize makes them of a weight matrix (contiguous, f32 / bf16 / f16): scale = max |w| / 7 rounded to
  * scale_dtype, code = round(w / scale) + 8.  pcb_head_pack lays codes and scales out in the order in which

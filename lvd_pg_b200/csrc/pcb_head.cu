@@ -16,7 +16,11 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 namespace {
+
+constexpr uint32_t MAX_FEATURES = 32768;   // three columns of them fit into shared memory
 
 struct HeadShape {
   uint32_t cats, features, group;
@@ -33,8 +37,9 @@ HeadShape head_shape(uint32_t cats, uint32_t features, uint32_t group) {
   return h;
 }
 int32_t check_shape(uint32_t cats, uint32_t features, uint32_t group) {
-  PCB_REQUIRE(cats >= 1 && cats <= 0x7fffffffu && features >= 1 && features <= 0x7fffffffu, "a head has at least one category and one feature");
+  PCB_REQUIRE(cats >= 1 && cats <= 0x7fffffffu && features >= 1, "a head has at least one category and one feature");
   PCB_REQUIRE(group == 32 || group == 64 || group == 128, "groups hold 32, 64 or 128 features");
+  if (features > MAX_FEATURES) return pcb_fail(PCB_ERR_TOO_LARGE, "a head has at most 32768 features");
   return PCB_OK;
 }
 bool is_dtype(int32_t d) { return d == PCB_F32 || d == PCB_BF16 || d == PCB_F16; }
@@ -191,61 +196,227 @@ __device__ __forceinline__ void store_y(void* y, uint64_t i, float v, int32_t dt
   else static_cast<__half*>(y)[i] = __float2half_rn(v);
 }
 
-// One warp per tile of 16 categories and 8 feature vectors.
-template <typename X>
-__global__ void __launch_bounds__(128) head_kernel(HeadArgs a) {
+// Persistent blocks of sixteen warps, in two halves of eight.  A half takes R tiles of 16 categories at a time; its warps
+// share the features, so that short heads fill the GPU too, and add up their parts through shared memory.  The feature
+// vectors stay in shared memory, as columns of the B operand (fp32: three columns each, one per term, joined at the end);
+// codes and scales go straight from memory to registers, four 16-byte loads per lane ahead of the four that are worked on,
+// across the boundaries of tiles.
+constexpr uint32_t HEAD_THREADS = 512, HALF_WARPS = 8;
+
+template <int R, int GH>
+struct Codes {   // R tiles x 4 / R blocks
+  uint4 q[4];
+  uint32_t s[4][GH == 1 ? 2 : 1];
+};
+
+struct HeadPass {
+  uint32_t columns;     // per pass: feature vectors x terms
+  uint32_t vectors;     // feature vectors per pass
+  uint32_t pitch;       // bytes between columns in shared memory
+  uint32_t groups;      // R tiles each
+};
+
+__device__ __forceinline__ uint4 load_codes(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+template <typename X, int R, int NT, int GH>   // GH: 32 features per group, times
+__global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadPass ps) {
   using F = Feature<X>;
   using Op = Operand<typename F::Op>;
-  const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint64_t tile = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (tile >= a.h.tiles) return;
-  const uint4* codes = reinterpret_cast<const uint4*>(a.packed) + tile * a.h.blocks * 32;
-  const uint32_t* scales = a.packed + a.h.code_words() + tile * a.h.quads * 32;
-  for (uint64_t m0 = (uint64_t)blockIdx.y * 8; m0 < a.rows; m0 += (uint64_t)gridDim.y * 8) {
-    const uint64_t m = m0 + g;
-    const X* x = static_cast<const X*>(a.x) + (m < a.rows ? m : 0) * a.x_stride;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t b = 0; b < a.h.blocks; ++b) {
-      const uint4 q = codes[(uint64_t)b * 32 + lane];
-      const uint32_t words[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (uint32_t h = 0; h < 2; ++h) {
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const uint32_t k0 = b * 64 + h * 32;
-#pragma unroll
-        for (uint32_t j = 0; j < 2; ++j) {
-          uint16_t v[4][3];
-#pragma unroll
-          for (uint32_t e = 0; e < 4; ++e) {
-            const uint32_t k = k0 + 8 * t + 4 * j + e;
-            X xv = X(0.0f);
-            if (m < a.rows && k < a.h.features) xv = x[k];
-            terms_of(xv, v[e]);
-          }
-          uint32_t frag[4];
-          const uint32_t w = words[2 * h + j];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) frag[i] = Op::minus8((w >> (4 * i) & 0x000f000fu) | Op::BASE);
-#pragma unroll
-          for (int s = 0; s < F::TERMS; ++s)
-            Op::mma(acc, frag, v[0][s] | (uint32_t)v[1][s] << 16, v[2][s] | (uint32_t)v[3][s] << 16);
-        }
-        const uint32_t group = k0 / a.h.group;
-        if (group >= 4 * a.h.quads) continue;   // the padding of the last block
-        const uint32_t two = scales[(group / 4) * 32 + g * 4 + group % 4];
-        const float s0 = scale_f32(two & 0xffffu, a.scale_dtype), s1 = scale_f32(two >> 16, a.scale_dtype);
-        sum[0] = fmaf(s0, acc[0], sum[0]);
-        sum[1] = fmaf(s0, acc[1], sum[1]);
-        sum[2] = fmaf(s1, acc[2], sum[2]);
-        sum[3] = fmaf(s1, acc[3], sum[3]);
-      }
-    }
+  constexpr int D = 4 / R;   // blocks per step
+  extern __shared__ __align__(16) uint8_t smem[];
+  const uint32_t tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t half = tid / 256, warp = tid / 32 % HALF_WARPS;
+  uint8_t* xs = smem;
+  float* parts = reinterpret_cast<float*>(smem + ps.columns * ps.pitch) + half * (HALF_WARPS * ps.columns * R * 16);   // [warp][column][16 R]
+  const uint64_t m0 = (uint64_t)blockIdx.y * ps.vectors;
+  const uint32_t vectors = (uint32_t)min((uint64_t)ps.vectors, a.rows - m0);
+  const uint32_t per_warp = (a.h.blocks + HALF_WARPS - 1) / HALF_WARPS;
+  const uint32_t b0 = min(a.h.blocks, warp * per_warp), b1 = min(a.h.blocks, b0 + per_warp), steps = (per_warp + D - 1) / D;
+  const uint4* codes = reinterpret_cast<const uint4*>(a.packed);
+  const uint32_t* scales = a.packed + a.h.code_words();
+
+  const auto fetch = [&](uint32_t group, uint32_t step) {
+    Codes<R, GH> c;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint64_t n = tile * 16 + g + 8 * (i >> 1), r = m0 + 2 * t + (i & 1);
-      if (n < a.h.cats && r < a.rows) store_y(a.y, r * a.h.cats + n, sum[i] + (a.bias ? a.bias[n] : 0.0f), a.y_dtype);
+      const uint32_t tile = group * R + i % R, b = b0 + step * D + i / R;
+      c.q[i] = {0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u};
+      c.s[i][0] = 0;
+      if (GH == 1) c.s[i][GH == 1 ? 1 : 0] = 0;
+      if (tile < a.h.tiles && b < b1) {
+        c.q[i] = load_codes(codes + ((uint64_t)tile * a.h.blocks + b) * 32 + lane);
+        // a block's groups: two of 32 features, one of 64, half a one of 128 (the last block's second may not be there)
+        const uint32_t first = GH == 1 ? 2 * b : GH == 2 ? b : b / 2;
+        const uint32_t* s = scales + ((uint64_t)tile * a.h.quads + first / 4) * 32 + g * 4 + first % 4;
+        c.s[i][0] = s[0];
+        if (GH == 1) c.s[i][GH == 1 ? 1 : 0] = s[1];
+      }
+    }
+    return c;
+  };
+  const uint32_t stride = gridDim.x * 2;
+  uint32_t group = blockIdx.x * 2 + half;
+  Codes<R, GH> next = fetch(min(group, ps.groups - 1), 0);
+
+  // the feature vectors: eight features a time, zeros behind the last
+  const uint32_t eights = a.h.blocks * 8;
+  for (uint32_t i = tid; i < ps.vectors * eights; i += HEAD_THREADS) {
+    const uint32_t m = i / eights, k = i % eights * 8;
+    const X* x = static_cast<const X*>(a.x) + (m0 + m) * a.x_stride + k;
+    __align__(16) X v[8];
+    if (m < vectors && k + 8 <= a.h.features && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+#pragma unroll
+      for (int j = 0; j < (int)sizeof(X) / 2; ++j) reinterpret_cast<uint4*>(v)[j] = reinterpret_cast<const uint4*>(x)[j];
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) v[e] = m < vectors && k + e < a.h.features ? x[e] : X(0.0f);
+    }
+    uint16_t terms[8][3];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) terms_of(v[e], terms[e]);
+#pragma unroll
+    for (int s = 0; s < F::TERMS; ++s) {
+      uint4 w;
+      w.x = terms[0][s] | (uint32_t)terms[1][s] << 16;
+      w.y = terms[2][s] | (uint32_t)terms[3][s] << 16;
+      w.z = terms[4][s] | (uint32_t)terms[5][s] << 16;
+      w.w = terms[6][s] | (uint32_t)terms[7][s] << 16;
+      *reinterpret_cast<uint4*>(xs + (m * F::TERMS + s) * ps.pitch + k * 2) = w;
     }
   }
+  __syncthreads();
+
+  for (; group < ps.groups; group += stride) {
+    float sum[R][NT][4];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sum[r][n][0] = sum[r][n][1] = sum[r][n][2] = sum[r][n][3] = 0.0f;
+    for (uint32_t step = 0; step < steps; ++step) {
+      const Codes<R, GH> c = next;
+      const bool more = step + 1 < steps;
+      if (more || group + stride < ps.groups) next = fetch(more ? group : group + stride, more ? step + 1 : 0);
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        const uint32_t b = b0 + step * D + d;
+        if (b >= b1) continue;
+        uint4 x[2][NT];   // eight features of a column: two k16 steps
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            x[h][n] = {0, 0, 0, 0};
+            if (n * 8 + g < ps.columns) x[h][n] = *reinterpret_cast<const uint4*>(xs + (n * 8 + g) * ps.pitch + b * 128 + h * 64 + t * 16);
+          }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const uint4 q = c.q[d * R + r];
+          const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+          float acc[NT][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h == 0 || GH == 1) {
+#pragma unroll
+              for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t frag[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) frag[i] = Op::minus8((words[2 * h + j] >> (4 * i) & 0x000f000fu) | Op::BASE);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) Op::mma(acc[n], frag, j ? x[h][n].z : x[h][n].x, j ? x[h][n].w : x[h][n].y);
+            }
+            if (h == 1 || GH == 1) {
+              const uint32_t two = c.s[d * R + r][GH == 1 ? h : 0];
+              const float s0 = scale_f32(two & 0xffffu, a.scale_dtype), s1 = scale_f32(two >> 16, a.scale_dtype);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                sum[r][n][0] = fmaf(s0, acc[n][0], sum[r][n][0]);
+                sum[r][n][1] = fmaf(s0, acc[n][1], sum[r][n][1]);
+                sum[r][n][2] = fmaf(s1, acc[n][2], sum[r][n][2]);
+                sum[r][n][3] = fmaf(s1, acc[n][3], sum[r][n][3]);
+              }
+            }
+          }
+        }
+      }
+    }
+    // the warps' parts, added up in order
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t column = n * 8 + 2 * t + (i & 1);
+          if (column < ps.columns) parts[(warp * ps.columns + column) * (R * 16) + r * 16 + g + 8 * (i >> 1)] = sum[r][n][i];
+        }
+    asm volatile("bar.sync %0, 256;" ::"r"(half + 1) : "memory");
+    for (uint32_t i = tid % 256; i < vectors * (R * 16); i += 256) {
+      const uint32_t m = i / (R * 16), n = i % (R * 16);
+      float y = 0.0f;
+#pragma unroll
+      for (int s = F::TERMS - 1; s >= 0; --s) {   // the smallest term first
+        float part = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < HALF_WARPS; ++w) part += parts[(w * ps.columns + m * F::TERMS + s) * (R * 16) + n];
+        y += part;
+      }
+      const uint64_t cat = (uint64_t)group * (R * 16) + n;
+      if (cat < a.h.cats) store_y(a.y, (m0 + m) * a.h.cats + cat, y + (a.bias ? a.bias[cat] : 0.0f), a.y_dtype);
+    }
+    asm volatile("bar.sync %0, 256;" ::"r"(half + 1) : "memory");
+  }
+}
+
+// Shared memory a block may have, and the columns that one pass takes: the fewest tiles of eight that hold all feature
+// vectors, or what fits.  (More vectors than a pass takes read the weights again.)
+constexpr uint32_t HEAD_SMEM = 220 * 1024;
+
+template <typename X, int R, int NT, int GH>
+cudaError_t launch_head(const HeadArgs& a, HeadPass ps, uint32_t sms, cudaStream_t st) {
+  static PcbPerDeviceOnce once;
+  const cudaError_t e = once.run([] { return cudaFuncSetAttribute(head_kernel<X, R, NT, GH>, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM); });
+  if (e != cudaSuccess) return e;
+  ps.groups = (a.h.tiles + R - 1) / R;
+  const uint32_t smem = ps.columns * (ps.pitch + 2 * HALF_WARPS * R * 16 * (uint32_t)sizeof(float));
+  const uint32_t passes = (uint32_t)((a.rows + ps.vectors - 1) / ps.vectors);
+  head_kernel<X, R, NT, GH><<<dim3(std::min((ps.groups + 1) / 2, sms), passes), HEAD_THREADS, smem, st>>>(a, ps);
+  return cudaGetLastError();
+}
+template <typename X, int R, int NT>
+cudaError_t launch_head_group(const HeadArgs& a, const HeadPass& ps, uint32_t sms, cudaStream_t st) {
+  if (a.h.group == 32) return launch_head<X, R, NT, 1>(a, ps, sms, st);
+  if (a.h.group == 64) return launch_head<X, R, NT, 2>(a, ps, sms, st);
+  return launch_head<X, R, NT, 4>(a, ps, sms, st);
+}
+template <typename X>
+cudaError_t launch_head_of(const HeadArgs& a, uint32_t sms, cudaStream_t st) {
+  constexpr uint32_t TERMS = Feature<X>::TERMS;
+  HeadPass ps;
+  ps.pitch = a.h.blocks * 128 + 64;   // 64 modulo 128: eight lanes of a load meet all banks
+  uint32_t most = HEAD_SMEM / (ps.pitch + 2 * HALF_WARPS * 16 * (uint32_t)sizeof(float)) / TERMS;   // vectors that fit with R = 1
+  most = std::min(most, 32 / TERMS);
+  ps.vectors = (uint32_t)std::min<uint64_t>(a.rows, most);
+  ps.columns = ps.vectors * TERMS;
+  // tiles per half: as many as leave eight rounds for every half of every SM, and fit
+  const auto fits = [&](uint32_t r) { return ps.columns * (ps.pitch + 2 * HALF_WARPS * r * 16 * (uint32_t)sizeof(float)) <= HEAD_SMEM && a.h.tiles >= 16 * sms * r; };
+  const uint32_t nt = (ps.columns + 7) / 8;
+  if (nt <= 1) {
+    if (fits(4)) return launch_head_group<X, 4, 1>(a, ps, sms, st);
+    if (fits(2)) return launch_head_group<X, 2, 1>(a, ps, sms, st);
+    return launch_head_group<X, 1, 1>(a, ps, sms, st);
+  }
+  if (nt <= 2) {
+    if (fits(2)) return launch_head_group<X, 2, 2>(a, ps, sms, st);
+    return launch_head_group<X, 1, 2>(a, ps, sms, st);
+  }
+  return launch_head_group<X, 1, 4>(a, ps, sms, st);
 }
 
 }  // namespace
@@ -305,11 +476,17 @@ extern "C" int32_t pcb_head_logits(const void* packed_dev, int32_t scale_dtype, 
   PCB_REQUIRE(packed_dev && x_dev && y_dev && ((uintptr_t)packed_dev & 15) == 0, "null argument, or a packed head that is not 16-byte aligned");
   PCB_REQUIRE(is_scale_dtype(scale_dtype) && is_dtype(dtype) && is_dtype(y_dtype), "features and logits are f32, bf16 or f16, scales bf16 or f16");
   HeadArgs a{head_shape(cats, features, group), static_cast<const uint32_t*>(packed_dev), scale_dtype, y_dtype, x_dev, rows, x_row_stride, bias_dev, y_dev};
-  const dim3 grid((a.h.tiles + 3) / 4, (uint32_t)((rows + 7) / 8 < 65535 ? (rows + 7) / 8 : 65535));
   cudaStream_t st = (cudaStream_t)s;
-  if (dtype == PCB_F32) head_kernel<float><<<grid, 128, 0, st>>>(a);
-  else if (dtype == PCB_BF16) head_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a);
-  else head_kernel<__half><<<grid, 128, 0, st>>>(a);
-  PCB_CUDA(cudaGetLastError());
+  const uint32_t sms = pcb_sm_count();
+  if (sms == 0) return pcb_fail(PCB_ERR_CUDA, "no CUDA device");
+  // the vectors of a launch's passes go into its second grid dimension
+  for (uint64_t done = 0; done < rows; done += 65536) {
+    HeadArgs part = a;
+    part.rows = rows - done < 65536 ? rows - done : 65536;
+    part.x = static_cast<const uint8_t*>(x_dev) + done * x_row_stride * (dtype == PCB_F32 ? 4 : 2);
+    part.y = static_cast<uint8_t*>(y_dev) + done * cats * (y_dtype == PCB_F32 ? 4 : 2);
+    PCB_CUDA(dtype == PCB_F32 ? launch_head_of<float>(part, sms, st) : dtype == PCB_BF16 ? launch_head_of<__nv_bfloat16>(part, sms, st)
+                                                                                        : launch_head_of<__half>(part, sms, st));
+  }
   return PCB_OK;
 }

@@ -326,6 +326,17 @@ struct PcbPerDeviceOnce {
   }
 };
 
+// SMs of the current device, looked up once; 0 without a device.
+static inline uint32_t pcb_sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if ((n = known[dev & 63].load(std::memory_order_relaxed)) > 0) return (uint32_t)n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  known[dev & 63].store(n, std::memory_order_relaxed);
+  return (uint32_t)n;
+}
+
 // Counts a launch of class `cls`; with profiling on, brackets it with two events on `st`.
 // A build with -DPCB_NVTX additionally wraps every launch scope (and the passes of a step, PcbNvtxRange) in an
 // NVTX range named after its kernel class, for timeline tools; the default build has no NVTX calls.

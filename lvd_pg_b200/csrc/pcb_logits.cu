@@ -1615,16 +1615,6 @@ cudaError_t launch_evidence(const EvidenceArgs& a, cudaStream_t st) {   // the g
   return launch_evidence_of<T, Most<T>::E>(a, t, st);
 }
 
-uint32_t sm_count() {   // of the current device, looked up once
-  static std::atomic<int> known[64];
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  if ((n = known[dev & 63].load(std::memory_order_relaxed)) > 0) return (uint32_t)n;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  known[dev & 63].store(n, std::memory_order_relaxed);
-  return (uint32_t)n;
-}
-
 int32_t check_logits(const void* x, int32_t dtype, uint32_t cats, float temperature) {
   PCB_REQUIRE(x, "null logits");
   PCB_REQUIRE(dtype == PCB_F32 || dtype == PCB_BF16 || dtype == PCB_F16, "logits are f32, bf16 or f16");
@@ -1648,7 +1638,7 @@ extern "C" int32_t pcb_token_logprobs(const void* x_dev, int32_t dtype, uint64_t
   PCB_REQUIRE(top_k == 0 || (top_ids_dev && top_logp_dev), "alternatives need their outputs");
   LogprobArgs a{x_dev, rows, row_stride, cats, top_k, token_bytes, 1.0f / temperature, LOG2E / temperature, tokens_dev,
                 logp_out_dev, entropy_dev, stats_dev, top_logp_dev, top_ids_dev};
-  const uint32_t sms = sm_count();
+  const uint32_t sms = pcb_sm_count();
   if (sms == 0) return pcb_fail(PCB_ERR_CUDA, "no CUDA device");
   PCB_CUDA(dtype == PCB_F32 ? launch_rows<float>(a, sms, (cudaStream_t)s) : dtype == PCB_BF16 ? launch_rows<__nv_bfloat16>(a, sms, (cudaStream_t)s)
                                                                                           : launch_rows<__half>(a, sms, (cudaStream_t)s));

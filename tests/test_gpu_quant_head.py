@@ -34,7 +34,8 @@ def _tol(x, values, scales, group, y, bias, dtype):
 @pytest.mark.parametrize("rows,cats,features,group", [
     (1, 1, 1, 32), (2, 15, 31, 32), (3, 16, 32, 32), (1, 17, 33, 64), (8, 100, 63, 64), (9, 33, 64, 64), (5, 40, 65, 128), (7, 1000, 777, 32),
     (1, 1000, 4096, 64), (16, 250, 1030, 128), (17, 48, 2048, 64), (64, 128, 200, 32), (133, 70, 129, 64), (1, 40000, 256, 64), (3, 5000, 8192, 128),
-    (2, 64, 20000, 64), (12, 300, 9001, 32)])
+    (2, 64, 20000, 64), (12, 300, 9001, 32), (4, 90, 32768, 128), (40, 4800, 64, 64), (33, 9600, 100, 32),
+    (2, 80001, 130, 64)])
 def test_shapes(dtype, rows, cats, features, group):
     scale_dtype = torch.bfloat16 if dtype == torch.bfloat16 else torch.float16
     packed, scales, values = _codes(cats, features, group, scale_dtype, cats)

@@ -6,7 +6,7 @@ import torch
 
 from lvd_pg_b200 import _lib, api, build
 
-INVALID = 1
+INVALID, TOO_LARGE = 1, 4
 
 
 @pytest.fixture(scope="module")
@@ -76,12 +76,15 @@ def test_head_arguments(lib):
     size = C.c_uint64()
     assert lib.pcb_head_packed_bytes(16, 64, 64, C.byref(size)) == 0
     assert size.value == 16 * 64 // 2 + 128     # codes, and one quad of groups' scales
-    for cats, features, group in ((0, 64, 64), (16, 0, 64), (16, 64, 48), (16, 64, 0), (1 << 31, 64, 64), (16, 1 << 31, 64)):
+    for cats, features, group in ((0, 64, 64), (16, 0, 64), (16, 64, 48), (16, 64, 0), (1 << 31, 64, 64)):
         assert lib.pcb_head_packed_bytes(cats, features, group, C.byref(size)) == INVALID
         assert lib.pcb_head_pack(at, at, cats, features, group, at, None) == INVALID
         assert lib.pcb_head_quantize(at, 0, cats, features, group, 1, at, at, None) == INVALID
         assert lib.pcb_head_weight(at, 1, cats, features, group, at, None) == INVALID
         assert lib.pcb_head_logits(at, 1, cats, features, group, at, 0, 1, 64, None, at, 0, None) == INVALID
+    for features in (32769, 1 << 31):
+        assert lib.pcb_head_packed_bytes(16, features, 64, C.byref(size)) == TOO_LARGE
+        assert lib.pcb_head_logits(at, 1, 16, features, 64, at, 0, 1, features, None, at, 0, None) == TOO_LARGE
     assert lib.pcb_head_packed_bytes(16, 64, 64, None) == INVALID
     assert lib.pcb_head_pack(None, at, 16, 64, 64, at, None) == INVALID
     assert lib.pcb_head_pack(at, at, 16, 64, 64, at + 4, None) == INVALID          # not 16-byte aligned
