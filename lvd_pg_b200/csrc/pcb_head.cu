@@ -146,12 +146,19 @@ struct HeadArgs {
   void* y;
 };
 
-template <typename T> struct Operand;   // two 16-bit values of the tensor cores' operand type
+// Two 16-bit values of the tensor cores' operand type.  A nibble in the mantissa of BASE is BASE + code 2^offset, exactly;
+// one multiply-add takes it to code - 8.  bf16 has room for the lowest place only (three shifts per word of eight codes),
+// fp16 for two (one shift).
+template <typename T> struct Operand;
 template <> struct Operand<__nv_bfloat16> {
   static constexpr uint32_t BASE = 0x43004300u;   // 128: the codes' ulp there is 1
-  static __device__ __forceinline__ uint32_t minus8(uint32_t v) {   // (128 + code) - 136, exact
+  static __device__ __forceinline__ uint32_t minus8(uint32_t v) {   // (128 + code) - 136
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), __floats2bfloat162_rn(136.0f, 136.0f));
     return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ void weights(uint32_t w, uint32_t* a) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = minus8((w >> (4 * i) & 0x000f000fu) | BASE);
   }
   static __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -160,9 +167,19 @@ template <> struct Operand<__nv_bfloat16> {
 };
 template <> struct Operand<__half> {
   static constexpr uint32_t BASE = 0x64006400u;   // 1024
-  static __device__ __forceinline__ uint32_t minus8(uint32_t v) {
-    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&v), __floats2half2_rn(1032.0f, 1032.0f));
-    return *reinterpret_cast<const uint32_t*>(&r);
+  static __device__ __forceinline__ __half2 based(uint32_t w, uint32_t mask) {
+    const uint32_t v = (w & mask) | BASE;
+    return *reinterpret_cast<const __half2*>(&v);
+  }
+  static __device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+  static __device__ __forceinline__ void weights(uint32_t w, uint32_t* a) {
+    const __half2 lo = __floats2half2_rn(-1032.0f, -1032.0f), sixteenth = __floats2half2_rn(0.0625f, 0.0625f), hi = __floats2half2_rn(-72.0f, -72.0f);
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const uint32_t v = w >> (4 * i);
+      a[i] = bits(__hadd2(based(v, 0x000f000fu), lo));                       // 1024 + code - 1032
+      a[i + 1] = bits(__hfma2(based(v, 0x00f000f0u), sixteenth, hi));       // (1024 + 16 code) / 16 - 72
+    }
   }
   static __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -203,10 +220,10 @@ __device__ __forceinline__ void store_y(void* y, uint64_t i, float v, int32_t dt
 // across the boundaries of tiles.
 constexpr uint32_t HEAD_THREADS = 512, HALF_WARPS = 8;
 
-template <int R, int GH>
+template <bool G32>
 struct Codes {   // R tiles x 4 / R blocks
   uint4 q[4];
-  uint32_t s[4][GH == 1 ? 2 : 1];
+  uint32_t s[4][G32 ? 2 : 1];
 };
 
 struct HeadPass {
@@ -222,7 +239,7 @@ __device__ __forceinline__ uint4 load_codes(const uint4* p) {
   return v;
 }
 
-template <typename X, int R, int NT, int GH>   // GH: 32 features per group, times
+template <typename X, int R, int NT, bool G32, bool BF16_SCALES>   // G32: a block of 64 features has two groups
 __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadPass ps) {
   using F = Feature<X>;
   using Op = Operand<typename F::Op>;
@@ -235,32 +252,39 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
   const uint64_t m0 = (uint64_t)blockIdx.y * ps.vectors;
   const uint32_t vectors = (uint32_t)min((uint64_t)ps.vectors, a.rows - m0);
   const uint32_t per_warp = (a.h.blocks + HALF_WARPS - 1) / HALF_WARPS;
-  const uint32_t b0 = min(a.h.blocks, warp * per_warp), b1 = min(a.h.blocks, b0 + per_warp), steps = (per_warp + D - 1) / D;
-  const uint4* codes = reinterpret_cast<const uint4*>(a.packed);
-  const uint32_t* scales = a.packed + a.h.code_words();
+  const uint32_t b0 = min(a.h.blocks, warp * per_warp), b1 = min(a.h.blocks, b0 + per_warp), steps = (per_warp + D - 1) / D, last = b1 > b0 ? b1 - 1 : a.h.blocks - 1;
+  const uint4* codes = reinterpret_cast<const uint4*>(a.packed) + lane;
+  const uint32_t* scales = a.packed + a.h.code_words() + g * 4;
+  const uint32_t per_group = a.h.group == 128 ? 1 : 0;   // blocks share a scale in pairs
 
+  // Tiles behind the last and blocks behind the warp's are read again, but not used.
   const auto fetch = [&](uint32_t group, uint32_t step) {
-    Codes<R, GH> c;
+    Codes<G32> c;
+    const uint32_t tile = group * R, most = a.h.tiles - 1 - tile;
+    const uint4* q = codes + (uint64_t)tile * a.h.blocks * 32;
+    const uint32_t* s = scales + (uint64_t)tile * a.h.quads * 32;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t tile = group * R + i % R, b = b0 + step * D + i / R;
-      c.q[i] = {0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u};
-      c.s[i][0] = 0;
-      if (GH == 1) c.s[i][GH == 1 ? 1 : 0] = 0;
-      if (tile < a.h.tiles && b < b1) {
-        c.q[i] = load_codes(codes + ((uint64_t)tile * a.h.blocks + b) * 32 + lane);
-        // a block's groups: two of 32 features, one of 64, half a one of 128 (the last block's second may not be there)
-        const uint32_t first = GH == 1 ? 2 * b : GH == 2 ? b : b / 2;
-        const uint32_t* s = scales + ((uint64_t)tile * a.h.quads + first / 4) * 32 + g * 4 + first % 4;
-        c.s[i][0] = s[0];
-        if (GH == 1) c.s[i][GH == 1 ? 1 : 0] = s[1];
+    for (int d = 0; d < D; ++d) {
+      const uint32_t b = min(b0 + step * D + d, last), first = G32 ? 2 * b : b >> per_group, at = (first & ~3u) * 8 + (first & 3u);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint32_t rr = R == 1 ? 0 : min((uint32_t)r, most);
+        c.q[d * R + r] = load_codes(q + (rr * a.h.blocks + b) * 32);
+        const uint32_t* to = s + rr * a.h.quads * 32 + at;
+        if constexpr (G32) {
+          const uint2 two = __ldg(reinterpret_cast<const uint2*>(to));
+          c.s[d * R + r][0] = two.x;
+          c.s[d * R + r][1] = two.y;
+        } else {
+          c.s[d * R + r][0] = __ldg(to);
+        }
       }
     }
     return c;
   };
   const uint32_t stride = gridDim.x * 2;
   uint32_t group = blockIdx.x * 2 + half;
-  Codes<R, GH> next = fetch(min(group, ps.groups - 1), 0);
+  Codes<G32> next = fetch(min(group, ps.groups - 1), 0);
 
   // the feature vectors: eight features a time, zeros behind the last
   const uint32_t eights = a.h.blocks * 8;
@@ -297,7 +321,7 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
 #pragma unroll
       for (int n = 0; n < NT; ++n) sum[r][n][0] = sum[r][n][1] = sum[r][n][2] = sum[r][n][3] = 0.0f;
     for (uint32_t step = 0; step < steps; ++step) {
-      const Codes<R, GH> c = next;
+      const Codes<G32> c = next;
       const bool more = step + 1 < steps;
       if (more || group + stride < ps.groups) next = fetch(more ? group : group + stride, more ? step + 1 : 0);
 #pragma unroll
@@ -319,21 +343,21 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
           float acc[NT][4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (h == 0 || GH == 1) {
+            if (h == 0 || G32) {
 #pragma unroll
               for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               uint32_t frag[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) frag[i] = Op::minus8((words[2 * h + j] >> (4 * i) & 0x000f000fu) | Op::BASE);
+              Op::weights(words[2 * h + j], frag);
 #pragma unroll
               for (int n = 0; n < NT; ++n) Op::mma(acc[n], frag, j ? x[h][n].z : x[h][n].x, j ? x[h][n].w : x[h][n].y);
             }
-            if (h == 1 || GH == 1) {
-              const uint32_t two = c.s[d * R + r][GH == 1 ? h : 0];
-              const float s0 = scale_f32(two & 0xffffu, a.scale_dtype), s1 = scale_f32(two >> 16, a.scale_dtype);
+            if (h == 1 || G32) {
+              const uint32_t two = c.s[d * R + r][G32 ? h : 0];
+              const float s0 = BF16_SCALES ? __uint_as_float(two << 16) : scale_f32(two & 0xffffu, PCB_F16);
+              const float s1 = BF16_SCALES ? __uint_as_float(two & 0xffff0000u) : scale_f32(two >> 16, PCB_F16);
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 sum[r][n][0] = fmaf(s0, acc[n][0], sum[r][n][0]);
@@ -378,22 +402,24 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
 // vectors, or what fits.  (More vectors than a pass takes read the weights again.)
 constexpr uint32_t HEAD_SMEM = 220 * 1024;
 
-template <typename X, int R, int NT, int GH>
+template <typename X, int R, int NT, bool G32, bool BF16_SCALES>
 cudaError_t launch_head(const HeadArgs& a, HeadPass ps, uint32_t sms, cudaStream_t st) {
   static PcbPerDeviceOnce once;
-  const cudaError_t e = once.run([] { return cudaFuncSetAttribute(head_kernel<X, R, NT, GH>, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM); });
+  const cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(head_kernel<X, R, NT, G32, BF16_SCALES>, cudaFuncAttributeMaxDynamicSharedMemorySize, HEAD_SMEM);
+  });
   if (e != cudaSuccess) return e;
   ps.groups = (a.h.tiles + R - 1) / R;
   const uint32_t smem = ps.columns * (ps.pitch + 2 * HALF_WARPS * R * 16 * (uint32_t)sizeof(float));
   const uint32_t passes = (uint32_t)((a.rows + ps.vectors - 1) / ps.vectors);
-  head_kernel<X, R, NT, GH><<<dim3(std::min((ps.groups + 1) / 2, sms), passes), HEAD_THREADS, smem, st>>>(a, ps);
+  head_kernel<X, R, NT, G32, BF16_SCALES><<<dim3(std::min((ps.groups + 1) / 2, sms), passes), HEAD_THREADS, smem, st>>>(a, ps);
   return cudaGetLastError();
 }
 template <typename X, int R, int NT>
 cudaError_t launch_head_group(const HeadArgs& a, const HeadPass& ps, uint32_t sms, cudaStream_t st) {
-  if (a.h.group == 32) return launch_head<X, R, NT, 1>(a, ps, sms, st);
-  if (a.h.group == 64) return launch_head<X, R, NT, 2>(a, ps, sms, st);
-  return launch_head<X, R, NT, 4>(a, ps, sms, st);
+  const bool bf16 = a.scale_dtype == PCB_BF16;
+  if (a.h.group == 32) return bf16 ? launch_head<X, R, NT, true, true>(a, ps, sms, st) : launch_head<X, R, NT, true, false>(a, ps, sms, st);
+  return bf16 ? launch_head<X, R, NT, false, true>(a, ps, sms, st) : launch_head<X, R, NT, false, false>(a, ps, sms, st);
 }
 template <typename X>
 cudaError_t launch_head_of(const HeadArgs& a, uint32_t sms, cudaStream_t st) {
@@ -404,8 +430,8 @@ cudaError_t launch_head_of(const HeadArgs& a, uint32_t sms, cudaStream_t st) {
   most = std::min(most, 32 / TERMS);
   ps.vectors = (uint32_t)std::min<uint64_t>(a.rows, most);
   ps.columns = ps.vectors * TERMS;
-  // tiles per half: as many as leave eight rounds for every half of every SM, and fit
-  const auto fits = [&](uint32_t r) { return ps.columns * (ps.pitch + 2 * HALF_WARPS * r * 16 * (uint32_t)sizeof(float)) <= HEAD_SMEM && a.h.tiles >= 16 * sms * r; };
+  // tiles per half: as many as leave four rounds for every half of every SM, and fit
+  const auto fits = [&](uint32_t r) { return ps.columns * (ps.pitch + 2 * HALF_WARPS * r * 16 * (uint32_t)sizeof(float)) <= HEAD_SMEM && a.h.tiles >= 8 * sms * r; };
   const uint32_t nt = (ps.columns + 7) / 8;
   if (nt <= 1) {
     if (fits(4)) return launch_head_group<X, 4, 1>(a, ps, sms, st);
