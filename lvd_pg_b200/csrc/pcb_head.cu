@@ -149,6 +149,11 @@ struct HeadArgs {
 // Two 16-bit values of the tensor cores' operand type.  A nibble in the mantissa of BASE is BASE + code 2^offset, exactly;
 // one multiply-add takes it to code - 8.  bf16 has room for the lowest place only (three shifts per word of eight codes),
 // fp16 for two (one shift).
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t base) {   // one instruction
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(base));
+  return r;
+}
 template <typename T> struct Operand;
 template <> struct Operand<__nv_bfloat16> {
   static constexpr uint32_t BASE = 0x43004300u;   // 128: the codes' ulp there is 1
@@ -158,17 +163,21 @@ template <> struct Operand<__nv_bfloat16> {
   }
   static __device__ __forceinline__ void weights(uint32_t w, uint32_t* a) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = minus8((w >> (4 * i) & 0x000f000fu) | BASE);
+    for (int i = 0; i < 4; ++i) a[i] = minus8(and_or(w >> (4 * i), 0x000f000fu, BASE));
   }
   static __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ void mma_first(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {   // from zero
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
   }
 };
 template <> struct Operand<__half> {
   static constexpr uint32_t BASE = 0x64006400u;   // 1024
   static __device__ __forceinline__ __half2 based(uint32_t w, uint32_t mask) {
-    const uint32_t v = (w & mask) | BASE;
+    const uint32_t v = and_or(w, mask, BASE);
     return *reinterpret_cast<const __half2*>(&v);
   }
   static __device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
@@ -182,8 +191,12 @@ template <> struct Operand<__half> {
     }
   }
   static __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ void mma_first(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {   // from zero
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
   }
 };
 
@@ -248,7 +261,7 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
   const uint32_t tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const uint32_t half = tid / 256, warp = tid / 32 % HALF_WARPS;
   uint8_t* xs = smem;
-  float* parts = reinterpret_cast<float*>(smem + ps.columns * ps.pitch) + half * (HALF_WARPS * ps.columns * R * 16);   // [warp][column][16 R]
+  float* all_parts = reinterpret_cast<float*>(smem + ps.columns * ps.pitch) + half * 2 * (HALF_WARPS * ps.columns * R * 16);   // twice [warp][column][16 R]
   const uint64_t m0 = (uint64_t)blockIdx.y * ps.vectors;
   const uint32_t vectors = (uint32_t)min((uint64_t)ps.vectors, a.rows - m0);
   const uint32_t per_warp = (a.h.blocks + HALF_WARPS - 1) / HALF_WARPS;
@@ -313,8 +326,12 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
     }
   }
   __syncthreads();
+  const uint8_t* column[NT];   // columns behind the last: the last again, not stored
+#pragma unroll
+  for (int n = 0; n < NT; ++n) column[n] = xs + min(n * 8 + g, ps.columns - 1) * ps.pitch + t * 16;
 
-  for (; group < ps.groups; group += stride) {
+  for (uint32_t turn = 0; group < ps.groups; group += stride, turn ^= 1) {
+    float* parts = all_parts + turn * (HALF_WARPS * ps.columns * R * 16);
     float sum[R][NT][4];
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -333,8 +350,7 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            x[h][n] = {0, 0, 0, 0};
-            if (n * 8 + g < ps.columns) x[h][n] = *reinterpret_cast<const uint4*>(xs + (n * 8 + g) * ps.pitch + b * 128 + h * 64 + t * 16);
+            x[h][n] = *reinterpret_cast<const uint4*>(column[n] + b * 128 + h * 64);
           }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -343,16 +359,15 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
           float acc[NT][4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (h == 0 || G32) {
-#pragma unroll
-              for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               uint32_t frag[4];
               Op::weights(words[2 * h + j], frag);
 #pragma unroll
-              for (int n = 0; n < NT; ++n) Op::mma(acc[n], frag, j ? x[h][n].z : x[h][n].x, j ? x[h][n].w : x[h][n].y);
+              for (int n = 0; n < NT; ++n) {
+                if (j == 0 && (h == 0 || G32)) Op::mma_first(acc[n], frag, x[h][n].x, x[h][n].y);
+                else Op::mma(acc[n], frag, j ? x[h][n].z : x[h][n].x, j ? x[h][n].w : x[h][n].y);
+              }
             }
             if (h == 1 || G32) {
               const uint32_t two = c.s[d * R + r][G32 ? h : 0];
@@ -394,7 +409,7 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
       const uint64_t cat = (uint64_t)group * (R * 16) + n;
       if (cat < a.h.cats) store_y(a.y, (m0 + m) * a.h.cats + cat, y + (a.bias ? a.bias[cat] : 0.0f), a.y_dtype);
     }
-    asm volatile("bar.sync %0, 256;" ::"r"(half + 1) : "memory");
+    // the next round's parts go beside these; nobody is two rounds ahead of the slowest reader, for the barrier in between
   }
 }
 
@@ -410,7 +425,7 @@ cudaError_t launch_head(const HeadArgs& a, HeadPass ps, uint32_t sms, cudaStream
   });
   if (e != cudaSuccess) return e;
   ps.groups = (a.h.tiles + R - 1) / R;
-  const uint32_t smem = ps.columns * (ps.pitch + 2 * HALF_WARPS * R * 16 * (uint32_t)sizeof(float));
+  const uint32_t smem = ps.columns * (ps.pitch + 4 * HALF_WARPS * R * 16 * (uint32_t)sizeof(float));
   const uint32_t passes = (uint32_t)((a.rows + ps.vectors - 1) / ps.vectors);
   head_kernel<X, R, NT, G32, BF16_SCALES><<<dim3(std::min((ps.groups + 1) / 2, sms), passes), HEAD_THREADS, smem, st>>>(a, ps);
   return cudaGetLastError();
@@ -426,12 +441,12 @@ cudaError_t launch_head_of(const HeadArgs& a, uint32_t sms, cudaStream_t st) {
   constexpr uint32_t TERMS = Feature<X>::TERMS;
   HeadPass ps;
   ps.pitch = a.h.blocks * 128 + 64;   // 64 modulo 128: eight lanes of a load meet all banks
-  uint32_t most = HEAD_SMEM / (ps.pitch + 2 * HALF_WARPS * 16 * (uint32_t)sizeof(float)) / TERMS;   // vectors that fit with R = 1
+  uint32_t most = HEAD_SMEM / (ps.pitch + 4 * HALF_WARPS * 16 * (uint32_t)sizeof(float)) / TERMS;   // vectors that fit with R = 1
   most = std::min(most, 32 / TERMS);
   ps.vectors = (uint32_t)std::min<uint64_t>(a.rows, most);
   ps.columns = ps.vectors * TERMS;
   // tiles per half: as many as leave four rounds for every half of every SM, and fit
-  const auto fits = [&](uint32_t r) { return ps.columns * (ps.pitch + 2 * HALF_WARPS * r * 16 * (uint32_t)sizeof(float)) <= HEAD_SMEM && a.h.tiles >= 8 * sms * r; };
+  const auto fits = [&](uint32_t r) { return ps.columns * (ps.pitch + 4 * HALF_WARPS * r * 16 * (uint32_t)sizeof(float)) <= HEAD_SMEM && a.h.tiles >= 8 * sms * r; };
   const uint32_t nt = (ps.columns + 7) / 8;
   if (nt <= 1) {
     if (fits(4)) return launch_head_group<X, 4, 1>(a, ps, sms, st);
