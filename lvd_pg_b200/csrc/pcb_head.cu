@@ -226,12 +226,12 @@ __device__ __forceinline__ void store_y(void* y, uint64_t i, float v, int32_t dt
   else static_cast<__half*>(y)[i] = __float2half_rn(v);
 }
 
-// Persistent blocks of sixteen warps, in two halves of eight.  A half takes R tiles of 16 categories at a time; its warps
-// share the features, so that short heads fill the GPU too, and add up their parts through shared memory.  The feature
-// vectors stay in shared memory, as columns of the B operand (fp32: three columns each, one per term, joined at the end);
-// codes and scales go straight from memory to registers, four 16-byte loads per lane ahead of the four that are worked on,
-// across the boundaries of tiles.
-constexpr uint32_t HEAD_THREADS = 512, HALF_WARPS = 8;
+// Persistent blocks of sixteen warps, in teams.  A team takes R tiles of 16 categories a round; its warps share the features
+// and add up their parts through shared memory: large teams for heads with few categories, which fill the GPU so, small ones
+// where there are enough (no warp waits for others in a team of one).  The feature vectors stay in shared memory, as
+// columns of the B operand (fp32: three columns each, one per term, joined at the end); codes and scales go straight from
+// memory to registers, four 16-byte loads per lane ahead of the four that are worked on, across the boundaries of rounds.
+constexpr uint32_t HEAD_THREADS = 512, HEAD_WARPS = 16;
 
 template <bool G32>
 struct Codes {   // R tiles x 4 / R blocks
@@ -244,6 +244,7 @@ struct HeadPass {
   uint32_t vectors;     // feature vectors per pass
   uint32_t pitch;       // bytes between columns in shared memory
   uint32_t groups;      // R tiles each
+  uint32_t team;        // warps
 };
 
 __device__ __forceinline__ uint4 load_codes(const uint4* p) {
@@ -259,12 +260,12 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
   constexpr int D = 4 / R;   // blocks per step
   extern __shared__ __align__(16) uint8_t smem[];
   const uint32_t tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t half = tid / 256, warp = tid / 32 % HALF_WARPS;
+  const uint32_t team = tid / 32 / ps.team, warp = tid / 32 % ps.team, teams = HEAD_WARPS / ps.team;
   uint8_t* xs = smem;
-  float* all_parts = reinterpret_cast<float*>(smem + ps.columns * ps.pitch) + half * 2 * (HALF_WARPS * ps.columns * R * 16);   // twice [warp][column][16 R]
+  float* all_parts = reinterpret_cast<float*>(smem + ps.columns * ps.pitch) + team * 2 * (ps.team * ps.columns * R * 16);   // twice [warp][column][16 R]
   const uint64_t m0 = (uint64_t)blockIdx.y * ps.vectors;
   const uint32_t vectors = (uint32_t)min((uint64_t)ps.vectors, a.rows - m0);
-  const uint32_t per_warp = (a.h.blocks + HALF_WARPS - 1) / HALF_WARPS;
+  const uint32_t per_warp = (a.h.blocks + ps.team - 1) / ps.team;
   const uint32_t b0 = min(a.h.blocks, warp * per_warp), b1 = min(a.h.blocks, b0 + per_warp), steps = (per_warp + D - 1) / D, last = b1 > b0 ? b1 - 1 : a.h.blocks - 1;
   const uint4* codes = reinterpret_cast<const uint4*>(a.packed) + lane;
   const uint32_t* scales = a.packed + a.h.code_words() + g * 4;
@@ -295,34 +296,42 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
     }
     return c;
   };
-  const uint32_t stride = gridDim.x * 2;
-  uint32_t group = blockIdx.x * 2 + half;
+  const uint32_t stride = gridDim.x * teams;
+  uint32_t group = team * gridDim.x + blockIdx.x;   // the first round spreads over the blocks
   Codes<G32> next = fetch(min(group, ps.groups - 1), 0);
 
-  // the feature vectors: eight features a time, zeros behind the last
-  const uint32_t eights = a.h.blocks * 8;
-  for (uint32_t i = tid; i < ps.vectors * eights; i += HEAD_THREADS) {
-    const uint32_t m = i / eights, k = i % eights * 8;
-    const X* x = static_cast<const X*>(a.x) + (m0 + m) * a.x_stride + k;
-    __align__(16) X v[8];
-    if (m < vectors && k + 8 <= a.h.features && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+  // the feature vectors: eight features a time, four times that in flight per thread, zeros behind the last
+  const uint32_t eights = a.h.blocks * 8, all = ps.vectors * eights, magic = 0xffffffffu / eights + 1;   // all < 2^18, eights <= 2^12: i / eights is exact
+  for (uint32_t i0 = tid; i0 < all; i0 += 4 * HEAD_THREADS) {
+    __align__(16) X v[4][8];
 #pragma unroll
-      for (int j = 0; j < (int)sizeof(X) / 2; ++j) reinterpret_cast<uint4*>(v)[j] = reinterpret_cast<const uint4*>(x)[j];
-    } else {
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t i = i0 + u * HEAD_THREADS, m = __umulhi(i, magic), k = (i - m * eights) * 8;
+      const X* x = static_cast<const X*>(a.x) + (m0 + m) * a.x_stride + k;
+      if (i < all && m < vectors && k + 8 <= a.h.features && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
 #pragma unroll
-      for (uint32_t e = 0; e < 8; ++e) v[e] = m < vectors && k + e < a.h.features ? x[e] : X(0.0f);
+        for (int j = 0; j < (int)sizeof(X) / 2; ++j) reinterpret_cast<uint4*>(v[u])[j] = __ldg(reinterpret_cast<const uint4*>(x) + j);
+      } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) v[u][e] = i < all && m < vectors && k + e < a.h.features ? x[e] : X(0.0f);
+      }
     }
-    uint16_t terms[8][3];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) terms_of(v[e], terms[e]);
+    for (uint32_t u = 0; u < 4; ++u) {
+      const uint32_t i = i0 + u * HEAD_THREADS, m = __umulhi(i, magic), k = (i - m * eights) * 8;
+      if (i >= all) continue;
+      uint16_t terms[8][3];
 #pragma unroll
-    for (int s = 0; s < F::TERMS; ++s) {
-      uint4 w;
-      w.x = terms[0][s] | (uint32_t)terms[1][s] << 16;
-      w.y = terms[2][s] | (uint32_t)terms[3][s] << 16;
-      w.z = terms[4][s] | (uint32_t)terms[5][s] << 16;
-      w.w = terms[6][s] | (uint32_t)terms[7][s] << 16;
-      *reinterpret_cast<uint4*>(xs + (m * F::TERMS + s) * ps.pitch + k * 2) = w;
+      for (int e = 0; e < 8; ++e) terms_of(v[u][e], terms[e]);
+#pragma unroll
+      for (int s = 0; s < F::TERMS; ++s) {
+        uint4 w;
+        w.x = terms[0][s] | (uint32_t)terms[1][s] << 16;
+        w.y = terms[2][s] | (uint32_t)terms[3][s] << 16;
+        w.z = terms[4][s] | (uint32_t)terms[5][s] << 16;
+        w.w = terms[6][s] | (uint32_t)terms[7][s] << 16;
+        *reinterpret_cast<uint4*>(xs + (m * F::TERMS + s) * ps.pitch + k * 2) = w;
+      }
     }
   }
   __syncthreads();
@@ -331,7 +340,7 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
   for (int n = 0; n < NT; ++n) column[n] = xs + min(n * 8 + g, ps.columns - 1) * ps.pitch + t * 16;
 
   for (uint32_t turn = 0; group < ps.groups; group += stride, turn ^= 1) {
-    float* parts = all_parts + turn * (HALF_WARPS * ps.columns * R * 16);
+    float* parts = all_parts + turn * (ps.team * ps.columns * R * 16);
     float sum[R][NT][4];
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -395,15 +404,15 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
           const uint32_t column = n * 8 + 2 * t + (i & 1);
           if (column < ps.columns) parts[(warp * ps.columns + column) * (R * 16) + r * 16 + g + 8 * (i >> 1)] = sum[r][n][i];
         }
-    asm volatile("bar.sync %0, 256;" ::"r"(half + 1) : "memory");
-    for (uint32_t i = tid % 256; i < vectors * (R * 16); i += 256) {
+    if (ps.team == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(ps.team * 32) : "memory");
+    for (uint32_t i = warp * 32 + lane; i < vectors * (R * 16); i += ps.team * 32) {
       const uint32_t m = i / (R * 16), n = i % (R * 16);
       float y = 0.0f;
 #pragma unroll
       for (int s = F::TERMS - 1; s >= 0; --s) {   // the smallest term first
         float part = 0.0f;
-#pragma unroll
-        for (uint32_t w = 0; w < HALF_WARPS; ++w) part += parts[(w * ps.columns + m * F::TERMS + s) * (R * 16) + n];
+        for (uint32_t w = 0; w < ps.team; ++w) part += parts[(w * ps.columns + m * F::TERMS + s) * (R * 16) + n];
         y += part;
       }
       const uint64_t cat = (uint64_t)group * (R * 16) + n;
@@ -425,9 +434,9 @@ cudaError_t launch_head(const HeadArgs& a, HeadPass ps, uint32_t sms, cudaStream
   });
   if (e != cudaSuccess) return e;
   ps.groups = (a.h.tiles + R - 1) / R;
-  const uint32_t smem = ps.columns * (ps.pitch + 4 * HALF_WARPS * R * 16 * (uint32_t)sizeof(float));
+  const uint32_t smem = ps.columns * (ps.pitch + 2 * HEAD_WARPS * R * 16 * (uint32_t)sizeof(float));
   const uint32_t passes = (uint32_t)((a.rows + ps.vectors - 1) / ps.vectors);
-  head_kernel<X, R, NT, G32, BF16_SCALES><<<dim3(std::min((ps.groups + 1) / 2, sms), passes), HEAD_THREADS, smem, st>>>(a, ps);
+  head_kernel<X, R, NT, G32, BF16_SCALES><<<dim3(std::min(ps.groups, sms), passes), HEAD_THREADS, smem, st>>>(a, ps);
   return cudaGetLastError();
 }
 template <typename X, int R, int NT>
@@ -441,20 +450,32 @@ cudaError_t launch_head_of(const HeadArgs& a, uint32_t sms, cudaStream_t st) {
   constexpr uint32_t TERMS = Feature<X>::TERMS;
   HeadPass ps;
   ps.pitch = a.h.blocks * 128 + 64;   // 64 modulo 128: eight lanes of a load meet all banks
-  uint32_t most = HEAD_SMEM / (ps.pitch + 4 * HALF_WARPS * 16 * (uint32_t)sizeof(float)) / TERMS;   // vectors that fit with R = 1
+  uint32_t most = HEAD_SMEM / (ps.pitch + 2 * HEAD_WARPS * 16 * (uint32_t)sizeof(float)) / TERMS;   // vectors that fit with R = 1
   most = std::min(most, 32 / TERMS);
   ps.vectors = (uint32_t)std::min<uint64_t>(a.rows, most);
   ps.columns = ps.vectors * TERMS;
-  // tiles per half: as many as leave four rounds for every half of every SM, and fit
-  const auto fits = [&](uint32_t r) { return ps.columns * (ps.pitch + 4 * HALF_WARPS * r * 16 * (uint32_t)sizeof(float)) <= HEAD_SMEM && a.h.tiles >= 8 * sms * r; };
+  // Tiles per round (R, as many as the columns' registers allow) and warps per team.  us, R / team:
+  //   131072 x 4096, one vector   4/8 63.6   2/4 65.0   1/2 67.7        50000 x 8192, four   4/8 53.2   2/4 51.1   1/2 53.3
+  //   32000 x 2048, one           4/8 13.8   2/4 12.5   1/2 13.7        4096 x 4096, one     4/8 10.4   2/4  9.7   1/8  7.1
   const uint32_t nt = (ps.columns + 7) / 8;
+  const auto fits = [&](uint32_t r) { return ps.columns * (ps.pitch + 2 * HEAD_WARPS * r * 16 * (uint32_t)sizeof(float)) <= HEAD_SMEM; };
+  uint32_t tiles = 1;
+  ps.team = 8;
+  if (a.h.tiles >= 4 * sms && nt <= 2 && fits(2)) {
+    tiles = 2;
+    ps.team = 4;
+  }
+  if (a.h.tiles >= 24 * sms && nt <= 1 && fits(4)) {
+    tiles = 4;
+    ps.team = 8;
+  }
   if (nt <= 1) {
-    if (fits(4)) return launch_head_group<X, 4, 1>(a, ps, sms, st);
-    if (fits(2)) return launch_head_group<X, 2, 1>(a, ps, sms, st);
+    if (tiles == 4) return launch_head_group<X, 4, 1>(a, ps, sms, st);
+    if (tiles == 2) return launch_head_group<X, 2, 1>(a, ps, sms, st);
     return launch_head_group<X, 1, 1>(a, ps, sms, st);
   }
   if (nt <= 2) {
-    if (fits(2)) return launch_head_group<X, 2, 2>(a, ps, sms, st);
+    if (tiles == 2) return launch_head_group<X, 2, 2>(a, ps, sms, st);
     return launch_head_group<X, 1, 2>(a, ps, sms, st);
   }
   return launch_head_group<X, 1, 4>(a, ps, sms, st);
