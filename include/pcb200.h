@@ -318,6 +318,7 @@ enum { PCB_F32 = 0, PCB_BF16 = 1, PCB_F16 = 2 };
  *   top_ids_dev [rows, top_k] (int64), top_logp_dev [rows, top_k]: the top_k <= 32 largest, in order, of equal ones the
  *                            lowest index first, NaN before everything (top_k = 0: not written)
  *   stats_dev [rows, 2]      the row's largest logit and the sum of exp(s - max s), 8-byte aligned: what the gradient needs
+ *                            (may be NULL)
  * A row whose logits are all -inf has logp -inf everywhere, entropy 0 and gradient 0; NaN or +inf in a row makes its
  * results NaN. */
 int32_t pcb_token_logprobs(const void* x_dev, int32_t dtype, uint64_t rows, uint32_t cats, uint64_t row_stride,

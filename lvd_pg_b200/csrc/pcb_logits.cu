@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_row_kernel(Lo
       if (tid == 0) {
         if (a.tokens) a.logp[row] = token_logp(a, token, x_token, l);
         a.entropy[row] = entropy_of(s.S, s.A, ln_of(s.S));
-        reinterpret_cast<float2*>(a.stats)[row] = {s.m, s.S};
+        if (a.stats) reinterpret_cast<float2*>(a.stats)[row] = {s.m, s.S};
       }
       if (tid < a.top_k) {
         const uint64_t key = sh.best[tid];
@@ -708,7 +708,7 @@ __device__ __forceinline__ void short_results(const LogprobArgs& a, const Kept& 
   const LogScale l = log_scale<T>(shift_of<T>(k.m, a.c), k.S, a.invT);
   if (a.tokens) a.logp[row] = token_logp(a, token, x_token, l);
   a.entropy[row] = entropy_of(k.S, k.A, ln_of(k.S));
-  reinterpret_cast<float2*>(a.stats)[row] = {k.m, k.S};
+  if (a.stats) reinterpret_cast<float2*>(a.stats)[row] = {k.m, k.S};
   if (a.top_k == 1) {
     a.top_ids[row] = k.at;
     a.top_logp[row] = logp_of(k.best, l);
@@ -1632,7 +1632,7 @@ extern "C" int32_t pcb_token_logprobs(const void* x_dev, int32_t dtype, uint64_t
                                       float* top_logp_dev, pcb_stream s) {
   if (rows == 0) return PCB_OK;
   if (int32_t rc = check_logits(x_dev, dtype, cats, temperature)) return rc;
-  PCB_REQUIRE(entropy_dev && stats_dev && ((uintptr_t)stats_dev & 7) == 0, "null argument, or statistics that are not 8-byte aligned");
+  PCB_REQUIRE(entropy_dev && ((uintptr_t)stats_dev & 7) == 0, "null argument, or statistics that are not 8-byte aligned");
   PCB_REQUIRE(!tokens_dev || (logp_out_dev && (token_bytes == 4 || token_bytes == 8)), "tokens are int32 or int64 and need an output");
   PCB_REQUIRE(top_k <= MAX_TOP && top_k <= cats, "at most 32 alternatives, and no more than there are categories");
   PCB_REQUIRE(top_k == 0 || (top_ids_dev && top_logp_dev), "alternatives need their outputs");

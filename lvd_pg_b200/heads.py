@@ -46,33 +46,42 @@ def _call(dev: torch.device, fn, *args) -> None:
 
 
 def _logits(x: torch.Tensor) -> int:
-    _need(isinstance(x, torch.Tensor) and x.is_cuda, "logits must be a CUDA tensor; there is no CPU fallback")
+    if not (isinstance(x, torch.Tensor) and x.is_cuda):
+        _need(False, "logits must be a CUDA tensor; there is no CPU fallback")
     dtype = _DTYPES.get(x.dtype)
-    _need(dtype is not None, "logits are float32, bfloat16 or float16")
-    _need(x.dim() >= 1 and x.shape[-1] >= 1, "logits need at least one category")
+    if dtype is None:
+        _need(False, "logits are float32, bfloat16 or float16")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        _need(False, "logits need at least one category")
     return dtype
 
 
+def _once() -> None:
+    """Called in a backward pass: gradients are enabled there only where a gradient of the gradient is asked for."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("pcb200: this operator can be differentiated once only (create_graph=True is not supported)")
+
+
 # ---- log-probabilities --------------------------------------------------------------------------------------
-def _logprobs_forward(x2, tokens, top_k, temperature, dtype):
+def _logprobs_forward(x2, tokens, top_k, temperature, dtype, stats=None):
     rows, cats = x2.shape
     dev = x2.device
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
     entropy = torch.empty(rows, dtype=torch.float32, device=dev)
     logp = None if tokens is None else torch.empty(rows, dtype=torch.float32, device=dev)
     top_ids = torch.empty((rows, top_k), dtype=torch.int64, device=dev) if top_k else None
     top_logp = torch.empty((rows, top_k), dtype=torch.float32, device=dev) if top_k else None
     _call(dev, _lib.lib().pcb_token_logprobs, x2.data_ptr(), dtype, rows, cats, x2.stride(0), temperature,
           None if tokens is None else tokens.data_ptr(), 0 if tokens is None else tokens.element_size(), top_k,
-          None if tokens is None else logp.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+          None if tokens is None else logp.data_ptr(), entropy.data_ptr(), None if stats is None else stats.data_ptr(),
           top_ids.data_ptr() if top_k else None, top_logp.data_ptr() if top_k else None)
-    return stats, logp, entropy, top_ids, top_logp
+    return logp, entropy, top_ids, top_logp
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x2, tokens, top_k, temperature, dtype):
-        stats, logp, entropy, top_ids, top_logp = _logprobs_forward(x2, tokens, top_k, temperature, dtype)
+        stats = torch.empty((x2.shape[0], 2), dtype=torch.float32, device=x2.device)
+        logp, entropy, top_ids, top_logp = _logprobs_forward(x2, tokens, top_k, temperature, dtype, stats)
         ctx.save_for_backward(x2, tokens, stats, entropy, top_ids)
         ctx.top_k, ctx.temperature, ctx.dtype = top_k, temperature, dtype
         ctx.set_materialize_grads(False)
@@ -81,8 +90,8 @@ class _TokenLogprobs(torch.autograd.Function):
         return logp, entropy, top_ids, top_logp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logp, g_entropy, _, g_top):
+        _once()
         x2, tokens, stats, entropy, top_ids = ctx.saved_tensors
         if g_logp is None and g_entropy is None and g_top is None:
             return None, None, None, None, None
@@ -123,7 +132,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     if torch.is_grad_enabled() and logits.requires_grad:
         logp, entropy, top_ids, top_logp = _TokenLogprobs.apply(x2, tokens, top_k, temperature, dtype)
     else:
-        _, logp, entropy, top_ids, top_logp = _logprobs_forward(x2, tokens, top_k, temperature, dtype)
+        logp, entropy, top_ids, top_logp = _logprobs_forward(x2, tokens, top_k, temperature, dtype)
     if logits.dim() != 2:
         entropy = entropy.view(shape)
         if tokens is not None:
@@ -134,14 +143,9 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
 
 
 # ---- soft evidence ------------------------------------------------------------------------------------------
-def _rows_fastest(shape, dev) -> torch.Tensor:
-    rows, variables, cats = shape
-    return torch.empty((cats, variables, rows), dtype=torch.float32, device=dev).permute(2, 1, 0)
-
-
 def _evidence_forward(x, miss, temperature, dtype, stats):
     rows, variables, cats = x.shape
-    out = _rows_fastest(x.shape, x.device)
+    out = torch.empty_strided(x.shape, (1, rows, rows * variables), dtype=torch.float32, device=x.device)
     _call(x.device, _lib.lib().pcb_soft_evidence, x.data_ptr(), dtype, rows, variables, cats, x.stride(0), x.stride(1),
           None if miss is None else miss.data_ptr(), 0 if miss is None else miss.stride(0), 0 if miss is None else miss.stride(1),
           temperature, out.data_ptr(), None if stats is None else stats.data_ptr())
@@ -158,11 +162,12 @@ class _SoftEvidence(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        _once()
         x, miss, stats = ctx.saved_tensors
         rows, variables, cats = x.shape
-        g = g.permute(2, 1, 0).contiguous()   # a copy only where it is not laid out as the evidence
+        if g.stride() != (1, rows, rows * variables):   # not laid out as the evidence is
+            g = g.permute(2, 1, 0).contiguous()
         dx = torch.empty((rows, variables, cats), dtype=x.dtype, device=x.device)
         _call(x.device, _lib.lib().pcb_soft_evidence_backward, x.data_ptr(), ctx.dtype, rows, variables, cats, x.stride(0), x.stride(1),
               None if miss is None else miss.data_ptr(), 0 if miss is None else miss.stride(0), 0 if miss is None else miss.stride(1),
@@ -252,7 +257,8 @@ class QuantHead:
         float32; meant for few rows: every eight of them read the weights once."""
         _need(isinstance(x, torch.Tensor) and x.device == self.device and x.dtype in _DTYPES,
               "features must be float32, bfloat16 or float16 on the head's device")
-        _need(x.dim() >= 1 and x.shape[-1] == self.features, f"features must end in {self.features} values")
+        if x.dim() < 1 or x.shape[-1] != self.features:
+            _need(False, f"features must end in {self.features} values")
         _need(not (x.requires_grad and torch.is_grad_enabled()), "a head in 4 bits gives no gradient: detach the features")
         out_dtype = out_dtype or x.dtype
         _need(out_dtype in _DTYPES, "logits are float32, bfloat16 or float16")

@@ -287,3 +287,12 @@ def test_inputs_changed_after_the_call_are_noticed():
         x.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(out.entropy.sum(), x)
+
+
+def test_no_gradient_of_the_gradient():
+    x = make_logits(3, 40, torch.float32, 1).requires_grad_()
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(api.token_logprobs(x).entropy.sum(), x, create_graph=True)
+    y = make_logits(6, 40, torch.float32, 1).view(2, 3, 40).requires_grad_()
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(api.soft_evidence(y).sum(), y, create_graph=True)

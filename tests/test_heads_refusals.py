@@ -31,7 +31,7 @@ def test_cpu_tensors_are_refused():
 @pytest.mark.parametrize("change", [
     dict(x=None), dict(dtype=3), dict(dtype=-1), dict(cats=0), dict(cats=1 << 31), dict(temperature=0.0), dict(temperature=-1.0),
     dict(temperature=float("nan")), dict(temperature=float("inf")), dict(temperature=1e-39), dict(token_bytes=2), dict(logp=None),
-    dict(top_k=33), dict(top_k=6), dict(top_k=2, ids=None), dict(top_k=2, top=None), dict(entropy=None), dict(stats=None)])
+    dict(top_k=33), dict(top_k=6), dict(top_k=2, ids=None), dict(top_k=2, top=None), dict(entropy=None), dict(stats=12)])
 def test_token_logprobs_arguments(lib, change):
     b = _buf()
     a = dict(x=b, dtype=0, rows=1, cats=5, stride=5, temperature=1.0, tokens=b, token_bytes=8, top_k=0, logp=b, entropy=b, stats=b,
