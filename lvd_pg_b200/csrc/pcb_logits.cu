@@ -577,21 +577,62 @@ __device__ __forceinline__ V over_lanes(V v, uint32_t lg, F f) {   // f over the
   return v;
 }
 
-template <typename T, int E, bool GRANULES>
+// Granules lie where memory has them: a row that begins inside one has `off` elements of others' in front, and its ends are
+// masked in registers.  (No granule is read that reaches over an end of the tensor, [lo, hi): its elements are.)
+struct Bounds { uintptr_t lo, hi; };
+enum Form { ELEMENTS, WHOLE, LOOSE };   // read by elements; in granules that rows begin and end on; in granules wherever rows begin
+template <typename T, int E, Form FORM>
 struct ShortRow {
-  static constexpr uint32_t N = GRANULES ? Vec<T>::N : 1;
+  static constexpr uint32_t N = FORM != ELEMENTS ? Vec<T>::N : 1;
   static constexpr int W = E / (int)PER_WORD<T>;
   uint32_t w[W];
+  uint32_t off;   // of a LOOSE row
+  __device__ __forceinline__ uint32_t front() const { return FORM == LOOSE ? off : 0; }
 
-  static __device__ __forceinline__ uint32_t index(int e, uint32_t sub, uint32_t lg) { return (sub + ((uint32_t)(e / N) << lg)) * N + e % N; }
-  __device__ __forceinline__ void load(const T* x, uint32_t sub, uint32_t lg, uint32_t cats) {
-    if constexpr (GRANULES) {
+  __device__ __forceinline__ uint32_t index(int e, uint32_t sub, uint32_t lg) const {   // 2^32 - 1 and less for what lies in front
+    return (sub + ((uint32_t)(e / N) << lg)) * N + e % N - front();
+  }
+  __device__ __forceinline__ void load(const T* x, uint32_t sub, uint32_t lg, uint32_t cats, const Bounds& bounds) {
+    if constexpr (FORM == WHOLE) {
 #pragma unroll
       for (int i = 0; i < W / 4; ++i) {
         const uint32_t g = sub + ((uint32_t)i << lg);
         uint4 v = {Word<T>::NONE, Word<T>::NONE, Word<T>::NONE, Word<T>::NONE};
         if (g * N < cats) v = load16(x + g * N);
         w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+    } else if constexpr (FORM == LOOSE) {
+      off = (uint32_t)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+      const T* base = x - off;
+      const uint32_t end = off + cats;
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        const uint32_t g = sub + ((uint32_t)i << lg);
+        const T* at = base + g * N;
+        uint4 v = {Word<T>::NONE, Word<T>::NONE, Word<T>::NONE, Word<T>::NONE};
+        if (g * N < end && reinterpret_cast<uintptr_t>(at) >= bounds.lo && reinterpret_cast<uintptr_t>(at + N) <= bounds.hi) v = load16(at);
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        const uint32_t g = sub + ((uint32_t)i << lg);
+        if (g * N >= end || (g * N >= off && (g + 1) * N <= end)) continue;
+        const T* at = base + g * N;
+        const bool held = reinterpret_cast<uintptr_t>(at) >= bounds.lo && reinterpret_cast<uintptr_t>(at + N) <= bounds.hi;
+#pragma unroll
+        for (uint32_t v = 0; v < N; ++v) {
+          const uint32_t j = g * N + v, word = 4 * i + v / PER_WORD<T>;
+          const bool mine = j >= off && j < end;
+          if constexpr (sizeof(T) == 4) {
+            if (!mine) w[word] = Word<T>::NONE;
+            else if (!held) w[word] = reinterpret_cast<const uint32_t*>(at)[v];
+          } else {
+            const uint32_t shift = 16 * (v & 1);
+            uint32_t bits = mine ? w[word] >> shift & 0xffffu : Word<T>::NONE & 0xffffu;
+            if (mine && !held) bits = reinterpret_cast<const uint16_t*>(at)[v];
+            w[word] = (w[word] & (0xffff0000u >> shift)) | bits << shift;
+          }
+        }
       }
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -606,23 +647,69 @@ struct ShortRow {
       }
     }
   }
+  // W words of results to the row's places at y, which lies towards 16-byte boundaries as the row does
+  __device__ __forceinline__ void store(T* y, const uint32_t* out, uint32_t sub, uint32_t lg, uint32_t cats) const {
+    if constexpr (FORM == WHOLE) {
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        const uint32_t at = (sub + ((uint32_t)i << lg)) * N;
+        if (at < cats) *reinterpret_cast<uint4*>(y + at) = {out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]};
+      }
+    } else if constexpr (FORM == LOOSE) {
+      T* base = y - off;
+      const uint32_t end = off + cats;
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        const uint32_t g = sub + ((uint32_t)i << lg);
+        if (g * N >= off && (g + 1) * N <= end) {
+          *reinterpret_cast<uint4*>(base + g * N) = {out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]};
+        } else if (g * N < end) {
+#pragma unroll
+          for (uint32_t v = 0; v < N; ++v) {
+            const uint32_t j = g * N + v;
+            if (j < off || j >= end) continue;
+            if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(base)[j] = out[4 * i + v];
+            else reinterpret_cast<uint16_t*>(base)[j] = (uint16_t)(out[4 * i + v / 2] >> (16 * (v & 1)));
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t j = index(e, sub, lg);
+        if (j >= cats) continue;
+        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(y)[j] = out[e];
+        else reinterpret_cast<uint16_t*>(y)[j] = (uint16_t)(out[e / 2] >> (16 * (e & 1)));
+      }
+    }
+  }
+  // the element at a place of this lane
+  __device__ __forceinline__ float pick(uint32_t place) const {
+    uint32_t v = w[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) v = place / PER_WORD<T> == (uint32_t)i ? w[i] : v;
+    if constexpr (sizeof(T) == 4) return __uint_as_float(v);
+    else return place & 1 ? Word<T>::floats(v).y : Word<T>::floats(v).x;
+  }
   // NaN in its place: counts no more in the lane's maximum and equals nothing
   __device__ __forceinline__ void strike(uint32_t e, bool yes) {
     const uint32_t place = yes ? e / PER_WORD<T> : 0xffffffffu, bits = sizeof(T) == 4 ? 0x7fffffffu : e & 1 ? 0x7fff0000u : 0x7fffu;
 #pragma unroll
     for (int i = 0; i < W; ++i) w[i] |= place == (uint32_t)i ? bits : 0u;
   }
-  // the first place that holds v, 0xffffffff if none does
-  __device__ __forceinline__ uint32_t find(float v) const {
+  // the first place of the row that holds v, 0xffffffff if none does
+  __device__ __forceinline__ uint32_t find(float v, uint32_t sub) const {
+    const uint32_t front = sub == 0 ? this->front() : 0;   // places in front of the row
     uint32_t hits = 0;   // fp32: bit e; else bit i for element 2 i, 16 + i for 2 i + 1
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int e = 0; e < E; ++e) hits |= __uint_as_float(w[e]) == v ? 1u << e : 0u;
+      hits &= 0xffffffffu << front;
       return hits ? __ffs(hits) - 1 : 0xffffffffu;
     } else {
 #pragma unroll
       for (int i = 0; i < W; ++i) hits |= Word<T>::equal(w[i], v) & (0x10001u << i);
-      const uint32_t lo = hits & 0xffffu, hi = hits >> 16;
+      const uint32_t lo = hits & 0xffffu & 0xffffffffu << ((front + 1) / 2), hi = hits >> 16 & 0xffffffffu << (front / 2);
       return min(lo ? 2 * (uint32_t)__ffs(lo) - 2 : 0xffffffffu, hi ? 2 * (uint32_t)__ffs(hi) - 1 : 0xffffffffu);
     }
   }
@@ -633,9 +720,9 @@ struct Kept { float m, S, A, best; uint32_t at; };
 
 // A row's statistics, in all lanes that hold it, and its alternatives: a single one goes into `k`, several are written at
 // once (`valid`: there is such a row).
-template <typename T, int E, bool GRANULES>
-__device__ __forceinline__ Kept short_row(const LogprobArgs& a, ShortRow<T, E, GRANULES>& r, uint64_t row, bool valid, uint32_t sub, uint32_t lg) {
-  using Row = ShortRow<T, E, GRANULES>;
+template <typename T, int E, Form FORM>
+__device__ __forceinline__ Kept short_row(const LogprobArgs& a, ShortRow<T, E, FORM>& r, uint64_t row, bool valid, uint32_t sub, uint32_t lg) {
+  using Row = ShortRow<T, E, FORM>;
   Kept k;
   k.m = over_lanes(most_of_words<T, Row::W>(r.w), lg, most_of);
   const Shift from = shift_of<T>(k.m, a.c);
@@ -658,7 +745,7 @@ __device__ __forceinline__ Kept short_row(const LogprobArgs& a, ShortRow<T, E, G
       uint64_t key = 0;
 #pragma unroll 1
       for (int e = 0; e < E; ++e) {
-        const uint32_t j = Row::index(e, sub, lg);
+        const uint32_t j = r.index(e, sub, lg);
         const uint64_t o = j < a.cats ? order_key(element_of<T>(w, e), j) : 0;
         if (o < last && o > key) key = o;
       }
@@ -680,7 +767,7 @@ __device__ __forceinline__ Kept short_row(const LogprobArgs& a, ShortRow<T, E, G
   uint32_t kept_at = 0;
   for (uint32_t n = 0; n < a.top_k; ++n) {
     if (n) best = over_lanes(most_of_words<T, Row::W>(r.w), lg, most_of);
-    const uint32_t own = r.find(best), at = own == 0xffffffffu ? own : Row::index(0, sub, lg) + (((own / Row::N) << lg) * Row::N) + own % Row::N;
+    const uint32_t own = r.find(best, sub), at = own == 0xffffffffu ? own : r.index(0, sub, lg) + (((own / Row::N) << lg) * Row::N) + own % Row::N;
     const uint32_t first = over_lanes(at, lg, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
     if (a.top_k == 1) {
       k.at = first;
@@ -718,16 +805,17 @@ __device__ __forceinline__ void short_results(const LogprobArgs& a, const Kept& 
 // Rows in memory: in 16-byte granules, or element by element, whatever their distance.  A warp takes `passes` times the rows
 // that its lanes hold at once, the next ones on their way while it works on these (granules), and writes the results of all
 // of them together: lane (g, j) those of the g-th row of pass j.
-template <typename T, int E, bool GRANULES>
+template <typename T, int E, Form FORM>
 __global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_short_kernel(LogprobArgs a, uint32_t lg, uint32_t passes) {
-  using Row = ShortRow<T, E, GRANULES>;
+  using Row = ShortRow<T, E, FORM>;
   const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1), group = lane >> lg;
   const uint64_t step = (uint64_t)gridDim.x * 8 * per_warp * passes;
+  const Bounds bounds = {reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + (a.rows - 1) * a.stride + a.cats)};
   for (uint64_t r0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * per_warp * passes; r0 < a.rows; r0 += step) {
     const auto row_of = [&](uint32_t pass) { return min(a.rows - 1, r0 + pass * per_warp + group); };
     const auto row_at = [&](uint64_t row) { return static_cast<const T*>(a.x) + row * a.stride; };
     Row next;
-    next.load(row_at(row_of(0)), sub, lg, a.cats);
+    next.load(row_at(row_of(0)), sub, lg, a.cats, bounds);
     const uint64_t mine = r0 + sub * per_warp + group;   // the row whose results this lane writes
     const bool writes = sub < passes && mine < a.rows;
     int64_t token = -1;
@@ -739,10 +827,10 @@ __global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_short_kernel(Log
     Kept kept = {0.0f, 0.0f, 0.0f, 0.0f, 0};
     for (uint32_t pass = 0; pass < passes && r0 + pass * per_warp < a.rows; ++pass) {
       Row r = next;
-      if (GRANULES && pass + 1 < passes) next.load(row_at(row_of(pass + 1)), sub, lg, a.cats);
-      const Kept k = short_row<T, E, GRANULES>(a, r, row_of(pass), r0 + pass * per_warp + group < a.rows, sub, lg);
+      if (FORM != ELEMENTS && pass + 1 < passes) next.load(row_at(row_of(pass + 1)), sub, lg, a.cats, bounds);
+      const Kept k = short_row<T, E, FORM>(a, r, row_of(pass), r0 + pass * per_warp + group < a.rows, sub, lg);
       if (sub == pass) kept = k;
-      if (!GRANULES && pass + 1 < passes) next.load(row_at(row_of(pass + 1)), sub, lg, a.cats);
+      if (FORM == ELEMENTS && pass + 1 < passes) next.load(row_at(row_of(pass + 1)), sub, lg, a.cats, bounds);
     }
     if (writes) short_results<T>(a, kept, mine, token, x_token);
   }
@@ -756,7 +844,7 @@ constexpr uint32_t STAGE_BYTES = 2048 + 32;   // 32 lanes' 64 bytes, and the gra
 
 template <typename T, int E>
 __global__ void __launch_bounds__(STAGED_THREADS, 6) logprob_staged_kernel(LogprobArgs a, uint32_t lg, uint32_t rows_staged) {
-  using Row = ShortRow<T, E, false>;
+  using Row = ShortRow<T, E, ELEMENTS>;
   constexpr uint32_t WARPS = STAGED_THREADS / 32;
   __shared__ __align__(16) uint8_t stages[WARPS][STAGES][STAGE_BYTES];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1), group = lane >> lg;
@@ -797,8 +885,8 @@ __global__ void __launch_bounds__(STAGED_THREADS, 6) logprob_staged_kernel(Logpr
       for (uint32_t pass = 0; pass < (1u << lg) && i0 + pass * per_warp < n; ++pass) {
         const uint32_t i = i0 + pass * per_warp + group;
         Row r;
-        r.load(rows + min(i, n - 1) * a.cats, sub, lg, a.cats);
-        const Kept k = short_row<T, E, false>(a, r, q0 + min(i, n - 1), i < n, sub, lg);
+        r.load(rows + min(i, n - 1) * a.cats, sub, lg, a.cats, Bounds{0, 0});
+        const Kept k = short_row<T, E, ELEMENTS>(a, r, q0 + min(i, n - 1), i < n, sub, lg);
         if (sub == pass) kept = k;
       }
       if (mine < n) short_results<T>(a, kept, q0 + mine, token, is_category(a, token) ? to_f32(rows[mine * a.cats + (uint32_t)token]) : 0.0f);
@@ -809,20 +897,28 @@ __global__ void __launch_bounds__(STAGED_THREADS, 6) logprob_staged_kernel(Logpr
 }
 
 struct ShortShape {
-  bool granules, staged;   // rows begin on 16 bytes and end on them; they lie one behind the other
+  Form form;
+  bool staged;             // short rows that lie one behind the other
   uint32_t lg, each;       // log2 of the lanes per row, elements per lane
 };
-// Few lanes per row; four at least where the row has as many granules (64 contiguous bytes per load), sixteen where it
-// is read from memory by elements.
+// Few lanes per row; four at least where it is read in granules (64 contiguous bytes per load), sixteen where it is read
+// from memory by elements.  With y: results of the rows go there, and have to lie towards 16-byte boundaries as the rows do.
 template <typename T>
 ShortShape short_shape(uint32_t cats, uint64_t stride, const void* x, const void* y = nullptr) {
   ShortShape s;
-  s.granules = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | stride * sizeof(T) | (uint64_t)cats * sizeof(T)) & 15) == 0;
-  s.staged = stride == cats && (!y || ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0);
-  const uint32_t units = s.granules ? cats / Vec<T>::N : cats, wanted = s.granules ? 4 : s.staged ? 1 : 16;
+  const bool alike = !y || (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) | (stride - cats) * sizeof(T)) & 15) == 0;
+  constexpr uint32_t N = Vec<T>::N;
+  const bool whole = ((reinterpret_cast<uintptr_t>(x) | stride * sizeof(T) | (uint64_t)cats * sizeof(T)) & 15) == 0;
+  const uint32_t units = whole ? cats / N : (cats + 2 * N - 2) / N;   // granules that a row may touch
+  // (loose granules from 512 bytes on: us both directions, 800000 rows of 51 fp16 staged 170, loose 228; one way 200000 of 333
+  // bf16 188, 168)
+  s.form = alike && units <= 32 * Most<T>::E / N && (whole || cats * sizeof(T) >= 512) ? whole ? WHOLE : LOOSE : ELEMENTS;
+  s.staged = s.form == ELEMENTS && alike && stride == cats;
+  const bool granules = s.form != ELEMENTS;
+  const uint32_t parts = granules ? units : cats, most = granules ? Most<T>::E / N : Most<T>::E, wanted = granules ? 4 : s.staged ? 1 : 16;
   s.lg = 0;
-  while (s.lg < 5 && (cats > (Most<T>::E << s.lg) || (1u << s.lg) < (units < wanted ? units : wanted))) ++s.lg;
-  s.each = s.granules ? ((units + (1u << s.lg) - 1) >> s.lg) * Vec<T>::N : (cats + (1u << s.lg) - 1) >> s.lg;
+  while (s.lg < 5 && (parts > (most << s.lg) || (1u << s.lg) < std::min(parts, wanted))) ++s.lg;
+  s.each = ((parts + (1u << s.lg) - 1) >> s.lg) * (granules ? N : 1);
   return s;
 }
 
@@ -851,21 +947,27 @@ void launch_staged(const LogprobArgs& a, const ShortShape& s, uint32_t sms, cuda
   const uint32_t grid = resident_blocks<logprob_staged_kernel<T, E>, STAGED_THREADS>(sms, (a.rows + per_block - 1) / per_block);
   logprob_staged_kernel<T, E><<<grid, STAGED_THREADS, 0, st>>>(a, s.lg, rows);
 }
-template <typename T, int E, bool GRANULES>
+// passes per warp: as many as results can be written together, while the launch is a few times what fits on the GPU
+uint32_t short_passes(uint64_t rows, uint32_t lg, uint32_t sms) {
+  const uint32_t per_pass = 256u >> lg;
+  uint32_t passes = 1u << lg;
+  while (passes > 1 && rows < (uint64_t)per_pass * passes * 12 * sms) passes /= 2;
+  return passes;
+}
+template <typename T, int E, Form FORM>
 void launch_passes(const LogprobArgs& a, const ShortShape& s, uint32_t sms, cudaStream_t st) {
-  // passes per warp: as many as results can be written together, while the launch is a few times what fits on the GPU
-  const uint32_t per_pass = 256u >> s.lg;
-  uint32_t passes = 1u << s.lg;
-  while (passes > 1 && a.rows < (uint64_t)per_pass * passes * 12 * sms) passes /= 2;
+  const uint32_t per_pass = 256u >> s.lg, passes = short_passes(a.rows, s.lg, sms);
   const uint64_t blocks = (a.rows + per_pass * passes - 1) / (per_pass * passes);
-  logprob_short_kernel<T, E, GRANULES><<<(uint32_t)std::min<uint64_t>(blocks, 0x7fffffff), 256, 0, st>>>(a, s.lg, passes);
+  logprob_short_kernel<T, E, FORM><<<(uint32_t)std::min<uint64_t>(blocks, 0x7fffffff), 256, 0, st>>>(a, s.lg, passes);
 }
 template <typename T, int E>
 void launch_short_as(const LogprobArgs& a, const ShortShape& s, uint32_t sms, cudaStream_t st) {
-  if constexpr (E >= (int)Vec<T>::N)
-    if (s.granules) return launch_passes<T, E, true>(a, s, sms, st);
+  if constexpr (E >= (int)Vec<T>::N) {
+    if (s.form == WHOLE) return launch_passes<T, E, WHOLE>(a, s, sms, st);
+    if (s.form == LOOSE) return launch_passes<T, E, LOOSE>(a, s, sms, st);
+  }
   if (s.staged) return launch_staged<T, E>(a, s, sms, st);
-  launch_passes<T, E, false>(a, s, sms, st);
+  launch_passes<T, E, ELEMENTS>(a, s, sms, st);
 }
 template <typename T>
 void launch_short(const LogprobArgs& a, uint32_t sms, cudaStream_t st) {
@@ -893,12 +995,14 @@ cudaError_t launch_rows(const LogprobArgs& a, uint32_t sms, cudaStream_t st) {
   }
   const uint32_t grid = (uint32_t)(a.rows < (1u << 24) ? a.rows : 1u << 24);
   const uint64_t bytes = (uint64_t)a.cats * sizeof(T);
-  // rows of few tiles by one warp or four, where there are enough of them to fill the GPU
+  // Where there are enough rows to fill the GPU: by one warp each if they have few tiles, else by four.  (Eight warps leave the
+  // last rows to half-empty SMs: us with eight / four, 2048 rows of 131072 bf16 105.0 / 104.2, 1021 of 50021 31.7 / 25.9, 2000
+  // of 32768 fp32 56.0 / 48.3.)
   if (bytes <= 16384 && a.rows >= 16 * (uint64_t)sms) {
     logprob_row_kernel<T, 32><<<grid, 32, 0, st>>>(a, 1);
     return cudaGetLastError();
   }
-  if (bytes <= 65536 && a.rows >= 4 * (uint64_t)sms) {
+  if (a.rows >= 4 * (uint64_t)sms) {
     logprob_row_kernel<T, 128><<<grid, 128, 0, st>>>(a, 1);
     return cudaGetLastError();
   }
@@ -1000,8 +1104,7 @@ __device__ __forceinline__ void grad_words(const uint32_t* w, const RowGrad& g, 
 }
 
 // A block takes GRAD_TILE bytes of a row: 64 per thread.  Granules are those of dx; x is read in them where it lies alike
-// towards 16-byte boundaries, by elements otherwise.  What the token and the alternatives point to is written again at the
-// end.  The last rows come first: the forward pass read them last, and some of them are still in the L2 cache.
+// towards 16-byte boundaries, by elements otherwise.  The last rows come first: the forward pass read them last, and some of them are still in the L2 cache.
 constexpr uint32_t GRAD_THREADS = 256, GRAD_TILE = 64 * GRAD_THREADS;
 template <typename T>
 __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(LogprobGradArgs a, uint32_t chunks) {
@@ -1019,6 +1122,15 @@ __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(LogprobGradA
     const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
     const uint32_t g0 = chunk * STEP, g1 = min((uint32_t)(((uint64_t)p.end + N - 1) / N), g0 + STEP);
     const T* xs = x - p.off;   // x's element for place j of the granules
+    // what the token and the alternatives point to in this chunk, one thread each
+    const uint32_t n = a.g_top ? a.top_k + 1 : a.g_logp ? 1 : 0;
+    int64_t pointed = -1;
+    float x_pointed = 0.0f;
+    if (tid < n) {
+      pointed = tid > 0 ? a.top_ids[row * a.top_k + tid - 1] : a.g_logp ? token_at(a.tokens, a.token_bytes, row) : -1;
+      if (pointed < 0 || pointed >= (int64_t)a.cats || ((uint32_t)pointed + p.off) / N < g0 || ((uint32_t)pointed + p.off) / N >= g1) pointed = -1;
+      else x_pointed = to_f32(x[pointed]);
+    }
     uint32_t w[4][4];
 #pragma unroll
     for (uint32_t u = 0; u < 4; ++u) {
@@ -1061,56 +1173,57 @@ __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(LogprobGradA
           }
       }
     }
-    if (g.token >= 0 || a.g_top) {
-      __syncthreads();
-      const uint32_t first = max(g0 * N, p.off) - p.off, last = min(g1 * N, p.end) - p.off;   // the chunk's categories
-      if (tid <= (a.g_top ? a.top_k : 0)) {
-        const int64_t j = tid == 0 ? g.token : a.top_ids[row * a.top_k + tid - 1];
-        if (j >= (int64_t)first && j < (int64_t)last) dx[j] = from_f32<T>(pointed_grad(a, g, row, (uint32_t)j, to_f32(x[j])));
-      }
+    if (n > 0) {
+      __syncthreads();   // the block's stores come before these
+      if (pointed >= 0) dx[pointed] = from_f32<T>(pointed_grad(a, g, row, (uint32_t)pointed, x_pointed));
     }
-    __syncthreads();
   }
 }
 
-// Short rows, 2^lg lanes each, as in logprob_short_kernel.
-template <typename T, int E, bool GRANULES>
-__global__ void __launch_bounds__(256, E >= 32 ? 3 : E >= 16 ? 4 : 6) logprob_grad_short_kernel(LogprobGradArgs a, uint32_t lg) {
-  using Row = ShortRow<T, E, GRANULES>;
-  const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1);
-  const uint64_t warps = (a.rows + per_warp - 1) / per_warp, step = (uint64_t)gridDim.x * 8;
-  for (uint64_t i = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < warps; i += step) {
-    const uint64_t r0 = (warps - 1 - i) * per_warp, mine = r0 + (lane >> lg), row = min(a.rows - 1, mine);   // the last rows first
-    const T* x = static_cast<const T*>(a.x) + row * a.stride;
-    T* dx = static_cast<T*>(a.dx) + row * a.cats;
-    Row r;
-    r.load(x, sub, lg, a.cats);
-    const RowGrad g = row_grad<T>(a, row);
-    uint32_t out[Row::W];
-    grad_words<T, Row::W>(r.w, g, out);
-    if (mine < a.rows) {
-      if constexpr (GRANULES) {
-#pragma unroll
-        for (int n = 0; n < Row::W / 4; ++n) {
-          const uint32_t at = (sub + ((uint32_t)n << lg)) * Row::N;
-          if (at < a.cats) *reinterpret_cast<uint4*>(dx + at) = {out[4 * n], out[4 * n + 1], out[4 * n + 2], out[4 * n + 3]};
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t j = Row::index(e, sub, lg);
-          if (j >= a.cats) continue;
-          if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(dx)[j] = out[e];
-          else reinterpret_cast<uint16_t*>(dx)[j] = (uint16_t)(out[e / 2] >> (16 * (e & 1)));
-        }
+// Short rows, 2^lg lanes each, as in logprob_short_kernel: a warp takes `passes` times the rows that its lanes hold at
+// once, lane (g, j) prepares the g-th row of pass j, and the next rows are on their way while it works on these.
+template <typename T, int E, Form FORM>
+__global__ void __launch_bounds__(256, E >= 16 ? 3 : 5) logprob_grad_short_kernel(LogprobGradArgs a, uint32_t lg, uint32_t passes) {
+  using Row = ShortRow<T, E, FORM>;
+  const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1), group = lane >> lg;
+  const Bounds bounds = {reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + (a.rows - 1) * a.stride + a.cats)};
+  const uint64_t rows_each = (uint64_t)per_warp * passes, all = (a.rows + rows_each - 1) / rows_each, step = (uint64_t)gridDim.x * 8;
+  for (uint64_t i = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < all; i += step) {
+    const uint64_t r0 = (all - 1 - i) * rows_each;   // the last rows first
+    const auto row_of = [&](uint32_t pass) { return min(a.rows - 1, r0 + pass * per_warp + group); };
+    const auto row_at = [&](uint64_t row) { return static_cast<const T*>(a.x) + row * a.stride; };
+    Row next;
+    next.load(row_at(row_of(0)), sub, lg, a.cats, bounds);
+    const RowGrad mine = row_grad<T>(a, min(a.rows - 1, r0 + min(sub, passes - 1) * per_warp + group));
+    const int32_t my_token = mine.token >= 0 && mine.token < (int64_t)a.cats ? (int32_t)mine.token : -1;
+    for (uint32_t pass = 0; pass < passes && r0 + pass * per_warp < a.rows; ++pass) {
+      const Row r = next;
+      if (pass + 1 < passes) next.load(row_at(row_of(pass + 1)), sub, lg, a.cats, bounds);
+      const uint32_t from = (lane & ~((1u << lg) - 1)) + pass;   // the lane that prepared this row
+      RowGrad g;
+      g.from = shift_of<T>(__shfl_sync(0xffffffffu, mine.from.m, from), a.c);
+      g.S = __shfl_sync(0xffffffffu, mine.S, from);
+      g.alpha = __shfl_sync(0xffffffffu, mine.alpha, from);
+      g.beta = __shfl_sync(0xffffffffu, mine.beta, from);
+      g.gl = __shfl_sync(0xffffffffu, mine.gl, from);
+      g.token = __shfl_sync(0xffffffffu, my_token, from);
+      const uint64_t row = row_of(pass);
+      const bool valid = r0 + pass * per_warp + group < a.rows;
+      T* dx = static_cast<T*>(a.dx) + row * a.cats;
+      uint32_t out[Row::W];
+      grad_words<T, Row::W>(r.w, g, out);
+      if (valid) r.store(dx, out, sub, lg, a.cats);
+      if (a.g_logp) {   // the token's, by the lane that holds it, over what it has just written
+        const uint32_t j = (uint32_t)g.token, at = j + r.front(), place = ((at / Row::N) >> lg) * Row::N + at % Row::N;
+        const float x = r.pick(place);
+        if (valid && (int32_t)g.token >= 0 && ((at / Row::N) & ((1u << lg) - 1)) == sub) dx[j] = from_f32<T>(pointed_grad(a, g, row, j, x));
       }
-    }
-    if (a.g_logp || a.g_top) {
-      __syncwarp();   // the lanes' stores come before these
-      const uint32_t n = a.g_top ? a.top_k + 1 : 1;
-      for (uint32_t k = sub; k < n; k += 1u << lg) {
-        const int64_t j = k == 0 ? g.token : a.top_ids[row * a.top_k + k - 1];
-        if (mine < a.rows && j >= 0 && j < (int64_t)a.cats) dx[j] = from_f32<T>(pointed_grad(a, g, row, (uint32_t)j, to_f32(x[j])));
+      if (a.g_top) {
+        __syncwarp();   // the lanes' stores come before these
+        for (uint32_t k = sub; k < a.top_k; k += 1u << lg) {
+          const int64_t j = a.top_ids[row * a.top_k + k];
+          if (valid && j >= 0 && j < (int64_t)a.cats) dx[j] = from_f32<T>(pointed_grad(a, g, row, (uint32_t)j, to_f32(row_at(row)[j])));
+        }
       }
     }
   }
@@ -1120,7 +1233,7 @@ __global__ void __launch_bounds__(256, E >= 32 ? 3 : E >= 16 ? 4 : 6) logprob_gr
 // logits in shared memory and leaves in granules, but for those that the stage shares with its neighbours.
 template <typename T, int E>
 __global__ void __launch_bounds__(STAGED_THREADS, 6) logprob_grad_staged_kernel(LogprobGradArgs a, uint32_t lg, uint32_t rows_staged) {
-  using Row = ShortRow<T, E, false>;
+  using Row = ShortRow<T, E, ELEMENTS>;
   constexpr uint32_t WARPS = STAGED_THREADS / 32;
   __shared__ __align__(16) uint8_t stages[WARPS][STAGE_BYTES];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1), group = lane >> lg;
@@ -1148,7 +1261,7 @@ __global__ void __launch_bounds__(STAGED_THREADS, 6) logprob_grad_staged_kernel(
       const uint64_t row = q0 + r;
       T* x = rows + r * a.cats;
       Row in;
-      in.load(x, sub, lg, a.cats);
+      in.load(x, sub, lg, a.cats, Bounds{0, 0});
       const RowGrad g = row_grad<T>(a, row);
       uint32_t out[Row::W];
       grad_words<T, Row::W>(in.w, g, out);
@@ -1168,7 +1281,7 @@ __global__ void __launch_bounds__(STAGED_THREADS, 6) logprob_grad_staged_kernel(
         if (k0 == 0 && valid) {
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            const uint32_t c = Row::index(e, sub, lg);
+            const uint32_t c = in.index(e, sub, lg);
             if (c >= a.cats) continue;
             if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(x)[c] = out[e];
             else reinterpret_cast<uint16_t*>(x)[c] = (uint16_t)(out[e / 2] >> (16 * (e & 1)));
@@ -1193,31 +1306,37 @@ __global__ void __launch_bounds__(STAGED_THREADS, 6) logprob_grad_staged_kernel(
 }
 
 template <typename T, int E>
-void launch_grad_short_as(const LogprobGradArgs& a, const ShortShape& s, cudaStream_t st) {
+void launch_grad_short_as(const LogprobGradArgs& a, const ShortShape& s, uint32_t sms, cudaStream_t st) {
   const uint32_t lg = s.lg;
-  if (s.staged && !s.granules) {
+  if (s.staged) {
     const uint32_t rows = staged_rows<T>(a.cats, lg), per_block = rows * (STAGED_THREADS / 32);
     const uint64_t n = (a.rows + per_block - 1) / per_block;
     logprob_grad_staged_kernel<T, E><<<(uint32_t)std::min<uint64_t>(n, 0x7fffffff), STAGED_THREADS, 0, st>>>(a, lg, rows);
     return;
   }
-  const uint64_t blocks = (a.rows + (256u >> lg) - 1) / (256u >> lg);
+  const uint32_t passes = short_passes(a.rows, lg, sms);
+  const uint64_t blocks = (a.rows + (uint64_t)(256u >> lg) * passes - 1) / ((uint64_t)(256u >> lg) * passes);
   const uint32_t grid = (uint32_t)std::min<uint64_t>(blocks, 0x7fffffff);
-  if constexpr (E >= (int)Vec<T>::N)
-    if (s.granules) {
-      logprob_grad_short_kernel<T, E, true><<<grid, 256, 0, st>>>(a, lg);
+  if constexpr (E >= (int)Vec<T>::N) {
+    if (s.form == WHOLE) {
+      logprob_grad_short_kernel<T, E, WHOLE><<<grid, 256, 0, st>>>(a, lg, passes);
       return;
     }
-  logprob_grad_short_kernel<T, E, false><<<grid, 256, 0, st>>>(a, lg);
+    if (s.form == LOOSE) {
+      logprob_grad_short_kernel<T, E, LOOSE><<<grid, 256, 0, st>>>(a, lg, passes);
+      return;
+    }
+  }
+  logprob_grad_short_kernel<T, E, ELEMENTS><<<grid, 256, 0, st>>>(a, lg, passes);
 }
 template <typename T>
-void launch_grad(const LogprobGradArgs& a, cudaStream_t st) {
+void launch_grad(const LogprobGradArgs& a, uint32_t sms, cudaStream_t st) {
   if (a.cats <= 32 * Most<T>::E) {
     const ShortShape s = short_shape<T>(a.cats, a.stride, a.x, a.dx);
-    if (s.each <= 4) launch_grad_short_as<T, 4>(a, s, st);
-    else if (s.each <= 8) launch_grad_short_as<T, 8>(a, s, st);
-    else if (s.each <= 16) launch_grad_short_as<T, 16>(a, s, st);
-    else launch_grad_short_as<T, Most<T>::E>(a, s, st);
+    if (s.each <= 4) launch_grad_short_as<T, 4>(a, s, sms, st);
+    else if (s.each <= 8) launch_grad_short_as<T, 8>(a, s, sms, st);
+    else if (s.each <= 16) launch_grad_short_as<T, 16>(a, s, sms, st);
+    else launch_grad_short_as<T, Most<T>::E>(a, s, sms, st);
     return;
   }
   const uint32_t chunks = (uint32_t)(((uint64_t)a.cats + 2 * Vec<T>::N) * sizeof(T) / GRAD_TILE + 1);
@@ -1250,13 +1369,16 @@ struct EvidenceTile {
   uint32_t cap;         // columns of a tile
   uint32_t vars;        // variables per tile (1 where a variable has more than cap categories)
   uint32_t row_tiles, var_tiles, lg, each;   // tiles of rows and of variables; lanes per distribution (log2), elements per lane
-  bool granules;        // distributions begin on 16 bytes and end on them
+  Form form;
 };
 
 template <typename T>
 __host__ __device__ __forceinline__ uint32_t tile_place(uint32_t column, uint32_t lg) {
   return column * EV_PITCH + (sizeof(T) == 4 ? (column >> 5) << (5 - lg) : 0);
 }
+
+// a granule's columns from here on are EV_PITCH apart
+template <typename T> __device__ __forceinline__ bool tile_run(uint32_t column) { return sizeof(T) == 2 || column % Vec<T>::N == 0; }
 
 // The distributions of a tile: q = row * vars + variable.
 struct TileOrder {
@@ -1322,12 +1444,13 @@ __device__ float2 stream_row(const T* x, uint32_t cats, float c) {
   return {s.m, s.S};
 }
 
-template <typename T, int E, bool GRANULES>
-__global__ void __launch_bounds__(EV_THREADS, sizeof(T) == 4 ? 4 : 5) evidence_kernel(EvidenceArgs a, EvidenceTile et) {
-  using Row = ShortRow<T, E, GRANULES>;
+template <typename T, int E, Form FORM>
+__global__ void __launch_bounds__(EV_THREADS, sizeof(T) == 4 || FORM == ELEMENTS ? 4 : 5) evidence_kernel(EvidenceArgs a, EvidenceTile et) {
+  using Row = ShortRow<T, E, FORM>;
   extern __shared__ __align__(16) float tile[];
   __shared__ float2 streamed[32];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = et.lg, sub = lane & ((1u << lg) - 1), per_pass = EV_THREADS >> lg;
+  const Bounds bounds = {reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + (a.rows - 1) * a.row_stride + (a.vars - 1) * a.var_stride + a.cats)};
   const uint64_t b0 = (uint64_t)blockIdx.x * 32;   // neighbouring blocks write neighbouring rows
   for (uint32_t vt = blockIdx.y; vt < et.var_tiles; vt += gridDim.y) {
     const uint32_t v0 = vt * et.vars, nv = min(et.vars, a.vars - v0);
@@ -1347,7 +1470,7 @@ __global__ void __launch_bounds__(EV_THREADS, sizeof(T) == 4 ? 4 : 5) evidence_k
       for (uint32_t q0 = 0; q0 < rows * nv; q0 += per_pass) {
         const uint32_t q = q0 + (threadIdx.x >> lg), qq = min(q, rows * nv - 1), r = order.row(qq), v = qq - r * nv;
         Row in;
-        in.load(x + r * a.row_stride + v * a.var_stride + c0, sub, lg, n);
+        in.load(x + r * a.row_stride + v * a.var_stride + c0, sub, lg, n, bounds);
         const uint64_t b = b0 + r;
         const bool missing = a.miss && a.miss[b * a.miss_row_stride + (v0 + v) * a.miss_var_stride];
         float m, S;
@@ -1362,14 +1485,19 @@ __global__ void __launch_bounds__(EV_THREADS, sizeof(T) == 4 ? 4 : 5) evidence_k
         }
         if (a.stats_out && c0 == 0 && sub == 0 && q == qq) reinterpret_cast<float2*>(a.stats_out)[b * a.vars + v0 + v] = {m, S};
         const LogScale l = log_scale<T>(shift_of<T>(m, a.c), S, a.invT);
-        const uint32_t column = v * a.cats + sub * Row::N;
-        const uint32_t mine = q == qq ? n : 0;   // a place is written where it lies below
+        const uint32_t column = v * a.cats, mine = q == qq ? n : 0;   // a place is written where it lies below
 #pragma unroll
         for (int e = 0; e < E; e += Row::N) {
-          if (sub * Row::N + (((uint32_t)e) << lg) >= mine) continue;
-          float* at = tile + tile_place<T>(column + ((uint32_t)e << lg), lg) + r;
+          const uint32_t first = in.index(e, sub, lg);
+          if (first < mine && first + Row::N <= mine && tile_run<T>(column + first)) {
+            float* at = tile + tile_place<T>(column + first, lg) + r;
 #pragma unroll
-          for (uint32_t h = 0; h < Row::N; ++h) at[h * EV_PITCH] = missing ? 0.0f : logp_of(element_of<T>(in.w, e + h), l);
+            for (uint32_t h = 0; h < Row::N; ++h) at[h * EV_PITCH] = missing ? 0.0f : logp_of(element_of<T>(in.w, e + h), l);
+          } else {
+#pragma unroll
+            for (uint32_t h = 0; h < Row::N; ++h)
+              if (first + h < mine) tile[tile_place<T>(column + first + h, lg) + r] = missing ? 0.0f : logp_of(element_of<T>(in.w, e + h), l);
+          }
         }
       }
       __syncthreads();
@@ -1381,12 +1509,13 @@ __global__ void __launch_bounds__(EV_THREADS, sizeof(T) == 4 ? 4 : 5) evidence_k
 }
 
 // dx_c = (g_c - p_c sum g) / T
-template <typename T, int E, bool GRANULES>
-__global__ void __launch_bounds__(EV_THREADS, GRANULES ? 4 : 3) evidence_grad_kernel(EvidenceArgs a, EvidenceTile et) {
-  using Row = ShortRow<T, E, GRANULES>;
+template <typename T, int E, Form FORM>
+__global__ void __launch_bounds__(EV_THREADS, FORM == WHOLE ? 4 : 3) evidence_grad_kernel(EvidenceArgs a, EvidenceTile et) {
+  using Row = ShortRow<T, E, FORM>;
   extern __shared__ __align__(16) float tile[];
   __shared__ float part[EV_WARPS][32];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = et.lg, sub = lane & ((1u << lg) - 1), per_pass = EV_THREADS >> lg;
+  const Bounds bounds = {reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + (a.rows - 1) * a.row_stride + (a.vars - 1) * a.var_stride + a.cats)};
   const uint64_t b0 = (uint64_t)blockIdx.x * 32;
   for (uint32_t vt = blockIdx.y; vt < et.var_tiles; vt += gridDim.y) {
     const uint32_t v0 = vt * et.vars, nv = min(et.vars, a.vars - v0);
@@ -1404,23 +1533,44 @@ __global__ void __launch_bounds__(EV_THREADS, GRANULES ? 4 : 3) evidence_grad_ke
     for (uint32_t c0 = 0; c0 < a.cats; c0 += width) {
       const uint32_t n = min(width, a.cats - c0);
       const float* gc = g + a.rows * ((uint64_t)a.vars * c0);
-      if (lane < rows) tile_columns(n, nv, a.rows, a.vars, gc, [&](uint32_t column, const float* at) { tile[tile_place<T>(column, lg) + lane] = *at; });
+      if (lane < rows) {
+        uint32_t c = warp;
+        if (nv == 1) {   // eight loads in flight
+          const uint64_t step = a.rows * a.vars * EV_WARPS;
+          const float* at = gc + a.rows * a.vars * warp;
+          for (; c + 7 * EV_WARPS < n; c += 8 * EV_WARPS) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k, at += step) v[k] = *at;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) tile[tile_place<T>(c + k * EV_WARPS, lg) + lane] = v[k];
+          }
+          for (; c < n; c += EV_WARPS, at += step) tile[tile_place<T>(c, lg) + lane] = *at;
+        } else {
+          tile_columns(n, nv, a.rows, a.vars, gc, [&](uint32_t column, const float* at) { tile[tile_place<T>(column, lg) + lane] = *at; });
+        }
+      }
       __syncthreads();
       for (uint32_t q0 = 0; q0 < rows * nv; q0 += per_pass) {
         const uint32_t q = q0 + (threadIdx.x >> lg), qq = min(q, rows * nv - 1), r = order.row(qq), v = qq - r * nv;
         Row in;
-        in.load(x + r * a.row_stride + v * a.var_stride + c0, sub, lg, n);
+        in.load(x + r * a.row_stride + v * a.var_stride + c0, sub, lg, n, bounds);
         const uint64_t b = b0 + r;
         const bool missing = a.miss && a.miss[b * a.miss_row_stride + (v0 + v) * a.miss_var_stride];
         const float2 st = reinterpret_cast<const float2*>(a.stats)[b * a.vars + v0 + v];
-        const uint32_t column = v * a.cats + sub * Row::N;
+        const uint32_t column = v * a.cats;
         float ge[E], sum = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; e += Row::N) {
-          const bool there = sub * Row::N + ((uint32_t)e << lg) < n;
-          const float* at = tile + tile_place<T>(column + (there ? (uint32_t)e << lg : 0), lg) + r;
+          const uint32_t first = in.index(e, sub, lg);
+          if (first < n && first + Row::N <= n && tile_run<T>(column + first)) {
+            const float* at = tile + tile_place<T>(column + first, lg) + r;
 #pragma unroll
-          for (uint32_t h = 0; h < Row::N; ++h) ge[e + h] = there ? at[h * EV_PITCH] : 0.0f;
+            for (uint32_t h = 0; h < Row::N; ++h) ge[e + h] = at[h * EV_PITCH];
+          } else {
+#pragma unroll
+            for (uint32_t h = 0; h < Row::N; ++h) ge[e + h] = first + h < n ? tile[tile_place<T>(column + first + h, lg) + r] : 0.0f;
+          }
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) sum += ge[e];
@@ -1449,24 +1599,7 @@ __global__ void __launch_bounds__(EV_THREADS, GRANULES ? 4 : 3) evidence_grad_ke
             out[e / 2] = Word<T>::bits(__floats2bfloat162_rn(value.x, value.y));
           }
         }
-        T* to = dx + ((uint64_t)r * a.vars + v) * a.cats + c0;
-        if (q == qq) {
-          if constexpr (GRANULES) {
-#pragma unroll
-            for (int j = 0; j < Row::W / 4; ++j) {
-              const uint32_t at = (sub + ((uint32_t)j << lg)) * Row::N;
-              if (at < n) *reinterpret_cast<uint4*>(to + at) = {out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]};
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-              const uint32_t j = Row::index(e, sub, lg);
-              if (j >= n) continue;
-              if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(to)[j] = out[e];
-              else reinterpret_cast<uint16_t*>(to)[j] = (uint16_t)(out[e / 2] >> (16 * (e & 1)));
-            }
-          }
-        }
+        if (q == qq) in.store(dx + ((uint64_t)r * a.vars + v) * a.cats + c0, out, sub, lg, n);
       }
       __syncthreads();
     }
@@ -1559,37 +1692,45 @@ EvidenceTile evidence_tile(const EvidenceArgs& a) {
   t.cap = t.vars > 1 ? t.vars * a.cats : a.cats <= EV_MOST<T> ? a.cats : EV_COLUMNS;
   t.row_tiles = (uint32_t)((a.rows + 31) / 32);
   t.var_tiles = (a.vars - 1) / t.vars + 1;
-  uint64_t at = reinterpret_cast<uintptr_t>(a.x) | (a.row_stride | (a.vars > 1 ? a.var_stride : 0) | a.cats) * sizeof(T);
-  if (a.dx) at |= reinterpret_cast<uintptr_t>(a.dx);   // contiguous: as the categories are
-  t.granules = (at & 15) == 0;
-  // few lanes per distribution; four at least where it has as many granules, eight where it is read by elements
-  const uint32_t n = std::min(a.cats, t.cap), units = t.granules ? n / Vec<T>::N : n, wanted = t.granules ? 4 : 8;
+  constexpr uint32_t N = Vec<T>::N;
+  const auto whole_at = [&](uint64_t row, uint64_t var) { return ((row | (a.vars > 1 ? var : 0)) * sizeof(T) & 15) == 0; };
+  const bool whole = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && whole_at(a.row_stride, a.var_stride) && a.cats % N == 0;
+  // dx is contiguous: it has to lie towards 16-byte boundaries as x does
+  const bool alike = !a.dx || (((reinterpret_cast<uintptr_t>(a.x) ^ reinterpret_cast<uintptr_t>(a.dx)) & 15) == 0 &&
+                               whole_at(a.row_stride - (uint64_t)a.vars * a.cats, a.var_stride - a.cats));
+  const uint32_t n = std::min(a.cats, t.cap), units = whole ? n / N : (n + 2 * N - 2) / N;
+  t.form = alike && units <= 32 * Most<T>::E / N && (whole || n * sizeof(T) >= 64) ? whole ? WHOLE : LOOSE : ELEMENTS;
+  const bool granules = t.form != ELEMENTS;
+  // few lanes per distribution; four at least where it is read in granules, eight where it is read by elements
+  const uint32_t parts = granules ? units : n, most = granules ? Most<T>::E / N : Most<T>::E, wanted = granules ? 4 : 8;
   t.lg = 0;
-  while (t.lg < 5 && (n > (Most<T>::E << t.lg) || (1u << t.lg) < std::min(units, wanted))) ++t.lg;
-  t.each = t.granules ? ((units + (1u << t.lg) - 1) >> t.lg) * Vec<T>::N : (n + (1u << t.lg) - 1) >> t.lg;
+  while (t.lg < 5 && (parts > (most << t.lg) || (1u << t.lg) < std::min(parts, wanted))) ++t.lg;
+  t.each = ((parts + (1u << t.lg) - 1) >> t.lg) * (granules ? N : 1);
   return t;
 }
 
-template <typename T, int E, bool GRANULES>
+template <typename T, int E, Form FORM>
 cudaError_t launch_evidence_as(const EvidenceArgs& a, const EvidenceTile& t, cudaStream_t st) {
   const dim3 grid(t.row_tiles, std::min(t.var_tiles, 65535u));
   const uint32_t smem = (tile_place<T>(t.cap, t.lg) + 32) * (uint32_t)sizeof(float);
   static PcbPerDeviceOnce once;
   const cudaError_t e = once.run([] {
     const int most = (int)((tile_place<T>(768, 0) + 32) * sizeof(float));
-    const cudaError_t f = cudaFuncSetAttribute(evidence_kernel<T, E, GRANULES>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    return f != cudaSuccess ? f : cudaFuncSetAttribute(evidence_grad_kernel<T, E, GRANULES>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    const cudaError_t f = cudaFuncSetAttribute(evidence_kernel<T, E, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    return f != cudaSuccess ? f : cudaFuncSetAttribute(evidence_grad_kernel<T, E, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   });
   if (e != cudaSuccess) return e;
-  if (a.dx) evidence_grad_kernel<T, E, GRANULES><<<grid, EV_THREADS, smem, st>>>(a, t);
-  else evidence_kernel<T, E, GRANULES><<<grid, EV_THREADS, smem, st>>>(a, t);
+  if (a.dx) evidence_grad_kernel<T, E, FORM><<<grid, EV_THREADS, smem, st>>>(a, t);
+  else evidence_kernel<T, E, FORM><<<grid, EV_THREADS, smem, st>>>(a, t);
   return cudaGetLastError();
 }
 template <typename T, int E>
 cudaError_t launch_evidence_of(const EvidenceArgs& a, const EvidenceTile& t, cudaStream_t st) {
-  if constexpr (E >= (int)Vec<T>::N)
-    if (t.granules) return launch_evidence_as<T, E, true>(a, t, st);
-  return launch_evidence_as<T, E, false>(a, t, st);
+  if constexpr (E >= (int)Vec<T>::N) {
+    if (t.form == WHOLE) return launch_evidence_as<T, E, WHOLE>(a, t, st);
+    if (t.form == LOOSE) return launch_evidence_as<T, E, LOOSE>(a, t, st);
+  }
+  return launch_evidence_as<T, E, ELEMENTS>(a, t, st);
 }
 template <typename T, int C>
 cudaError_t launch_thin(const EvidenceArgs& a, const EvidenceTile& t, cudaStream_t st) {
@@ -1658,9 +1799,11 @@ extern "C" int32_t pcb_token_logprobs_backward(const void* x_dev, int32_t dtype,
   PCB_REQUIRE(!g_top_dev || (top_k > 0 && top_ids_dev), "a gradient of the alternatives needs their indices");
   LogprobGradArgs a{x_dev, rows, row_stride, g_logp_stride, g_entropy_stride, cats, top_k, token_bytes, 1.0f / temperature,
                     LOG2E / temperature, tokens_dev, top_ids_dev, stats_dev, entropy_dev, g_logp_dev, g_entropy_dev, g_top_dev, dx_dev};
-  if (dtype == PCB_F32) launch_grad<float>(a, (cudaStream_t)s);
-  else if (dtype == PCB_BF16) launch_grad<__nv_bfloat16>(a, (cudaStream_t)s);
-  else launch_grad<__half>(a, (cudaStream_t)s);
+  const uint32_t sms = pcb_sm_count();
+  if (sms == 0) return pcb_fail(PCB_ERR_CUDA, "no CUDA device");
+  if (dtype == PCB_F32) launch_grad<float>(a, sms, (cudaStream_t)s);
+  else if (dtype == PCB_BF16) launch_grad<__nv_bfloat16>(a, sms, (cudaStream_t)s);
+  else launch_grad<__half>(a, sms, (cudaStream_t)s);
   PCB_CUDA(cudaGetLastError());
   return PCB_OK;
 }
