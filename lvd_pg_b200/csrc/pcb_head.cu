@@ -537,14 +537,17 @@ extern "C" int32_t pcb_head_logits(const void* packed_dev, int32_t scale_dtype, 
   if (rows == 0) return PCB_OK;
   PCB_REQUIRE(packed_dev && x_dev && y_dev && ((uintptr_t)packed_dev & 15) == 0, "null argument, or a packed head that is not 16-byte aligned");
   PCB_REQUIRE(is_scale_dtype(scale_dtype) && is_dtype(dtype) && is_dtype(y_dtype), "features and logits are f32, bf16 or f16, scales bf16 or f16");
+  PCB_REQUIRE(((uintptr_t)x_dev & (dtype == PCB_F32 ? 3 : 1)) == 0 && ((uintptr_t)y_dev & (y_dtype == PCB_F32 ? 3 : 1)) == 0,
+              "features or logits that are not aligned to their own size");
   HeadArgs a{head_shape(cats, features, group), static_cast<const uint32_t*>(packed_dev), scale_dtype, y_dtype, x_dev, rows, x_row_stride, bias_dev, y_dev};
   cudaStream_t st = (cudaStream_t)s;
   const uint32_t sms = pcb_sm_count();
   if (sms == 0) return pcb_fail(PCB_ERR_CUDA, "no CUDA device");
   // the vectors of a launch's passes go into its second grid dimension
-  for (uint64_t done = 0; done < rows; done += 65536) {
+  constexpr uint64_t AT_ONCE = 65535;
+  for (uint64_t done = 0; done < rows; done += AT_ONCE) {
     HeadArgs part = a;
-    part.rows = rows - done < 65536 ? rows - done : 65536;
+    part.rows = std::min(rows - done, AT_ONCE);
     part.x = static_cast<const uint8_t*>(x_dev) + done * x_row_stride * (dtype == PCB_F32 ? 4 : 2);
     part.y = static_cast<uint8_t*>(y_dev) + done * cats * (y_dtype == PCB_F32 ? 4 : 2);
     PCB_CUDA(dtype == PCB_F32 ? launch_head_of<float>(part, sms, st) : dtype == PCB_BF16 ? launch_head_of<__nv_bfloat16>(part, sms, st)

@@ -569,8 +569,23 @@ template <> struct Most<float> { static constexpr uint32_t E = 16; };
 template <> struct Most<__nv_bfloat16> { static constexpr uint32_t E = 32; };
 template <> struct Most<__half> { static constexpr uint32_t E = 32; };
 
-__device__ __forceinline__ float most_of(float x, float y) { return fmaxf(x, y); }
 __device__ __forceinline__ float sum_of(float x, float y) { return x + y; }
+// the largest value over the 2^lg lanes of a row (NaN does not count), and the smallest index: one instruction where a warp
+// holds one row
+__device__ __forceinline__ float most_over_lanes(float v, uint32_t lg) {
+  if (lg == 5) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+  }
+  for (uint32_t o = 1u << lg >> 1; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ uint32_t least_over_lanes(uint32_t v, uint32_t lg) {
+  if (lg == 5) return __reduce_min_sync(0xffffffffu, v);
+  for (uint32_t o = 1u << lg >> 1; o; o >>= 1) v = min(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
 template <typename V, typename F>
 __device__ __forceinline__ V over_lanes(V v, uint32_t lg, F f) {   // f over the 2^lg lanes of a row
   for (uint32_t o = 1u << lg >> 1; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -724,7 +739,7 @@ template <typename T, int E, Form FORM>
 __device__ __forceinline__ Kept short_row(const LogprobArgs& a, ShortRow<T, E, FORM>& r, uint64_t row, bool valid, uint32_t sub, uint32_t lg) {
   using Row = ShortRow<T, E, FORM>;
   Kept k;
-  k.m = over_lanes(most_of_words<T, Row::W>(r.w), lg, most_of);
+  k.m = most_over_lanes(most_of_words<T, Row::W>(r.w), lg);
   const Shift from = shift_of<T>(k.m, a.c);
   float2 S2 = {0.0f, 0.0f}, A2 = {0.0f, 0.0f};
   add_words<T, Row::W>(r.w, from, S2, A2);
@@ -766,9 +781,9 @@ __device__ __forceinline__ Kept short_row(const LogprobArgs& a, ShortRow<T, E, F
   float best = k.m, kept = 0.0f;
   uint32_t kept_at = 0;
   for (uint32_t n = 0; n < a.top_k; ++n) {
-    if (n) best = over_lanes(most_of_words<T, Row::W>(r.w), lg, most_of);
+    if (n) best = most_over_lanes(most_of_words<T, Row::W>(r.w), lg);
     const uint32_t own = r.find(best, sub), at = own == 0xffffffffu ? own : r.index(0, sub, lg) + (((own / Row::N) << lg) * Row::N) + own % Row::N;
-    const uint32_t first = over_lanes(at, lg, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
+    const uint32_t first = least_over_lanes(at, lg);
     if (a.top_k == 1) {
       k.at = first;
       break;
@@ -1475,7 +1490,7 @@ __global__ void __launch_bounds__(EV_THREADS, sizeof(T) == 4 || FORM == ELEMENTS
         const bool missing = a.miss && a.miss[b * a.miss_row_stride + (v0 + v) * a.miss_var_stride];
         float m, S;
         if (one) {
-          m = over_lanes(most_of_words<T, Row::W>(in.w), lg, most_of);
+          m = most_over_lanes(most_of_words<T, Row::W>(in.w), lg);
           float2 S2 = {0.0f, 0.0f}, none = {0.0f, 0.0f};
           add_words<T, Row::W, false>(in.w, shift_of<T>(m, a.c), S2, none);
           S = over_lanes(S2.x + S2.y, lg, sum_of);
@@ -1743,7 +1758,7 @@ cudaError_t launch_thin(const EvidenceArgs& a, const EvidenceTile& t, cudaStream
 template <typename T>
 cudaError_t launch_evidence(const EvidenceArgs& a, cudaStream_t st) {   // the gradient where dx is given
   const EvidenceTile t = evidence_tile<T>(a);
-  if (t.vars > 1 && a.cats <= 32) {
+  if (a.cats <= 32 && (t.vars > 1 || a.vars == 1)) {
     if (a.cats <= 2) return launch_thin<T, 2>(a, t, st);
     if (a.cats <= 4) return launch_thin<T, 4>(a, t, st);
     if (a.cats <= 8) return launch_thin<T, 8>(a, t, st);
@@ -1794,6 +1809,7 @@ extern "C" int32_t pcb_token_logprobs_backward(const void* x_dev, int32_t dtype,
   if (rows == 0) return PCB_OK;
   if (int32_t rc = check_logits(x_dev, dtype, cats, temperature)) return rc;
   PCB_REQUIRE(stats_dev && entropy_dev && dx_dev, "null argument");
+  PCB_REQUIRE(((uintptr_t)dx_dev & (dtype == PCB_F32 ? 3 : 1)) == 0, "a gradient that is not aligned to its own size");
   PCB_REQUIRE(!g_logp_dev || (tokens_dev && (token_bytes == 4 || token_bytes == 8)), "a gradient of logp needs the tokens, int32 or int64");
   PCB_REQUIRE(top_k <= MAX_TOP && top_k <= cats, "at most 32 alternatives, and no more than there are categories");
   PCB_REQUIRE(!g_top_dev || (top_k > 0 && top_ids_dev), "a gradient of the alternatives needs their indices");
@@ -1830,6 +1846,7 @@ extern "C" int32_t pcb_soft_evidence_backward(const void* x_dev, int32_t dtype, 
   if (rows == 0 || vars == 0) return PCB_OK;
   if (int32_t rc = check_logits(x_dev, dtype, cats, temperature)) return rc;
   PCB_REQUIRE(stats_dev && g_dev && dx_dev, "null argument");
+  PCB_REQUIRE(((uintptr_t)dx_dev & (dtype == PCB_F32 ? 3 : 1)) == 0, "a gradient that is not aligned to its own size");
   EvidenceArgs a{x_dev, rows, row_stride, var_stride, miss_row_stride, miss_var_stride, vars, cats, 1.0f / temperature,
                  LOG2E / temperature, miss_dev, nullptr, nullptr, stats_dev, g_dev, dx_dev};
   PCB_REQUIRE(((uintptr_t)stats_dev & 7) == 0, "statistics that are not 8-byte aligned");

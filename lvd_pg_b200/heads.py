@@ -199,7 +199,8 @@ class QuantHead:
     """A categorical head y = x W^T + bias for serving, its weights W [cats, features] in 4 bits: W[n, k] =
     scales[n, k // group] * (code - 8), codes 0..15, 16-bit scales.  `QuantHead(weight)` quantises (scale = max |w| / 7 of the
     group); `QuantHead.from_codes` takes codes and scales that another program made.  The weights are laid out once, on
-    construction, on the weight's device; calls keep nothing.  For inference: features that require a gradient are refused."""
+    construction, on the weight's device; calls keep nothing.  A captured graph holds their address: keep the head while it
+    lives.  For inference: features that require a gradient are refused."""
 
     def __init__(self, weight: torch.Tensor, group: int = 64, bias: Optional[torch.Tensor] = None):
         _need(isinstance(weight, torch.Tensor) and weight.is_cuda and weight.dim() == 2 and weight.dtype in _DTYPES,
@@ -237,16 +238,26 @@ class QuantHead:
         if bias is not None:
             _need(isinstance(bias, torch.Tensor) and bias.device == self.device and tuple(bias.shape) == (self.cats,),
                   "bias must be [cats] on the codes' device")
-            bias = bias.detach().float().contiguous()
+            bias = bias.detach().to(torch.float32, copy=True).contiguous()
         self.bias, self._scale_dtype = bias, _DTYPES[scales.dtype]
         lib, size = _lib.lib(), C.c_uint64()
         _lib.check(lib.pcb_head_packed_bytes(self.cats, self.features, self.group, C.byref(size)))
         self.packed = torch.empty(size.value, dtype=torch.uint8, device=self.device)
         _call(self.device, lib.pcb_head_pack, codes.data_ptr(), scales.data_ptr(), self.cats, self.features, self.group,
               self.packed.data_ptr())
+        self._made_on = torch._C._cuda_getCurrentRawStream(self.device.index)
+
+    def _hold(self) -> None:
+        """Weights that another stream than their own reads are not handed out again before it is done."""
+        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._made_on:
+            stream = torch.cuda.current_stream(self.device)
+            self.packed.record_stream(stream)
+            if self.bias is not None:
+                self.bias.record_stream(stream)
 
     def weight(self) -> torch.Tensor:
         """The weights that the codes stand for, [cats, features] float32."""
+        self._hold()
         out = torch.empty((self.cats, self.features), dtype=torch.float32, device=self.device)
         _call(self.device, _lib.lib().pcb_head_weight, self.packed.data_ptr(), self._scale_dtype, self.cats, self.features, self.group,
               out.data_ptr())
@@ -265,6 +276,7 @@ class QuantHead:
         x2 = x if x.dim() == 2 else x.reshape(-1, self.features)
         if x2.stride(1) != 1 and self.features > 1:
             x2 = x2.contiguous()
+        self._hold()
         y = torch.empty((x2.shape[0], self.cats), dtype=out_dtype, device=self.device)
         _call(self.device, _lib.lib().pcb_head_logits, self.packed.data_ptr(), self._scale_dtype, self.cats, self.features, self.group,
               x2.data_ptr(), _DTYPES[x.dtype], x2.shape[0], x2.stride(0), None if self.bias is None else self.bias.data_ptr(), y.data_ptr(),

@@ -211,3 +211,33 @@ def test_refusals_on_the_device():
         assert e.value.code == 1
     with torch.no_grad():
         head.logits(x.clone().requires_grad_())
+
+
+def test_more_vectors_than_one_launch_takes():
+    packed, scales, values = _codes(20, 40, 32, torch.bfloat16, 1)
+    bias = torch.randn(20, device="cuda")
+    head = api.QuantHead.from_codes(packed, scales, 40, 32, bias=bias)
+    x = torch.randn(70001, 40, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    want = x.double() @ _weight(values, scales, 32).t() + bias.double()
+    assert_within(head.logits(x, torch.float32), want, _tol(x, values, scales, 32, want, bias, torch.float32))
+    bias.zero_()   # the head has its own
+    assert_within(head.logits(x[:9], torch.float32), want[:9], _tol(x[:9], values, scales, 32, want[:9], head.bias, torch.float32))
+
+
+def test_a_head_used_and_dropped_on_another_stream():
+    side = torch.cuda.Stream()
+    packed, scales, values = _codes(3000, 512, 64, torch.bfloat16, 2)
+    x = torch.randn(4, 512, device="cuda").bfloat16()
+    want = api.QuantHead.from_codes(packed, scales, 512, 64).logits(x)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        head = api.QuantHead.from_codes(packed, scales, 512, 64)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = head.logits(x)
+        size = head.packed.numel()
+        del head
+        junk = torch.full((size,), 255, dtype=torch.uint8, device="cuda")   # would take the weights' place
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del junk

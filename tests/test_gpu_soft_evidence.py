@@ -51,7 +51,8 @@ def _check(x, miss, temperature=1.0, g=None):
 @pytest.mark.parametrize("rows,variables,cats,temperature", [
     (1, 1, 1, 1.0), (1, 3, 2, 1.0), (70, 5, 2, 0.7), (33, 2, 3, 1.0), (31, 4, 16, 1.0), (64, 3, 31, 1.3), (5, 9, 33, 1.0), (100, 3, 64, 1.0),
     (37, 3, 200, 1.0), (32, 2, 256, 1.0), (130, 2, 257, 0.5), (9, 2, 500, 1.0), (40, 2, 513, 1.0), (33, 2, 1000, 1.0), (20, 1, 1024, 1.0),
-    (65, 1, 2049, 1.0), (3, 2, 5003, 1.0), (34, 1, 40000, 0.8)])
+    (65, 1, 2049, 1.0), (3, 2, 5003, 1.0), (34, 1, 40000, 0.8), (300, 1, 7, 1.0), (40, 300, 3, 1.0), (35, 20, 30, 1.0), (70, 9, 41, 1.0),
+    (33, 3, 130, 1.0), (32, 3, 767, 1.0), (40, 2, 1023, 1.0)])
 def test_shapes(dtype, rows, variables, cats, temperature):
     x = _logits(rows, variables, cats, dtype, rows + cats)
     _check(x, None, temperature)

@@ -53,7 +53,8 @@ def _check(x, tokens, top_k, temperature=1.0, grads=(1, 1, 1)):
     (1, 1, 1, 1.0), (5, 2, 0, 0.7), (33, 2, 2, 1.0), (7, 3, 3, 2.0), (64, 31, 5, 1.0), (9, 32, 32, 1.3), (17, 33, 1, 1.0),
     (40, 200, 4, 1.0), (513, 256, 1, 1.0), (3, 257, 20, 0.5), (12, 1000, 7, 1.0), (5, 1024, 32, 1.0), (4, 1025, 20, 1.0),
     (300, 1500, 8, 0.8), (2, 4099, 32, 1.0), (700, 4096, 3, 1.0), (1, 32000, 20, 1.0), (3, 50021, 5, 0.8), (2, 131072, 20, 1.0),
-    (1, 262147, 32, 1.0), (1, 1000003, 4, 1.0)])
+    (1, 262147, 32, 1.0), (1, 1000003, 4, 1.0), (2500, 1999, 5, 1.0), (700, 33001, 6, 0.9), (2400, 5000, 2, 1.0),
+    (40000, 7, 3, 1.0), (9000, 63, 2, 1.0), (5000, 333, 12, 1.0), (30000, 128, 1, 1.0), (160, 9000, 32, 1.0)])
 def test_shapes(dtype, rows, cats, top_k, temperature):
     _check(make_logits(rows, cats, dtype, rows + cats), _tokens(rows, cats), top_k, temperature)
 
