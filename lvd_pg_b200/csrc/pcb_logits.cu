@@ -96,9 +96,11 @@ __device__ __forceinline__ Shift shift_of(float m, float c) {
 __device__ __forceinline__ float scaled(const Shift& s, float x) {   // d, clamped; x finite or not
   return max_nan(s.near ? fmaf(x, s.c, -s.mc) : (x - s.m) * s.c, NO_MASS);
 }
+// what rounding m c has left off
+__device__ __forceinline__ float left_off(const Shift& s) { return s.near ? fmaf(s.m, s.c, -s.mc) : 0.0f; }
 // log2 of the factor between powers counted from a and from b
 __device__ __forceinline__ float between(const Shift& a, const Shift& b) {
-  return max_nan(a.near && b.near ? a.mc - b.mc : (a.m - b.m) * a.c, NO_MASS);
+  return max_nan(a.near && b.near ? a.mc - b.mc : fmaf(a.m - b.m, a.c, left_off(b) - left_off(a)), NO_MASS);
 }
 
 struct Stat { float m, S, A; };   // maximum, sum of 2^d, sum of 2^d d
@@ -216,7 +218,7 @@ struct LogScale { float m, invT, ln; };
 template <typename T>
 __device__ __forceinline__ LogScale log_scale(const Shift& s, float S, float invT) {
   const float ln = S == 0.0f ? 0.0f : logf(S);
-  return {finite_shift(s.m), invT, s.near ? fmaf(-LN2, fmaf(s.m, s.c, -s.mc), ln) : ln};
+  return {finite_shift(s.m), invT, fmaf(-LN2, left_off(s), ln)};
 }
 __device__ __forceinline__ float logp_of(float x, const LogScale& l) { return fmaf(x - l.m, l.invT, -l.ln); }
 __device__ __forceinline__ float ln_of(float S) { return S == 0.0f ? 0.0f : logf(S); }

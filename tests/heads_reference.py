@@ -89,9 +89,10 @@ def rounding(value, dtype):
 
 
 def assert_within(got, want, tol, what=""):
-    """Equal infinities and NaN in the same places, everything else within the bound; past the range of fp32 is infinite."""
+    """Equal infinities and NaN in the same places, everything else within the bound; past the range of got's type is infinite."""
+    most = torch.finfo(got.dtype).max   # of fp16: 65504, so that a gradient of 1 / T = 1e6 is infinite
     got, want = got.detach().double(), want.double()
-    want = torch.where(want.abs() > torch.finfo(torch.float32).max, want.sign() * np.inf, want)
+    want = torch.where(want.abs() > most, want.sign() * np.inf, want)
     assert got.shape == want.shape, (what, got.shape, want.shape)
     assert torch.equal(torch.isnan(got), torch.isnan(want)), what
     special = torch.isnan(want) | torch.isinf(want)

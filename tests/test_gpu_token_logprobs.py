@@ -98,6 +98,31 @@ def test_masks(dtype, cats, temperature):
     assert (torch.autograd.grad([out.entropy, out.logp], empty, [torch.ones(2, device="cuda")] * 2)[0] == 0).all()
 
 
+@pytest.mark.parametrize("cats", [30, 300, 3000, 40000])
+@pytest.mark.parametrize("temperature", [1.0, 40.0, 150.0])
+def test_logits_near_the_lowest_of_half_precision(cats, temperature):
+    """Where what stands for impossible categories would still weigh beside the row's own: the sums change their form at a
+    line that goes through the row."""
+    gen = torch.Generator().manual_seed(cats)
+    x = -65504 + 12000 * torch.rand(6, cats, generator=gen)
+    x[1] = -65504 + 300 * torch.rand(cats, generator=gen)
+    x[2, ::3] = -math.inf
+    x[3, : cats // 2] = -65504
+    _check(x.half().cuda(), _tokens(6, cats), 3, temperature)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("temperature", [1e-6, 1e-3, 1e4, 1e20])
+def test_extreme_temperatures_and_offsets(dtype, temperature):
+    for cats in (50, 2500):
+        x = make_logits(5, cats, dtype, 3)
+        x[1] += 1000.0
+        x[2] *= 0.0
+        x[3, 1:] = -math.inf
+        x = x.to(dtype)
+        _check(x, _tokens(5, cats), 2, temperature, (1, 0, 0) if temperature < 1e-2 else (1, 1, 1))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("cats", [5, 300, 3000, 40000])
 def test_nan_and_inf_stay_in_their_rows(dtype, cats):
