@@ -413,32 +413,36 @@ __device__ __forceinline__ void short_results(const LogprobArgs& a, const Kept& 
 // Rows in memory: in 16-byte granules, or element by element, whatever their distance.  A warp takes `passes` times the rows
 // that its lanes hold at once, the next ones on their way while it works on these (granules), and writes the results of all
 // of them together: lane (g, j) those of the g-th row of pass j.
-template <typename T, int E, Form FORM>
-__global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_short_kernel(LogprobArgs a, uint32_t lg, uint32_t passes) {
+template <typename T, int E, Form FORM, int LG>
+__global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_short_kernel(LogprobArgs a, uint32_t lanes_log2, uint32_t passes) {
   using Row = ShortRow<T, E, FORM>;
+  const uint32_t lg = LG >= 0 ? LG : lanes_log2;
   const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1), group = lane >> lg;
   const uint64_t step = (uint64_t)gridDim.x * 8 * per_warp * passes;
   const Bounds bounds = {reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + (a.rows - 1) * a.stride + a.cats)};
   for (uint64_t r0 = ((uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * per_warp * passes; r0 < a.rows; r0 += step) {
-    const auto row_of = [&](uint32_t pass) { return min(a.rows - 1, r0 + pass * per_warp + group); };
-    const auto row_at = [&](uint64_t row) { return static_cast<const T*>(a.x) + row * a.stride; };
+    const uint64_t first = min(a.rows - 1, r0 + group);
+    const uint32_t there = (uint32_t)min((uint64_t)passes, (a.rows - r0 + per_warp - 1) / per_warp);   // passes with rows
+    const uint32_t last = (uint32_t)min((uint64_t)passes, (a.rows - 1 - first) / per_warp);            // this lane's last pass with a row
+    const T* x = static_cast<const T*>(a.x) + first * a.stride;
+    const auto row_at = [&](uint32_t pass) { return x + (uint64_t)(min(pass, last) * per_warp) * a.stride; };
     Row next;
-    next.load(row_at(row_of(0)), sub, lg, a.cats, bounds);
+    next.load(row_at(0), sub, lg, a.cats, bounds);
     const uint64_t mine = r0 + sub * per_warp + group;   // the row whose results this lane writes
     const bool writes = sub < passes && mine < a.rows;
     int64_t token = -1;
     float x_token = 0.0f;
     if (writes && a.tokens) {
       token = token_at(a.tokens, a.token_bytes, mine);
-      if (is_category(a, token)) x_token = to_f32(row_at(mine)[token]);
+      if (is_category(a, token)) x_token = to_f32((static_cast<const T*>(a.x) + mine * a.stride)[token]);
     }
     Kept kept = {0.0f, 0.0f, 0.0f, 0.0f, 0};
-    for (uint32_t pass = 0; pass < passes && r0 + pass * per_warp < a.rows; ++pass) {
+    for (uint32_t pass = 0; pass < there; ++pass) {
       Row r = next;
-      if (FORM != ELEMENTS && pass + 1 < passes) next.load(row_at(row_of(pass + 1)), sub, lg, a.cats, bounds);
-      const Kept k = short_row<T, E, FORM>(a, r, row_of(pass), r0 + pass * per_warp + group < a.rows, sub, lg);
+      if (FORM != ELEMENTS && pass + 1 < there) next.load(row_at(pass + 1), sub, lg, a.cats, bounds);
+      const Kept k = short_row<T, E, FORM>(a, r, first + pass * per_warp, r0 + group < a.rows && pass <= last, sub, lg);
       if (sub == pass) kept = k;
-      if (FORM == ELEMENTS && pass + 1 < passes) next.load(row_at(row_of(pass + 1)), sub, lg, a.cats, bounds);
+      if (FORM == ELEMENTS && pass + 1 < there) next.load(row_at(pass + 1), sub, lg, a.cats, bounds);
     }
     if (writes) short_results<T>(a, kept, mine, token, x_token);
   }
@@ -524,7 +528,11 @@ template <typename T, int E, Form FORM>
 void launch_passes(const LogprobArgs& a, const ShortShape& s, uint32_t sms, cudaStream_t st) {
   const uint32_t per_pass = 256u >> s.lg, passes = short_passes(a.rows, s.lg, sms);
   const uint64_t blocks = (a.rows + per_pass * passes - 1) / (per_pass * passes);
-  logprob_short_kernel<T, E, FORM><<<(uint32_t)std::min<uint64_t>(blocks, 0x7fffffff), 256, 0, st>>>(a, s.lg, passes);
+  const uint32_t grid = (uint32_t)std::min<uint64_t>(blocks, 0x7fffffff);
+#define PCB_CALL(LG) logprob_short_kernel<T, E, FORM, LG><<<grid, 256, 0, st>>>(a, s.lg, passes)
+  if constexpr (FORM != ELEMENTS && E == (int)Most<T>::E) PCB_LANES(true, s.lg, PCB_CALL);
+  else PCB_CALL(-1);
+#undef PCB_CALL
 }
 template <typename T, int E>
 void launch_short_as(const LogprobArgs& a, const ShortShape& s, uint32_t sms, cudaStream_t st) {

@@ -263,16 +263,19 @@ __device__ __forceinline__ float most_over_lanes(float v, uint32_t lg) {
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
   }
+#pragma unroll
   for (uint32_t o = 1u << lg >> 1; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 __device__ __forceinline__ uint32_t least_over_lanes(uint32_t v, uint32_t lg) {
   if (lg == 5) return __reduce_min_sync(0xffffffffu, v);
+#pragma unroll
   for (uint32_t o = 1u << lg >> 1; o; o >>= 1) v = min(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 template <typename V, typename F>
 __device__ __forceinline__ V over_lanes(V v, uint32_t lg, F f) {   // f over the 2^lg lanes of a row
+#pragma unroll
   for (uint32_t o = 1u << lg >> 1; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
@@ -450,6 +453,17 @@ uint32_t staged_rows(uint32_t cats, uint32_t lg) {
   const uint32_t per_warp = 32u >> lg, fit = std::min(2048 / (cats * (uint32_t)sizeof(T)), STAGED_ROWS_MOST);
   return fit >= 32 ? fit / 32 * 32 : fit > per_warp ? fit / per_warp * per_warp : per_warp;
 }
+// CALL(LG) for the lanes per row that a kernel instance is made for: known when it is compiled where a lane's registers are
+// full (few lanes: shuffles without loops), -1 (its argument says) otherwise.
+#define PCB_LANES(full, lg, CALL)  \
+  do {                             \
+    if ((full) && (lg) == 2) CALL(2);      \
+    else if ((full) && (lg) == 3) CALL(3); \
+    else if ((full) && (lg) == 4) CALL(4); \
+    else if ((full) && (lg) == 5) CALL(5); \
+    else CALL(-1);                 \
+  } while (0)
+
 // passes per warp: as many as results can be written together, while the launch is a few times what fits on the GPU
 inline uint32_t short_passes(uint64_t rows, uint32_t lg, uint32_t sms) {
   const uint32_t per_pass = 256u >> lg;

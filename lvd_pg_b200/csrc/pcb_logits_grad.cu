@@ -167,23 +167,27 @@ __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(LogprobGradA
 
 // Short rows, 2^lg lanes each, as in logprob_short_kernel: a warp takes `passes` times the rows that its lanes hold at
 // once, lane (g, j) prepares the g-th row of pass j, and the next rows are on their way while it works on these.
-template <typename T, int E, Form FORM>
-__global__ void __launch_bounds__(256, E >= 16 ? 3 : 5) logprob_grad_short_kernel(LogprobGradArgs a, uint32_t lg, uint32_t passes) {
+template <typename T, int E, Form FORM, int LG>
+__global__ void __launch_bounds__(256, E >= 16 ? 3 : 5) logprob_grad_short_kernel(LogprobGradArgs a, uint32_t lanes_log2, uint32_t passes) {
   using Row = ShortRow<T, E, FORM>;
+  const uint32_t lg = LG >= 0 ? LG : lanes_log2;
   const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1), group = lane >> lg;
   const Bounds bounds = {reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + (a.rows - 1) * a.stride + a.cats)};
   const uint64_t rows_each = (uint64_t)per_warp * passes, all = (a.rows + rows_each - 1) / rows_each, step = (uint64_t)gridDim.x * 8;
   for (uint64_t i = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < all; i += step) {
-    const uint64_t r0 = (all - 1 - i) * rows_each;   // the last rows first
-    const auto row_of = [&](uint32_t pass) { return min(a.rows - 1, r0 + pass * per_warp + group); };
-    const auto row_at = [&](uint64_t row) { return static_cast<const T*>(a.x) + row * a.stride; };
+    const uint64_t r0 = (all - 1 - i) * rows_each, first = min(a.rows - 1, r0 + group);   // the last rows first
+    const uint32_t there = (uint32_t)min((uint64_t)passes, (a.rows - r0 + per_warp - 1) / per_warp);   // passes with rows
+    const uint32_t last = (uint32_t)min((uint64_t)passes, (a.rows - 1 - first) / per_warp);            // this lane's last pass with a row
+    const T* x = static_cast<const T*>(a.x) + first * a.stride;
+    T* dx0 = static_cast<T*>(a.dx) + first * a.cats;
+    const auto row_at = [&](uint32_t pass) { return x + (uint64_t)(min(pass, last) * per_warp) * a.stride; };
     Row next;
-    next.load(row_at(row_of(0)), sub, lg, a.cats, bounds);
+    next.load(row_at(0), sub, lg, a.cats, bounds);
     const RowGrad mine = row_grad<T>(a, min(a.rows - 1, r0 + min(sub, passes - 1) * per_warp + group));
     const int32_t my_token = mine.token >= 0 && mine.token < (int64_t)a.cats ? (int32_t)mine.token : -1;
-    for (uint32_t pass = 0; pass < passes && r0 + pass * per_warp < a.rows; ++pass) {
+    for (uint32_t pass = 0; pass < there; ++pass) {
       const Row r = next;
-      if (pass + 1 < passes) next.load(row_at(row_of(pass + 1)), sub, lg, a.cats, bounds);
+      if (pass + 1 < there) next.load(row_at(pass + 1), sub, lg, a.cats, bounds);
       const uint32_t from = (lane & ~((1u << lg) - 1)) + pass;   // the lane that prepared this row
       RowGrad g;
       g.from = shift_of<T>(__shfl_sync(0xffffffffu, mine.from.m, from), a.c);
@@ -192,9 +196,9 @@ __global__ void __launch_bounds__(256, E >= 16 ? 3 : 5) logprob_grad_short_kerne
       g.beta = __shfl_sync(0xffffffffu, mine.beta, from);
       g.gl = __shfl_sync(0xffffffffu, mine.gl, from);
       g.token = __shfl_sync(0xffffffffu, my_token, from);
-      const uint64_t row = row_of(pass);
-      const bool valid = r0 + pass * per_warp + group < a.rows;
-      T* dx = static_cast<T*>(a.dx) + row * a.cats;
+      const uint64_t row = first + min(pass, last) * per_warp;
+      const bool valid = r0 + group < a.rows && pass <= last;
+      T* dx = dx0 + (uint64_t)(min(pass, last) * per_warp) * a.cats;
       uint32_t out[Row::W];
       grad_words<T, Row::W>(r.w, g, out);
       if (valid) r.store(dx, out, sub, lg, a.cats);
@@ -207,7 +211,7 @@ __global__ void __launch_bounds__(256, E >= 16 ? 3 : 5) logprob_grad_short_kerne
         __syncwarp();   // the lanes' stores come before these
         for (uint32_t k = sub; k < a.top_k; k += 1u << lg) {
           const int64_t j = a.top_ids[row * a.top_k + k];
-          if (valid && j >= 0 && j < (int64_t)a.cats) dx[j] = from_f32<T>(pointed_grad(a, g, row, (uint32_t)j, to_f32(row_at(row)[j])));
+          if (valid && j >= 0 && j < (int64_t)a.cats) dx[j] = from_f32<T>(pointed_grad(a, g, row, (uint32_t)j, to_f32(row_at(pass)[j])));
         }
       }
     }
@@ -302,17 +306,25 @@ void launch_grad_short_as(const LogprobGradArgs& a, const ShortShape& s, uint32_
   const uint32_t passes = short_passes(a.rows, lg, sms);
   const uint64_t blocks = (a.rows + (uint64_t)(256u >> lg) * passes - 1) / ((uint64_t)(256u >> lg) * passes);
   const uint32_t grid = (uint32_t)std::min<uint64_t>(blocks, 0x7fffffff);
+#define PCB_CALL(LG) logprob_grad_short_kernel<T, E, FORM, LG><<<grid, 256, 0, st>>>(a, lg, passes)
+  constexpr bool full = E == (int)Most<T>::E;
   if constexpr (E >= (int)Vec<T>::N) {
     if (s.form == WHOLE) {
-      logprob_grad_short_kernel<T, E, WHOLE><<<grid, 256, 0, st>>>(a, lg, passes);
+      constexpr Form FORM = WHOLE;
+      if constexpr (full) PCB_LANES(true, lg, PCB_CALL);
+      else PCB_CALL(-1);
       return;
     }
     if (s.form == LOOSE) {
-      logprob_grad_short_kernel<T, E, LOOSE><<<grid, 256, 0, st>>>(a, lg, passes);
+      constexpr Form FORM = LOOSE;
+      if constexpr (full) PCB_LANES(true, lg, PCB_CALL);
+      else PCB_CALL(-1);
       return;
     }
   }
-  logprob_grad_short_kernel<T, E, ELEMENTS><<<grid, 256, 0, st>>>(a, lg, passes);
+  constexpr Form FORM = ELEMENTS;
+  PCB_CALL(-1);
+#undef PCB_CALL
 }
 template <typename T>
 void launch_grad(const LogprobGradArgs& a, uint32_t sms, cudaStream_t st) {
