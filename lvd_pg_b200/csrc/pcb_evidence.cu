@@ -106,12 +106,12 @@ __device__ float2 stream_row(const T* x, uint32_t cats, float c) {
   return {s.m, s.S};
 }
 
-template <typename T, int E, Form FORM>
+template <typename T, int E, Form FORM, int LG>
 __global__ void __launch_bounds__(EV_THREADS, sizeof(T) == 4 || FORM == ELEMENTS ? 4 : 5) evidence_kernel(EvidenceArgs a, EvidenceTile et) {
   using Row = ShortRow<T, E, FORM>;
   extern __shared__ __align__(16) float tile[];
   __shared__ float2 streamed[32];
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = et.lg, sub = lane & ((1u << lg) - 1), per_pass = EV_THREADS >> lg;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = LG >= 0 ? (uint32_t)LG : et.lg, sub = lane & ((1u << lg) - 1), per_pass = EV_THREADS >> lg;
   const Bounds bounds = {reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + (a.rows - 1) * a.row_stride + (a.vars - 1) * a.var_stride + a.cats)};
   const uint64_t b0 = (uint64_t)blockIdx.x * 32;   // neighbouring blocks write neighbouring rows
   for (uint32_t vt = blockIdx.y; vt < et.var_tiles; vt += gridDim.y) {
@@ -171,12 +171,12 @@ __global__ void __launch_bounds__(EV_THREADS, sizeof(T) == 4 || FORM == ELEMENTS
 }
 
 // dx_c = (g_c - p_c sum g) / T
-template <typename T, int E, Form FORM>
+template <typename T, int E, Form FORM, int LG>
 __global__ void __launch_bounds__(EV_THREADS, FORM == WHOLE ? 4 : 3) evidence_grad_kernel(EvidenceArgs a, EvidenceTile et) {
   using Row = ShortRow<T, E, FORM>;
   extern __shared__ __align__(16) float tile[];
   __shared__ float part[EV_WARPS][32];
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = et.lg, sub = lane & ((1u << lg) - 1), per_pass = EV_THREADS >> lg;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = LG >= 0 ? (uint32_t)LG : et.lg, sub = lane & ((1u << lg) - 1), per_pass = EV_THREADS >> lg;
   const Bounds bounds = {reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + (a.rows - 1) * a.row_stride + (a.vars - 1) * a.var_stride + a.cats)};
   const uint64_t b0 = (uint64_t)blockIdx.x * 32;
   for (uint32_t vt = blockIdx.y; vt < et.var_tiles; vt += gridDim.y) {
@@ -371,20 +371,27 @@ EvidenceTile evidence_tile(const EvidenceArgs& a) {
   return t;
 }
 
-template <typename T, int E, Form FORM>
-cudaError_t launch_evidence_as(const EvidenceArgs& a, const EvidenceTile& t, cudaStream_t st) {
+template <typename T, int E, Form FORM, int LG>
+cudaError_t launch_evidence_lanes(const EvidenceArgs& a, const EvidenceTile& t, cudaStream_t st) {
   const dim3 grid(t.row_tiles, std::min(t.var_tiles, 65535u));
   const uint32_t smem = (tile_place<T>(t.cap, t.lg) + 32) * (uint32_t)sizeof(float);
   static PcbPerDeviceOnce once;
   const cudaError_t e = once.run([] {
     const int most = (int)((tile_place<T>(768, 0) + 32) * sizeof(float));
-    const cudaError_t f = cudaFuncSetAttribute(evidence_kernel<T, E, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    return f != cudaSuccess ? f : cudaFuncSetAttribute(evidence_grad_kernel<T, E, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    const cudaError_t f = cudaFuncSetAttribute(evidence_kernel<T, E, FORM, LG>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    return f != cudaSuccess ? f : cudaFuncSetAttribute(evidence_grad_kernel<T, E, FORM, LG>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   });
   if (e != cudaSuccess) return e;
-  if (a.dx) evidence_grad_kernel<T, E, FORM><<<grid, EV_THREADS, smem, st>>>(a, t);
-  else evidence_kernel<T, E, FORM><<<grid, EV_THREADS, smem, st>>>(a, t);
+  if (a.dx) evidence_grad_kernel<T, E, FORM, LG><<<grid, EV_THREADS, smem, st>>>(a, t);
+  else evidence_kernel<T, E, FORM, LG><<<grid, EV_THREADS, smem, st>>>(a, t);
   return cudaGetLastError();
+}
+template <typename T, int E, Form FORM>
+cudaError_t launch_evidence_as(const EvidenceArgs& a, const EvidenceTile& t, cudaStream_t st) {
+#define PCB_CALL(LG) return launch_evidence_lanes<T, E, FORM, LG>(a, t, st)
+  if constexpr (FORM != ELEMENTS && E == (int)Most<T>::E) PCB_LANES(true, t.lg, PCB_CALL);
+  else PCB_CALL(-1);
+#undef PCB_CALL
 }
 template <typename T, int E>
 cudaError_t launch_evidence_of(const EvidenceArgs& a, const EvidenceTile& t, cudaStream_t st) {

@@ -416,7 +416,7 @@ __device__ __forceinline__ void short_results(const LogprobArgs& a, const Kept& 
 template <typename T, int E, Form FORM, int LG>
 __global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_short_kernel(LogprobArgs a, uint32_t lanes_log2, uint32_t passes) {
   using Row = ShortRow<T, E, FORM>;
-  const uint32_t lg = LG >= 0 ? LG : lanes_log2;
+  const uint32_t lg = LG >= 0 ? (uint32_t)LG : lanes_log2;
   const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1), group = lane >> lg;
   const uint64_t step = (uint64_t)gridDim.x * 8 * per_warp * passes;
   const Bounds bounds = {reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + (a.rows - 1) * a.stride + a.cats)};

@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(LogprobGradA
 template <typename T, int E, Form FORM, int LG>
 __global__ void __launch_bounds__(256, E >= 16 ? 3 : 5) logprob_grad_short_kernel(LogprobGradArgs a, uint32_t lanes_log2, uint32_t passes) {
   using Row = ShortRow<T, E, FORM>;
-  const uint32_t lg = LG >= 0 ? LG : lanes_log2;
+  const uint32_t lg = LG >= 0 ? (uint32_t)LG : lanes_log2;
   const uint32_t lane = threadIdx.x & 31, per_warp = 32u >> lg, sub = lane & ((1u << lg) - 1), group = lane >> lg;
   const Bounds bounds = {reinterpret_cast<uintptr_t>(a.x), reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + (a.rows - 1) * a.stride + a.cats)};
   const uint64_t rows_each = (uint64_t)per_warp * passes, all = (a.rows + rows_each - 1) / rows_each, step = (uint64_t)gridDim.x * 8;
