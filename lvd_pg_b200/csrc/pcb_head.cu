@@ -88,32 +88,41 @@ __device__ __forceinline__ void nibble_place(uint32_t lane, uint32_t w, uint32_t
   k = 32 * (w >> 1) + 8 * (lane & 3) + 4 * (w & 1) + 2 * (i >> 1) + e;
 }
 
+// A block per tile.  A word's nibbles are two bytes of category g and two of g + 8.
 __global__ void __launch_bounds__(256) head_pack_kernel(HeadShape h, const uint8_t* codes, const uint16_t* scales, uint32_t* out) {
-  const uint64_t nc = h.code_words(), total = nc + h.scale_words();
   const uint32_t bytes = (h.features + 1) / 2, groups = (h.features + h.group - 1) / h.group;
-  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
-    uint32_t word = 0;
-    if (i < nc) {
-      const uint32_t w = i & 3, lane = (i >> 2) & 31;
-      const uint64_t tb = i >> 7, tile = tb / h.blocks, block = tb % h.blocks;
-      for (uint32_t p = 0; p < 8; ++p) {
-        uint32_t row, k;
-        nibble_place(lane, w, p, row, k);
-        const uint64_t n = tile * 16 + row, kk = block * 64 + k;
-        uint32_t code = 8;
-        if (n < h.cats && kk < h.features) code = (codes[n * bytes + kk / 2] >> (4 * (kk & 1))) & 15u;
-        word |= code << (4 * p);
+  for (uint64_t tile = blockIdx.x; tile < h.tiles; tile += gridDim.x) {
+    uint32_t* words = out + tile * h.blocks * 128;
+    for (uint32_t i = threadIdx.x; i < h.blocks * 128; i += 256) {
+      const uint32_t w = i & 3, lane = i >> 2 & 31, k = (i >> 7) * 64 + 32 * (w >> 1) + 8 * (lane & 3) + 4 * (w & 1);
+      const uint64_t n = tile * 16 + (lane >> 2);
+      uint32_t word = 0;
+#pragma unroll
+      for (uint32_t half = 0; half < 2; ++half) {
+        uint32_t four = 0x8888u;   // features k .. k + 3 of one category; what is not there is 0
+        if (n + 8 * half < h.cats && k < h.features) {
+          const uint8_t* at = codes + (n + 8 * half) * bytes + k / 2;
+          four = at[0];
+          if (k + 2 < h.features) four |= (uint32_t)at[1] << 8;
+          const uint32_t there = min(4u, h.features - k);
+          four = (four & ((1u << (4 * there)) - 1)) | (0x8888u & ~((1u << (4 * there)) - 1));
+        }
+        // features k, k + 1 to nibbles half, half + 4, features k + 2, k + 3 to half + 2, half + 6
+        word |= ((four & 0xfu) | (four & 0xf0u) << 12 | (four & 0xf00u) | (four & 0xf000u) << 12) << (4 * half);
       }
-    } else {
-      const uint64_t r = i - nc;   // [tile][quad][g][group of the quad]
-      const uint32_t j = r & 3, g = (r >> 2) & 7;
-      const uint64_t tq = r >> 5, tile = tq / h.quads, group = tq % h.quads * 4 + j;
-      for (uint32_t e = 0; e < 2; ++e) {
-        const uint64_t n = tile * 16 + g + 8 * e;
-        if (n < h.cats && group < groups) word |= (uint32_t)scales[n * groups + group] << (16 * e);
-      }
+      words[i] = word;
     }
-    out[i] = word;
+    uint32_t* two = out + h.code_words() + tile * h.quads * 32;   // [quad][g][group of the quad]
+    for (uint32_t i = threadIdx.x; i < h.quads * 32; i += 256) {
+      const uint64_t n = tile * 16 + (i >> 2 & 7);
+      const uint32_t group = (i >> 5) * 4 + (i & 3);
+      uint32_t word = 0;
+      if (group < groups) {
+        if (n < h.cats) word = scales[n * groups + group];
+        if (n + 8 < h.cats) word |= (uint32_t)scales[(n + 8) * groups + group] << 16;
+      }
+      two[i] = word;
+    }
   }
 }
 
@@ -513,8 +522,7 @@ extern "C" int32_t pcb_head_pack(const uint8_t* codes_dev, const void* scales_de
   if (int32_t rc = check_shape(cats, features, group)) return rc;
   PCB_REQUIRE(codes_dev && scales_dev && packed_dev && ((uintptr_t)packed_dev & 15) == 0, "null argument, or a packed head that is not 16-byte aligned");
   const HeadShape h = head_shape(cats, features, group);
-  head_pack_kernel<<<blocks_for(h.code_words() + h.scale_words()), 256, 0, (cudaStream_t)s>>>(h, codes_dev, static_cast<const uint16_t*>(scales_dev),
-                                                                                             static_cast<uint32_t*>(packed_dev));
+  head_pack_kernel<<<h.tiles, 256, 0, (cudaStream_t)s>>>(h, codes_dev, static_cast<const uint16_t*>(scales_dev), static_cast<uint32_t*>(packed_dev));
   PCB_CUDA(cudaGetLastError());
   return PCB_OK;
 }
