@@ -269,10 +269,18 @@ __global__ void __launch_bounds__(EV_THREADS, FORM == WHOLE ? 4 : 3) evidence_gr
 }
 
 // Variables of at most 32 categories that lie one behind the other: a lane is a row, holds a distribution of at most C
-// categories, and needs no shuffles; rows come (and the gradient's go) by elements, 32 neighbouring ones at a time.
+// categories, and needs no shuffles; rows come (and the gradient's go) by elements, 32 neighbouring ones at a time.  What lies by
+// rows goes through shared memory too, since a load by a lane per row touches 32 lines: statistics always, missing variables
+// where there are many (gradient, us by rows / by lanes: 1000 x 784 x 2 16.3 / 20.9, 100 x 784 x 8 10.2 / 9.6, 500 x 192 x 16 12.7 / 12.2).
+// The gradient makes the statistics anew, from the powers that it needs anyway, and asks for the g of several short distributions
+// at a time (16000 x 784 x 2: 183 us, one at a time 208).  Bound by the 32-byte pieces that rows of few columns come and go in,
+// and by latency in small batches: 2.3 TB/s at 16000 x 784 x 2, 2.8 TB/s one way at 5000 x 784 x 4 bf16.
 template <typename T, int C, bool GRADIENT>
-__global__ void __launch_bounds__(EV_THREADS, GRADIENT ? 3 : 4) evidence_thin_kernel(EvidenceArgs a, EvidenceTile et) {
+__global__ void __launch_bounds__(EV_THREADS, C <= 8 ? 5 : GRADIENT ? 3 : 4) evidence_thin_kernel(EvidenceArgs a, EvidenceTile et) {
+  constexpr bool BY_ROWS = C <= 4;
+  constexpr uint32_t AT_ONCE = GRADIENT && C <= 8 ? 8 / C : 1;   // variables
   extern __shared__ __align__(16) float tile[];
+  __shared__ uint32_t missing_bits[EV_COLUMNS / 32][32];   // [variables / 32][row]
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint64_t step = a.rows * a.vars, b0 = (uint64_t)blockIdx.x * 32, b = b0 + lane;
   for (uint32_t vt = blockIdx.y; vt < et.var_tiles; vt += gridDim.y) {
@@ -289,16 +297,46 @@ __global__ void __launch_bounds__(EV_THREADS, GRADIENT ? 3 : 4) evidence_thin_ke
       for (uint32_t k = 0; k < EV_COLUMNS / 32; ++k)
         if (32 * k + lane < columns) tile[(32 * k + lane) * EV_PITCH + r] = to_f32(raw[k]);
     }
-    __syncthreads();
-    for (uint32_t v = warp; v < nv; v += EV_WARPS) {
-      if (lane >= rows) continue;
-      float* at = tile + v * a.cats * EV_PITCH + lane;
-      const bool missing = a.miss && a.miss[b * a.miss_row_stride + (v0 + v) * a.miss_var_stride];
-      const uint64_t memory = b + a.rows * (v0 + v);
-      float xc[C];
+    if (BY_ROWS && a.miss) {
+      const uint8_t* miss = a.miss + b0 * a.miss_row_stride + (v0 + lane) * a.miss_var_stride;
+      for (uint32_t k = 0; 32 * k < nv; ++k, miss += 32 * a.miss_var_stride) {
+        uint8_t gone[32 / EV_WARPS];
 #pragma unroll
-      for (int c = 0; c < C; ++c) xc[c] = c < (int)a.cats ? at[c * EV_PITCH] : -INFINITY;
-      if constexpr (!GRADIENT) {
+        for (uint32_t i = 0; i < 32 / EV_WARPS; ++i) {
+          const uint32_t r = warp + i * EV_WARPS;
+          gone[i] = r < rows && 32 * k + lane < nv ? miss[r * a.miss_row_stride] : 0;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 32 / EV_WARPS; ++i) {
+          const uint32_t bits = __ballot_sync(0xffffffffu, gone[i] != 0);
+          if (lane == 0) missing_bits[k][warp + i * EV_WARPS] = bits;
+        }
+      }
+    }
+    __syncthreads();
+    for (uint32_t first = warp; first < nv; first += EV_WARPS * AT_ONCE) {
+      if (lane >= rows) continue;
+      float gc[GRADIENT ? AT_ONCE : 1][C];
+      if constexpr (GRADIENT) {
+#pragma unroll
+        for (uint32_t u = 0; u < AT_ONCE; ++u) {
+          const uint32_t v = first + u * EV_WARPS;
+          const float* g = a.g + b + a.rows * (v0 + v);
+#pragma unroll
+          for (int c = 0; c < C; ++c) gc[u][c] = v < nv && c < (int)a.cats ? g[step * c] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < AT_ONCE; ++u) {
+        const uint32_t v = first + u * EV_WARPS;
+        if (v >= nv) continue;
+        float* at = tile + v * a.cats * EV_PITCH + lane;
+        bool missing = false;
+        if (BY_ROWS) missing = a.miss && missing_bits[v >> 5][lane] >> (v & 31) & 1;
+        else missing = a.miss && a.miss[b * a.miss_row_stride + (v0 + v) * a.miss_var_stride];
+        float p[C], xc[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) xc[c] = c < (int)a.cats ? at[c * EV_PITCH] : -INFINITY;
         float m = xc[0], S = 0.0f;
 #pragma unroll
         for (int c = 1; c < C; ++c) m = fmaxf(m, xc[c]);
@@ -306,31 +344,31 @@ __global__ void __launch_bounds__(EV_THREADS, GRADIENT ? 3 : 4) evidence_thin_ke
         const Shift from = shift_of<T>(m, a.c);
         if (from.near) {
 #pragma unroll
-          for (int c = 0; c < C; ++c) S += ex2_ftz(fmaf(xc[c], from.c, -from.mc));
+          for (int c = 0; c < C; ++c) S += p[c] = ex2_ftz(fmaf(xc[c], from.c, -from.mc));
         } else {
 #pragma unroll
-          for (int c = 0; c < C; ++c) S += ex2_ftz(max_nan((xc[c] - finite_shift(m)) * from.c, NO_MASS));
+          for (int c = 0; c < C; ++c) S += p[c] = ex2_ftz(max_nan((xc[c] - finite_shift(m)) * from.c, NO_MASS));
         }
-        const LogScale l = log_scale<T>(from, S, a.invT);
-        if (a.stats_out) reinterpret_cast<float2*>(a.stats_out)[b * a.vars + v0 + v] = {m, S};
-        float* out = a.out + memory;
+        if constexpr (!GRADIENT) {
+          const LogScale l = log_scale<T>(from, S, a.invT);
+          float* out = a.out + b + a.rows * (v0 + v);
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-          if (c < (int)a.cats) out[step * c] = missing ? 0.0f : logp_of(xc[c], l);
-      } else {
-        const float* g = a.g + memory;
-        float gc[C], sum = 0.0f;
+          for (int c = 0; c < C; ++c)
+            if (c < (int)a.cats) out[step * c] = missing ? 0.0f : logp_of(xc[c], l);
+          if (a.stats_out) {   // in the places of the first two categories; with one category, behind all
+            at[0] = m;
+            tile[(a.cats > 1 ? v * a.cats + 1 : columns + v) * EV_PITCH + lane] = S;
+          }
+        } else {
+          float sum = 0.0f;
 #pragma unroll
-        for (int c = 0; c < C; ++c) gc[c] = c < (int)a.cats ? g[step * c] : 0.0f;
+          for (int c = 0; c < C; ++c) sum += gc[u][c];
+          const bool none = missing || S == 0.0f;
+          const float k = sum / S;
 #pragma unroll
-        for (int c = 0; c < C; ++c) sum += gc[c];
-        const float2 st = reinterpret_cast<const float2*>(a.stats)[b * a.vars + v0 + v];
-        const Shift from = shift_of<T>(st.x, a.c);
-        const bool none = missing || st.y == 0.0f;
-        const float k = sum / st.y;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-          if (c < (int)a.cats) at[c * EV_PITCH] = none ? 0.0f : (gc[c] - ex2_ftz(scaled(from, xc[c])) * k) * a.invT;
+          for (int c = 0; c < C; ++c)
+            if (c < (int)a.cats) at[c * EV_PITCH] = none ? 0.0f : (gc[u][c] - p[c] * k) * a.invT;
+        }
       }
     }
     __syncthreads();
@@ -341,6 +379,13 @@ __global__ void __launch_bounds__(EV_THREADS, GRADIENT ? 3 : 4) evidence_thin_ke
         for (uint32_t j = lane; j < columns; j += 32) to[j] = from_f32<T>(tile[j * EV_PITCH + r]);
       }
       __syncthreads();
+    } else if (a.stats_out) {
+      for (uint32_t r = warp; r < rows; r += EV_WARPS) {
+        float2* to = reinterpret_cast<float2*>(a.stats_out) + (b0 + r) * a.vars + v0;
+        for (uint32_t v = lane; v < nv; v += 32)
+          to[v] = {tile[v * a.cats * EV_PITCH + r], tile[(a.cats > 1 ? v * a.cats + 1 : columns + v) * EV_PITCH + r]};
+      }
+      __syncthreads();
     }
   }
 }
@@ -348,11 +393,15 @@ __global__ void __launch_bounds__(EV_THREADS, GRADIENT ? 3 : 4) evidence_thin_ke
 // Tiles of up to EV_COLUMNS columns; a variable of up to EV_MOST categories is held whole.
 template <typename T> constexpr uint32_t EV_MOST = 32 * Most<T>::E < 768 ? 32 * Most<T>::E : 768;
 template <typename T>
-EvidenceTile evidence_tile(const EvidenceArgs& a) {
+EvidenceTile evidence_tile(const EvidenceArgs& a, uint32_t sms) {
   EvidenceTile t;
   t.vars = a.var_stride == a.cats && a.cats <= EV_COLUMNS / 2 ? std::min(EV_COLUMNS / a.cats, a.vars) : 1;
+  const uint64_t row_tiles = (a.rows + 31) / 32;
+  // smaller tiles where there are few (us with none / 2 / 4 tiles per SM wanted: 1000 x 784 x 2 gradient 28.8 / 20.9 / 25.2,
+  // one way 9.7 / 6.6 / 7.6, 100 x 784 x 8 14.6 / 9.7 / 9.7)
+  while (t.vars > 8 && row_tiles * ((a.vars - 1) / t.vars + 1) < 2 * (uint64_t)sms) t.vars = (t.vars + 1) / 2;
   t.cap = t.vars > 1 ? t.vars * a.cats : a.cats <= EV_MOST<T> ? a.cats : EV_COLUMNS;
-  t.row_tiles = (uint32_t)((a.rows + 31) / 32);
+  t.row_tiles = (uint32_t)row_tiles;
   t.var_tiles = (a.vars - 1) / t.vars + 1;
   constexpr uint32_t N = Vec<T>::N;
   const auto whole_at = [&](uint64_t row, uint64_t var) { return ((row | (a.vars > 1 ? var : 0)) * sizeof(T) & 15) == 0; };
@@ -404,14 +453,21 @@ cudaError_t launch_evidence_of(const EvidenceArgs& a, const EvidenceTile& t, cud
 template <typename T, int C>
 cudaError_t launch_thin(const EvidenceArgs& a, const EvidenceTile& t, cudaStream_t st) {
   const dim3 grid(t.row_tiles, std::min(t.var_tiles, 65535u));
-  const uint32_t smem = t.cap * EV_PITCH * (uint32_t)sizeof(float);
+  const uint32_t smem = (t.cap + (a.cats == 1 && a.stats_out ? t.vars : 0)) * EV_PITCH * (uint32_t)sizeof(float);
+  static PcbPerDeviceOnce once;   // distributions of one category need twice the columns
+  const cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(evidence_thin_kernel<T, C, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * EV_COLUMNS * EV_PITCH * (int)sizeof(float));
+  });
+  if (e != cudaSuccess) return e;
   if (a.dx) evidence_thin_kernel<T, C, true><<<grid, EV_THREADS, smem, st>>>(a, t);
   else evidence_thin_kernel<T, C, false><<<grid, EV_THREADS, smem, st>>>(a, t);
   return cudaGetLastError();
 }
 template <typename T>
 cudaError_t launch_evidence(const EvidenceArgs& a, cudaStream_t st) {   // the gradient where dx is given
-  const EvidenceTile t = evidence_tile<T>(a);
+  const uint32_t sms = pcb_sm_count();
+  if (sms == 0) return cudaErrorNoDevice;
+  const EvidenceTile t = evidence_tile<T>(a, sms);
   if (a.cats <= 32 && (t.vars > 1 || a.vars == 1)) {
     if (a.cats <= 2) return launch_thin<T, 2>(a, t, st);
     if (a.cats <= 4) return launch_thin<T, 4>(a, t, st);

@@ -235,11 +235,17 @@ __device__ __forceinline__ void store_y(void* y, uint64_t i, float v, int32_t dt
   else static_cast<__half*>(y)[i] = __float2half_rn(v);
 }
 
-// Persistent blocks of sixteen warps, in teams.  A team takes R tiles of 16 categories a round; its warps share the features
-// and add up their parts through shared memory: large teams for heads with few categories, which fill the GPU so, small ones
-// where there are enough (no warp waits for others in a team of one).  The feature vectors stay in shared memory, as
+// Persistent blocks of sixteen warps, in teams of four or eight.  A team takes R tiles of 16 categories a round; its warps
+// share the features and add up their parts through shared memory: large teams for heads with few categories, which fill the
+// GPU so, smaller ones where there are enough (fewer wait for one another).  The feature vectors stay in shared memory, as
 // columns of the B operand (fp32: three columns each, one per term, joined at the end); codes and scales go straight from
 // memory to registers, four 16-byte loads per lane ahead of the four that are worked on, across the boundaries of rounds.
+//
+// Bound by what turns codes into operands, not by the products: one vector at 131072 x 4096 bf16 takes 62.8 us for 285 MB
+// (4.5 TB/s, 70 % of what a copy reaches) with the pipe of shifts and masks 60 % busy, three shifts, four masks and four
+// subtractions per eight codes.  Wide multiplies in place of shifts (76 -> 88 us then), a step loop unrolled by two (64 -> 65)
+// and prefetching the next round into the L2 cache (64 -> 78) did not pay.  fp16 needs one shift: 32000 x 2048, sixteen
+// vectors, 15.3 us (2.3 TB/s: launch, feature vectors and the last round weigh there).
 constexpr uint32_t HEAD_THREADS = 512, HEAD_WARPS = 16;
 
 template <bool G32>
@@ -413,8 +419,7 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
           const uint32_t column = n * 8 + 2 * t + (i & 1);
           if (column < ps.columns) parts[(warp * ps.columns + column) * (R * 16) + r * 16 + g + 8 * (i >> 1)] = sum[r][n][i];
         }
-    if (ps.team == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(ps.team * 32) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(ps.team * 32) : "memory");
     for (uint32_t i = warp * 32 + lane; i < vectors * (R * 16); i += ps.team * 32) {
       const uint32_t m = i / (R * 16), n = i % (R * 16);
       float y = 0.0f;
@@ -431,8 +436,8 @@ __global__ void __launch_bounds__(HEAD_THREADS, 1) head_kernel(HeadArgs a, HeadP
   }
 }
 
-// Shared memory a block may have, and the columns that one pass takes: the fewest tiles of eight that hold all feature
-// vectors, or what fits.  (More vectors than a pass takes read the weights again.)
+// Shared memory a block may have.  A pass takes up to 32 columns (32 feature vectors of 16 bits, 10 of fp32), or what fits;
+// more vectors than that read the weights again.
 constexpr uint32_t HEAD_SMEM = 220 * 1024;
 
 template <typename X, int R, int NT, bool G32, bool BF16_SCALES>

@@ -7,7 +7,10 @@
 
 The reference trains its teachers in PyTorch (src/models/, src/maskedAE, src/pixelcnn) and hands their outputs to the
 circuits as arrays; these run on the GPU beside the circuit.  Every call is enqueued on the current stream of its tensors'
-device, allocates through torch's allocator alone and does not synchronise.
+device, allocates through torch's allocator alone and does not synchronise.  Forward and backward passes can be captured into
+CUDA graphs; as for every torch operator, a captured backward pass needs leaves of its own (made in the capture, as
+`static.detach().requires_grad_()`): with leaves that an eager graph still holds, torch waits for that graph's stream and the
+capture fails.
 """
 from __future__ import annotations
 
@@ -265,7 +268,8 @@ class QuantHead:
 
     def logits(self, x: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """x [..., features] (float32, bfloat16 or float16) -> [..., cats] in `out_dtype` (default: x's type).  Sums are
-        float32; meant for few rows: every eight of them read the weights once."""
+        float32.  Meant for few rows: up to 32 of them (10 of float32; fewer beyond about 2400 features, 21 and 7 at 4096)
+        read the weights once."""
         _need(isinstance(x, torch.Tensor) and x.device == self.device and x.dtype in _DTYPES,
               "features must be float32, bfloat16 or float16 on the head's device")
         if x.dim() < 1 or x.shape[-1] != self.features:

@@ -133,6 +133,30 @@ def test_another_stream_and_a_replayed_graph():
         assert torch.equal(out, fresh) and torch.equal(dx, torch.autograd.grad(fresh, leaf2, g)[0])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,variables,cats", [(33, 300, 1), (40, 290, 2), (100, 70, 3), (5, 33, 8), (65, 13, 30), (40, 3, 300), (33, 2, 1500)])
+def test_statistics_of_every_distribution(dtype, rows, variables, cats):
+    """Many variables a tile, batches that end inside one; the largest logit exactly, the sum of powers within its bound, and
+    nothing written behind them."""
+    x, miss = _logits(rows, variables, cats, dtype, cats), _miss(rows, variables, 3)
+    if cats > 1:
+        x[1, 0] = -math.inf
+    _check(x, miss)
+    out = torch.full((cats * variables * rows + 64,), 7.0, device="cuda")
+    stats = torch.full((rows * variables * 2 + 64,), 7.0, device="cuda")
+    _lib.check(_lib.lib().pcb_soft_evidence(x.data_ptr(), DTYPES.index(dtype), rows, variables, cats, variables * cats, cats, miss.data_ptr(), variables,
+                                            1, 1.0, out.data_ptr(), stats.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(out[:-64].view(cats, variables, rows).permute(2, 1, 0), api.soft_evidence(x, miss))
+    assert (out[-64:] == 7).all() and (stats[-64:] == 7).all()
+    got = stats[:-64].view(rows * variables, 2)
+    ref = Logprobs(x.reshape(-1, cats), None, 0, 1.0)
+    assert torch.equal(got[:, 0], x.reshape(-1, cats).float().amax(1))
+    # S counts from the rounded product of the maximum and log2(e): half a step of it beside the bound of the sum itself
+    shift = torch.where(ref.empty, 0.0, ref.x.amax(1))
+    want = (ref.x - shift[:, None]).exp().sum(1)
+    assert_within(got[:, 1], want, want * (ref.tol_S + 2 * U * (1 + shift.abs() * LOG2E)))
+
+
 def test_more_elements_than_32_bits_count():
     rows, variables, cats = 70001, 64, 512
     x = torch.empty(rows, variables, cats, dtype=torch.bfloat16, device="cuda")
