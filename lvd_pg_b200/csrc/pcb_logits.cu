@@ -31,6 +31,10 @@ __device__ __forceinline__ float token_logp(const LogprobArgs& a, int64_t token,
 // those (rows of few different values, or large ones side by side in few groups) raise the bound to the k-th of what
 // was collected, as long as that helps; what is left then (mostly ties) goes by rounds over what lies above the bound and
 // one walk in index order over what equals it.
+//
+// Bound by memory and by the end of each row, where a block reads what it noted: 2048 rows of 131072 bf16 with 8 alternatives
+// 105 us (5.1 TB/s, 79 % of a copy; 96 us without alternatives); a single row of 131072 fp32 with 20 alternatives, on a cluster
+// of eight blocks, 9.4 us, all of it latency (launch, one pass of sixteen tiles, selection, two cluster barriers).
 constexpr uint32_t SLOTS = 16, CAND = 256, PAIRS = 256, MAX_CLUSTER = 8;
 
 template <typename T> struct Tile { static constexpr uint32_t U = sizeof(T) == 4 ? 8 : 4; };   // granules per thread
@@ -412,7 +416,9 @@ __device__ __forceinline__ void short_results(const LogprobArgs& a, const Kept& 
 
 // Rows in memory: in 16-byte granules, or element by element, whatever their distance.  A warp takes `passes` times the rows
 // that its lanes hold at once, the next ones on their way while it works on these (granules), and writes the results of all
-// of them together: lane (g, j) those of the g-th row of pass j.
+// of them together: lane (g, j) those of the g-th row of pass j.  Bound by instructions (a power, two sums and the maximum per
+// element; finding the best alternative and writing results per row): 401408 rows of 256 fp16 with one alternative 53.4 us
+// (4.1 TB/s, 63 % of a copy).
 template <typename T, int E, Form FORM, int LG>
 __global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_short_kernel(LogprobArgs a, uint32_t lanes_log2, uint32_t passes) {
   using Row = ShortRow<T, E, FORM>;
@@ -450,7 +456,7 @@ __global__ void __launch_bounds__(256, E >= 16 ? 3 : 4) logprob_short_kernel(Log
 
 // Rows one behind the other (stride = cats), of any length and alignment: every warp stages the bytes of `rows_staged` of
 // them, from the 16-byte boundary below their beginning on, with asynchronous copies, STAGES - 1 of them ahead of its work,
-// and its lanes read their elements there.
+// and its lanes read their elements there.  (Both directions of 800000 rows of 51 fp16: 170 us, by granules from memory 228.)
 template <typename T, int E>
 __global__ void __launch_bounds__(STAGED_THREADS, 6) logprob_staged_kernel(LogprobArgs a, uint32_t lg, uint32_t rows_staged) {
   using Row = ShortRow<T, E, ELEMENTS>;
