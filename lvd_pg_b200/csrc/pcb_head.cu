@@ -471,6 +471,7 @@ cudaError_t launch_head_of(const HeadArgs& a, uint32_t sms, cudaStream_t st) {
   // Tiles per round (R, as many as the columns' registers allow) and warps per team.  us, R / team:
   //   131072 x 4096, one vector   4/8 63.6   2/4 65.0   1/2 67.7        50000 x 8192, four   4/8 53.2   2/4 51.1   1/2 53.3
   //   32000 x 2048, one           4/8 13.8   2/4 12.5   1/2 13.7        4096 x 4096, one     4/8 10.4   2/4  9.7   1/8  7.1
+  //   32000 x 2048 fp16, sixteen  2/4 15.2   2/8 16.7   1/4 15.7   1/8 16.6    50000 x 1024 bf16, nine  2/4 13.9   2/8 15.3   1/4 15.2   1/8 18.5
   const uint32_t nt = (ps.columns + 7) / 8;
   const auto fits = [&](uint32_t r) { return ps.columns * (ps.pitch + 2 * HEAD_WARPS * r * 16 * (uint32_t)sizeof(float)) <= HEAD_SMEM; };
   uint32_t tiles = 1;
