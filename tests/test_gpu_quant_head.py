@@ -241,3 +241,43 @@ def test_a_head_used_and_dropped_on_another_stream():
         torch.cuda.synchronize()
         assert torch.equal(got, want)
         del junk
+
+
+def test_calls_of_two_threads_at_once():
+    """Two host threads on streams of their own, the same head and logits: head, scores, evidence and gradients as alone."""
+    import threading
+
+    packed, scales, values = _codes(3000, 256, 64, torch.bfloat16, 4)
+    head = api.QuantHead.from_codes(packed, scales, 256, 64)
+    x = torch.randn(6, 256, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    logits = torch.randn(40, 30, 60, generator=torch.Generator().manual_seed(2)).cuda()
+    long = torch.randn(3, 200000, generator=torch.Generator().manual_seed(3)).cuda()
+    tokens = torch.randint(0, 60, (40, 30), generator=torch.Generator().manual_seed(4)).cuda()
+
+    def work():
+        leaf = logits.detach().requires_grad_()
+        scores = api.token_logprobs(leaf, tokens, 3)
+        evidence = api.soft_evidence(leaf)
+        grad, = torch.autograd.grad([scores.logp, evidence], leaf, [torch.ones_like(scores.logp), torch.ones_like(evidence)])
+        return [*head.logprobs(x, None, 4)[1:], *scores, evidence, grad, *api.token_logprobs(long, None, 32)[1:]]
+
+    want = [t.detach().clone() for t in work()]
+    torch.cuda.synchronize()
+    failures = []
+
+    def run():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(15):
+                    got = work()
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(got, want))
+        except BaseException as e:   # for the main thread
+            failures.append(e)
+
+    threads = [threading.Thread(target=run) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
