@@ -87,12 +87,12 @@ template <typename T> constexpr uint32_t PER_WORD = 4 / sizeof(T);
 
 // Where the powers of a row count from.
 struct Shift {
-  float m, c, mc;   // mc: m c, rounded
+  float m, c, mc;   // mc: m c, rounded (an explicit product: fused into a difference of two it would not be the one that powers count from)
   bool near;
 };
 template <typename T>
 __device__ __forceinline__ Shift shift_of(float m, float c) {
-  return {m, c, m * c, fabsf(m) < 1e29f && (m - Word<T>::FLOOR) * c > 200.0f && c < 1e8f};
+  return {m, c, __fmul_rn(m, c), fabsf(m) < 1e29f && (m - Word<T>::FLOOR) * c > 200.0f && c < 1e8f};
 }
 __device__ __forceinline__ float scaled(const Shift& s, float x) {   // d, clamped; x finite or not
   return max_nan(s.near ? fmaf(x, s.c, -s.mc) : (x - s.m) * s.c, NO_MASS);
