@@ -6,9 +6,11 @@
 //   logp_j = ln2 d_j - ln S          H = ln S - ln2 A / S          p_j = 2^d_j / S
 // d is formed in one of two ways.  Near: fma(x, c, -round(m c)) with x raised to a floor first, so that impossible
 // categories (-inf) have 2^d = 0 and a finite d: 0 * inf stays out of A, one instruction per two elements; what rounding
-// m c leaves off is the same in every d of the row, in S and in A, and cancels.  Far, where m c could overflow (a row of
-// the type's lowest values, as masks leave it) or the floor would still weigh: (x - m) c, clamped at -200.  NaN passes
-// both (max.NaN).  A row without any possible category has S = 0, logp -inf, H = 0 and gradient 0.
+// m c leaves off is the same in every d of the row, in S and in A, and cancels.  It has to stay small, since the largest
+// power of the row is two to it: at most 2^-5 below |m c| = 2^20, 2^7 and out of range from 2^31 on.  Far, where m c is
+// above that (rows that a mask's -1e10 or lowest value fills, temperatures near 0) or the floor would still weigh:
+// (x - m) c, clamped at -200.  NaN passes both (max.NaN).  A row without any possible category has S = 0, logp -inf, H = 0
+// and gradient 0.
 #pragma once
 #include "pcb_internal.h"
 #include "pcb_tc.cuh"
@@ -92,7 +94,7 @@ struct Shift {
 };
 template <typename T>
 __device__ __forceinline__ Shift shift_of(float m, float c) {
-  return {m, c, __fmul_rn(m, c), fabsf(m) < 1e29f && (m - Word<T>::FLOOR) * c > 200.0f && c < 1e8f};
+  return {m, c, __fmul_rn(m, c), fabsf(m * c) < 0x1p20f && (m - Word<T>::FLOOR) * c > 200.0f && c < 1e8f};
 }
 __device__ __forceinline__ float scaled(const Shift& s, float x) {   // d, clamped; x finite or not
   return max_nan(s.near ? fmaf(x, s.c, -s.mc) : (x - s.m) * s.c, NO_MASS);
