@@ -44,8 +44,8 @@ __device__ __forceinline__ RowGrad row_grad(const LogprobGradArgs& a, uint64_t r
   return g;
 }
 __device__ __forceinline__ float grad_of(const RowGrad& g, float x) {
-  const float d = scaled(g.from, x);
-  return ex2_ftz(d) * fmaf(g.beta, d, g.alpha);
+  const float d = scaled(g.from, x), power = ex2_ftz(d);
+  return fmaf(power * d, g.beta, power * g.alpha);
 }
 __device__ __forceinline__ bool no_mass(const RowGrad& g) { return g.S == 0.0f; }
 // the whole gradient of an element that the token or an alternative points to
@@ -58,7 +58,7 @@ __device__ __forceinline__ float pointed_grad(const LogprobGradArgs& a, const Ro
       if (a.top_ids[row * a.top_k + k] == (int64_t)j) v += a.g_top[row * a.top_k + k] * a.invT;
   return v;
 }
-// p_j (alpha + beta d) of W words, as words
+// p_j alpha + p_j d beta of W words, as words
 template <typename T, int W>
 __device__ __forceinline__ void grad_words(const uint32_t* w, const RowGrad& g, uint32_t* out) {
   constexpr int E = W * (int)PER_WORD<T>;
@@ -76,7 +76,8 @@ __device__ __forceinline__ void grad_words(const uint32_t* w, const RowGrad& g, 
       const float m = finite_shift(g.from.m);
       d = {max_nan((x.x - m) * g.from.c, NO_MASS), max_nan((x.y - m) * g.from.c, NO_MASS)};
     }
-    const float2 v = mul2({ex2_ftz(d.x), ex2_ftz(d.y)}, fma2({beta, beta}, d, {alpha, alpha}));
+    // 2^d d first: it is 0 where 2^d is, while beta d passes the range beside a floor's d of -1e30 and more
+    const float2 power = {ex2_ftz(d.x), ex2_ftz(d.y)}, v = fma2(mul2(power, d), {beta, beta}, mul2(power, {alpha, alpha}));
     if constexpr (sizeof(T) == 4) {
       out[e] = __float_as_uint(v.x);
       out[e + 1] = __float_as_uint(v.y);

@@ -62,7 +62,7 @@ def test_evidence(dtype, temperature, rows, variables, cats):
     check_evidence(_rows(rows * variables, cats, dtype, cats).view(rows, variables, cats), None, temperature)
 
 
-def _within_up_to_the_last_step(got, want, tol, what=""):
+def within_up_to_the_last_step(got, want, tol, what=""):
     """`assert_within`, but for the end of the type's range: the largest number is (2 - eps) 2^e with steps of eps 2^e, so that
     values up to half a step above it round to it, not to infinity (fp16: 65504 up to 65520)."""
     f = torch.finfo(got.dtype)
@@ -75,7 +75,7 @@ def _within_up_to_the_last_step(got, want, tol, what=""):
 @pytest.mark.parametrize("temperature", [1e-5, 1e-7])
 def test_half_precision_at_low_temperatures(cats, temperature, monkeypatch):
     for module in (test_gpu_soft_evidence, test_gpu_token_logprobs):   # gradients of 1 / T pass the range of fp16
-        monkeypatch.setattr(module, "assert_within", _within_up_to_the_last_step)
+        monkeypatch.setattr(module, "assert_within", within_up_to_the_last_step)
     x = make_logits(8, cats, torch.float32, cats, device="cpu")
     x[0], x[1], x[2], x[3] = 65504, -65504, 4000, -60000
     x[2, 1::2], x[2, 0], x[3, cats // 2] = 3999, 3998, -59968
