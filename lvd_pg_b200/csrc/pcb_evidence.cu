@@ -147,8 +147,9 @@ __global__ void __launch_bounds__(EV_THREADS, sizeof(T) == 4 || FORM == ELEMENTS
           m = streamed[r].x;
           S = streamed[r].y;
         }
-        if (a.stats_out && c0 == 0 && sub == 0 && q == qq) reinterpret_cast<float2*>(a.stats_out)[b * a.vars + v0 + v] = {m, S};
-        const LogScale l = log_scale<T>(shift_of<T>(m, a.c), S, a.invT);
+        const Shift from = shift_of<T>(m, a.c);
+        if (a.stats_out && c0 == 0 && sub == 0 && q == qq) reinterpret_cast<float2*>(a.stats_out)[b * a.vars + v0 + v] = {m, sum_out(from, S)};
+        const LogScale l = log_scale<T>(from, S, a.invT);
         const uint32_t column = v * a.cats, mine = q == qq ? n : 0;   // a place is written where it lies below
 #pragma unroll
         for (int e = 0; e < E; e += Row::N) {
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(EV_THREADS, FORM == WHOLE ? 4 : 3) evidence_gr
           for (uint32_t k = 0; k < EV_WARPS; ++k) sum += part[k][r];
         }
         const Shift from = shift_of<T>(st.x, a.c);
-        const float scale = missing || st.y == 0.0f ? 0.0f : a.invT, k = -sum / st.y * a.invT;
+        const float scale = missing || st.y == 0.0f ? 0.0f : a.invT, k = -sum / sum_in(from, st.y) * a.invT;
         uint32_t out[Row::W];
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
@@ -359,7 +360,7 @@ __global__ void __launch_bounds__(EV_THREADS, C <= 8 ? 5 : GRADIENT ? 3 : 4) evi
             if (c < (int)a.cats) out[step * c] = missing ? 0.0f : logp_of(xc[c], l);
           if (a.stats_out) {   // in the places of the first two categories; with one category, behind all
             at[0] = m;
-            tile[(a.cats > 1 ? v * a.cats + 1 : columns + v) * EV_PITCH + lane] = S;
+            tile[(a.cats > 1 ? v * a.cats + 1 : columns + v) * EV_PITCH + lane] = sum_out(from, S);
           }
         } else {
           float sum = 0.0f;

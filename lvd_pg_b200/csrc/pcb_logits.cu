@@ -311,11 +311,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprob_row_kernel(Lo
       }
     }
     if (rank == 0) {
-      const LogScale l = log_scale<T>(shift_of<T>(s.m, a.c), s.S, a.invT);
+      const Shift from_all = shift_of<T>(s.m, a.c);
+      const LogScale l = log_scale<T>(from_all, s.S, a.invT);
       if (tid == 0) {
         if (a.tokens) a.logp[row] = token_logp(a, token, x_token, l);
         a.entropy[row] = entropy_of(s.S, s.A, ln_of(s.S));
-        if (a.stats) reinterpret_cast<float2*>(a.stats)[row] = {s.m, s.S};
+        if (a.stats) reinterpret_cast<float2*>(a.stats)[row] = {s.m, sum_out(from_all, s.S)};
       }
       if (tid < a.top_k) {
         const uint64_t key = sh.best[tid];
@@ -404,10 +405,11 @@ __device__ __forceinline__ Kept short_row(const LogprobArgs& a, ShortRow<T, E, F
 // The results of up to 32 rows, one per lane.
 template <typename T>
 __device__ __forceinline__ void short_results(const LogprobArgs& a, const Kept& k, uint64_t row, int64_t token, float x_token) {
-  const LogScale l = log_scale<T>(shift_of<T>(k.m, a.c), k.S, a.invT);
+  const Shift from = shift_of<T>(k.m, a.c);
+  const LogScale l = log_scale<T>(from, k.S, a.invT);
   if (a.tokens) a.logp[row] = token_logp(a, token, x_token, l);
   a.entropy[row] = entropy_of(k.S, k.A, ln_of(k.S));
-  if (a.stats) reinterpret_cast<float2*>(a.stats)[row] = {k.m, k.S};
+  if (a.stats) reinterpret_cast<float2*>(a.stats)[row] = {k.m, sum_out(from, k.S)};
   if (a.top_k == 1) {
     a.top_ids[row] = k.at;
     a.top_logp[row] = logp_of(k.best, l);

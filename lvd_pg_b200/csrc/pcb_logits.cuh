@@ -101,6 +101,9 @@ __device__ __forceinline__ float scaled(const Shift& s, float x) {   // d, clamp
 }
 // what rounding m c has left off
 __device__ __forceinline__ float left_off(const Shift& s) { return s.near ? fmaf(s.m, s.c, -s.mc) : 0.0f; }
+// Statistics go out, and come back to the gradients, as sums of exp(s_j - max s), free of that.
+__device__ __forceinline__ float sum_out(const Shift& s, float S) { return S * ex2_ftz(-left_off(s)); }
+__device__ __forceinline__ float sum_in(const Shift& s, float S) { return S * ex2_ftz(left_off(s)); }
 // log2 of the factor between powers counted from a and from b
 __device__ __forceinline__ float between(const Shift& a, const Shift& b) {
   return max_nan(a.near && b.near ? a.mc - b.mc : fmaf(a.m - b.m, a.c, left_off(b) - left_off(a)), NO_MASS);

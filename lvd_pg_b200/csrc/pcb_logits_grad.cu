@@ -27,7 +27,7 @@ template <typename T>
 __device__ __forceinline__ RowGrad row_grad(const LogprobGradArgs& a, uint64_t row) {
   RowGrad g;
   g.from = shift_of<T>(a.stats[2 * row], a.c);
-  g.S = a.stats[2 * row + 1];
+  g.S = sum_in(g.from, a.stats[2 * row + 1]);
   g.token = -1;
   g.gl = 0.0f;
   if (a.g_logp && a.tokens) {

@@ -5,8 +5,8 @@ import math
 import pytest
 import torch
 
-from lvd_pg_b200 import api
-from tests.heads_reference import Logprobs, make_logits
+from lvd_pg_b200 import _lib, api
+from tests.heads_reference import Logprobs, U, assert_within, make_logits
 from tests.test_gpu_heads_offsets import within_up_to_the_last_step
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +28,33 @@ def test_impossible_categories_beside_a_large_weight_of_the_entropy(dtype, cats,
     want, tol = Logprobs(x, None, 0, temperature).grad(None, torch.full_like(entropy, weight), None, dtype)
     assert (dx[:, 1::3] == 0).all() and (dx[3, 1:] == 0).all()
     within_up_to_the_last_step(dx, want, tol, "gradient")   # fp16: some lie at the end of its range
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cats,rows", [(2, 40), (20, 9000), (256, 40), (333, 40), (900, 40), (5000, 40), (140000, 2)])
+@pytest.mark.parametrize("temperature", [1.0, 0.01, 1e-4])
+def test_statistics_are_of_the_softmax_itself(dtype, cats, rows, temperature):
+    """The largest logit and the sum of exp((x - max) / T), as the header says, from the scores and from evidence: no more than
+    the sum's bound, two roundings and a power of two (4 u) beside it, so that max / T + log(sum) is the logarithm of the sum
+    of exponentials."""
+    x = make_logits(rows, cats, torch.float32, cats, device="cpu")
+    x += torch.linspace(-40, 40, rows)[:, None]
+    x[0] = -math.inf
+    x[rows - 1, 1:] = x[rows - 1, :1]
+    x = x.to(dtype).cuda()
+    ref = Logprobs(x, None, 0, temperature)
+    shift = torch.where(ref.empty, 0.0, ref.x.amax(1))
+    want = ((ref.x - shift[:, None]) / temperature).exp().sum(1)
+    tol = want * (ref.tol_S + 8 * U)
+    stream = torch.cuda.current_stream().cuda_stream
+    entropy, stats = torch.empty(rows, device="cuda"), torch.empty(rows, 2, device="cuda")
+    _lib.check(_lib.lib().pcb_token_logprobs(x.data_ptr(), DTYPES.index(dtype), rows, cats, cats, temperature, None, 0, 0, None,
+                                             entropy.data_ptr(), stats.data_ptr(), None, None, stream))
+    assert torch.equal(stats[:, 0], x.float().amax(1))
+    assert_within(stats[:, 1], want, tol, "scores")
+    for variables in (1, 2):   # [rows / variables, variables, cats]
+        out, stats = torch.empty(rows * cats, device="cuda"), torch.empty(rows, 2, device="cuda")
+        _lib.check(_lib.lib().pcb_soft_evidence(x.data_ptr(), DTYPES.index(dtype), rows // variables, variables, cats, variables * cats, cats,
+                                                None, 0, 0, temperature, out.data_ptr(), stats.data_ptr(), stream))
+        assert torch.equal(stats[:, 0], x.float().amax(1))
+        assert_within(stats[:, 1], want, tol, "evidence")
