@@ -337,7 +337,7 @@ int32_t pcb_token_logprobs_backward(const void* x_dev, int32_t dtype, uint64_t r
 /* Soft evidence of logits x_dev [rows, vars, cats] (category fastest, the other two at their strides): the normalised
  * log-weights logp, [rows, vars, cats] column-major in out_dev: what pcb_evidence.soft_dev takes.  A variable that is
  * missing in a row (miss_dev, nonzero bytes at the two strides; may be NULL) gets 0 for every category.  stats_dev
- * [rows, vars, 2] (may be NULL) as in pcb_token_logprobs.  At most 2^35 - 1 rows. */
+ * [rows, vars, 2] (may be NULL) as in pcb_token_logprobs.  At most 2^35 - 1 rows and 2^31 - 1 variables. */
 int32_t pcb_soft_evidence(const void* x_dev, int32_t dtype, uint64_t rows, uint32_t vars, uint32_t cats,
                           uint64_t row_stride, uint64_t var_stride, const uint8_t* miss_dev, uint64_t miss_row_stride,
                           uint64_t miss_var_stride, float temperature, float* out_dev, float* stats_dev, pcb_stream s);

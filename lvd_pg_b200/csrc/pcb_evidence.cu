@@ -495,7 +495,7 @@ extern "C" int32_t pcb_soft_evidence(const void* x_dev, int32_t dtype, uint64_t 
   EvidenceArgs a{x_dev, rows, row_stride, var_stride, miss_row_stride, miss_var_stride, vars, cats, 1.0f / temperature,
                  LOG2E / temperature, miss_dev, out_dev, stats_dev, nullptr, nullptr, nullptr};
   PCB_REQUIRE(!stats_dev || ((uintptr_t)stats_dev & 7) == 0, "statistics that are not 8-byte aligned");
-  PCB_REQUIRE(rows < (1ull << 35), "at most 2^35 rows");
+  PCB_REQUIRE(rows < (1ull << 35) && vars <= 0x7fffffffu, "at most 2^35 - 1 rows and 2^31 - 1 variables");
   cudaStream_t st = (cudaStream_t)s;
   PCB_CUDA(dtype == PCB_F32 ? launch_evidence<float>(a, st) : dtype == PCB_BF16 ? launch_evidence<__nv_bfloat16>(a, st) : launch_evidence<__half>(a, st));
   return PCB_OK;
@@ -512,7 +512,7 @@ extern "C" int32_t pcb_soft_evidence_backward(const void* x_dev, int32_t dtype, 
   EvidenceArgs a{x_dev, rows, row_stride, var_stride, miss_row_stride, miss_var_stride, vars, cats, 1.0f / temperature,
                  LOG2E / temperature, miss_dev, nullptr, nullptr, stats_dev, g_dev, dx_dev};
   PCB_REQUIRE(((uintptr_t)stats_dev & 7) == 0, "statistics that are not 8-byte aligned");
-  PCB_REQUIRE(rows < (1ull << 35), "at most 2^35 rows");
+  PCB_REQUIRE(rows < (1ull << 35) && vars <= 0x7fffffffu, "at most 2^35 - 1 rows and 2^31 - 1 variables");
   cudaStream_t st = (cudaStream_t)s;
   PCB_CUDA(dtype == PCB_F32 ? launch_evidence<float>(a, st) : dtype == PCB_BF16 ? launch_evidence<__nv_bfloat16>(a, st)
                                                                                     : launch_evidence<__half>(a, st));
