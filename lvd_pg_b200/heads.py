@@ -22,6 +22,7 @@ import torch
 from . import _lib
 
 MAX_ALTERNATIVES = 32
+MOST = 2 ** 31 - 1   # categories, variables, features that the library is told of in 32 bits
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -56,6 +57,8 @@ def _logits(x: torch.Tensor) -> int:
         _need(False, "logits are float32, bfloat16 or float16")
     if x.dim() < 1 or x.shape[-1] < 1:
         _need(False, "logits need at least one category")
+    if x.shape[-1] > MOST:
+        _need(False, "logits have at most 2^31 - 1 categories")
     return dtype
 
 
@@ -186,6 +189,7 @@ def soft_evidence(logits: torch.Tensor, miss: Optional[torch.Tensor] = None, tem
     (not twice); where missing, or where all logits are -inf (evidence -inf throughout), the gradient is 0."""
     dtype = _logits(logits)
     _need(logits.dim() == 3, "logits must be [rows, vars, cats]")
+    _need(logits.shape[1] <= MOST, "soft evidence has at most 2^31 - 1 variables")
     _need(0.0 < temperature < float("inf"), "the temperature must be positive and finite")
     if miss is not None:
         _need(isinstance(miss, torch.Tensor) and miss.device == logits.device and miss.dtype in (torch.bool, torch.uint8),
@@ -208,7 +212,7 @@ class QuantHead:
     def __init__(self, weight: torch.Tensor, group: int = 64, bias: Optional[torch.Tensor] = None):
         _need(isinstance(weight, torch.Tensor) and weight.is_cuda and weight.dim() == 2 and weight.dtype in _DTYPES,
               "weight must be a [cats, features] CUDA tensor of float32, bfloat16 or float16")
-        _need(weight.shape[0] >= 1 and weight.shape[1] >= 1, "a head has at least one category and one feature")
+        _need(1 <= weight.shape[0] <= MOST and 1 <= weight.shape[1] <= MOST, "a head has 1 to 2^31 - 1 categories and at least one feature")
         _need(group in (32, 64, 128), "groups hold 32, 64 or 128 features")
         w = weight.detach().contiguous()
         cats, features = w.shape
@@ -228,7 +232,7 @@ class QuantHead:
         _need(isinstance(codes, torch.Tensor) and codes.is_cuda and codes.dtype == torch.uint8 and codes.dim() == 2,
               "codes must be a uint8 CUDA matrix")
         cats = codes.shape[0]
-        _need(cats >= 1 and features >= 1 and codes.shape[1] == (features + 1) // 2, "codes must be [cats, ceil(features / 2)]")
+        _need(1 <= cats <= MOST and 1 <= features <= MOST and codes.shape[1] == (features + 1) // 2, "codes must be [cats, ceil(features / 2)]")
         _need(isinstance(scales, torch.Tensor) and scales.device == codes.device and scales.dtype in (torch.bfloat16, torch.float16),
               "scales must be bfloat16 or float16 on the codes' device")
         _need(tuple(scales.shape) == (cats, -(-features // group)), "scales must be [cats, ceil(features / group)]")

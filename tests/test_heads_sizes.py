@@ -2,8 +2,9 @@
 import ctypes as C
 
 import pytest
+import torch
 
-from lvd_pg_b200 import _lib, build
+from lvd_pg_b200 import _lib, api, build
 
 INVALID = 1
 
@@ -22,3 +23,23 @@ def test_more_variables_than_tiles_are_counted(lib, variables):
     assert b"variables" in lib.pcb_last_error()
     assert lib.pcb_soft_evidence_backward(b, 0, 1, variables, 1, 0, 0, None, 0, 0, 1.0, b, b, b, None) == INVALID
     assert b"variables" in lib.pcb_last_error()
+
+
+class _OnDevice(torch.Tensor):   # passes for a CUDA tensor where arguments are looked at
+    is_cuda = property(lambda self: True)
+
+
+def _wide(*shape, dtype=torch.float32):
+    return torch.zeros((1,) * len(shape), dtype=dtype).expand(shape).as_subclass(_OnDevice)
+
+
+def test_sizes_that_32_bits_do_not_hold():
+    """The library is told of them in 32 bits, where 2^32 + 5 would be 5."""
+    for wide in ((1 << 32) + 5, 1 << 31):
+        for call in (lambda: api.token_logprobs(_wide(2, wide)), lambda: api.soft_evidence(_wide(1, 1, wide)),
+                     lambda: api.soft_evidence(_wide(1, wide, 2)), lambda: api.QuantHead(_wide(wide, 32)), lambda: api.QuantHead(_wide(1, wide)),
+                     lambda: api.QuantHead.from_codes(_wide(wide, 16, dtype=torch.uint8), _wide(wide, 1, dtype=torch.float16), 32),
+                     lambda: api.QuantHead.from_codes(_wide(1, (wide + 1) // 2, dtype=torch.uint8), _wide(1, -(-wide // 64), dtype=torch.float16), wide)):
+            with pytest.raises(_lib.PcbError) as e:
+                call()
+            assert e.value.code == INVALID
