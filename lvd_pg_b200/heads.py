@@ -18,6 +18,7 @@ import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -49,6 +50,12 @@ def _call(dev: torch.device, fn, *args) -> None:
         _lib.check(code)
 
 
+def _no_tangent(x: torch.Tensor) -> None:
+    """These operators are differentiated backwards; a tangent of forward mode would be lost without a word."""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:   # (the level first: a microsecond less)
+        _need(False, "no forward-mode derivatives: the argument carries a tangent")
+
+
 def _logits(x: torch.Tensor) -> int:
     if not (isinstance(x, torch.Tensor) and x.is_cuda):
         _need(False, "logits must be a CUDA tensor; there is no CPU fallback")
@@ -59,6 +66,7 @@ def _logits(x: torch.Tensor) -> int:
         _need(False, "logits need at least one category")
     if x.shape[-1] > MOST:
         _need(False, "logits have at most 2^31 - 1 categories")
+    _no_tangent(x)
     return dtype
 
 
@@ -118,7 +126,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     """Scores of `logits` [..., cats] (float32, bfloat16 or float16; any strides), with logp = log_softmax(logits / temperature):
     the log-probability of `tokens` [...] (int32 or int64), the entropy, and the `top_k` <= 32 best alternatives with their
     log-probabilities, of equal logits the lowest index first.  Everything is float32 and differentiable with respect to
-    the logits (not twice).
+    the logits (not twice, and backwards only: a tangent of forward mode is refused).
 
     A negative token means that none is given: its log-probability is 0, its gradient nothing.  One past the last category
     gives NaN.  A row of -inf throughout has log-probabilities -inf, entropy 0 and gradient 0; a row with NaN or +inf is NaN."""
@@ -186,7 +194,7 @@ def soft_evidence(logits: torch.Tensor, miss: Optional[torch.Tensor] = None, tem
     log-weights log_softmax(logits / temperature) [rows, vars, cats] with the row index fastest, as `forward_ex(soft=...)`,
     `em_step_ex` and `mini_batch_em_soft` take them (regularization/reg_likelihood.jl:51-91).  A variable that is missing in
     a row (`miss` [rows, vars], bool or uint8) weighs all its categories alike: 0.  Differentiable with respect to the logits
-    (not twice); where missing, or where all logits are -inf (evidence -inf throughout), the gradient is 0."""
+    (not twice, and not in forward mode); where missing, or where all logits are -inf (evidence -inf throughout), the gradient is 0."""
     dtype = _logits(logits)
     _need(logits.dim() == 3, "logits must be [rows, vars, cats]")
     _need(logits.shape[1] <= MOST, "soft evidence has at most 2^31 - 1 variables")
@@ -207,7 +215,7 @@ class QuantHead:
     scales[n, k // group] * (code - 8), codes 0..15, 16-bit scales.  `QuantHead(weight)` quantises (scale = max |w| / 7 of the
     group); `QuantHead.from_codes` takes codes and scales that another program made.  The weights are laid out once, on
     construction, on the weight's device; calls keep nothing.  A captured graph holds their address: keep the head while it
-    lives.  For inference: features that require a gradient are refused."""
+    lives.  For inference: features that require a gradient or carry a tangent are refused."""
 
     def __init__(self, weight: torch.Tensor, group: int = 64, bias: Optional[torch.Tensor] = None):
         _need(isinstance(weight, torch.Tensor) and weight.is_cuda and weight.dim() == 2 and weight.dtype in _DTYPES,
@@ -279,6 +287,7 @@ class QuantHead:
         if x.dim() < 1 or x.shape[-1] != self.features:
             _need(False, f"features must end in {self.features} values")
         _need(not (x.requires_grad and torch.is_grad_enabled()), "a head in 4 bits gives no gradient: detach the features")
+        _no_tangent(x)
         out_dtype = out_dtype or x.dtype
         _need(out_dtype in _DTYPES, "logits are float32, bfloat16 or float16")
         x2 = x if x.dim() == 2 else x.reshape(-1, self.features)

@@ -58,3 +58,24 @@ def test_statistics_are_of_the_softmax_itself(dtype, cats, rows, temperature):
                                                 None, 0, 0, temperature, out.data_ptr(), stats.data_ptr(), stream))
         assert torch.equal(stats[:, 0], x.float().amax(1))
         assert_within(stats[:, 1], want, tol, "evidence")
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent would be lost without a word: these operators run backwards only."""
+    import torch.autograd.forward_ad as forward_ad
+
+    x = torch.randn(3, 4, 64, device="cuda")
+    head = api.QuantHead(torch.randn(20, 64, device="cuda"))
+    calls = (lambda t: api.token_logprobs(t), lambda t: api.token_logprobs(t[0], top_k=2), lambda t: api.soft_evidence(t), head.logits,
+             head.logprobs, head.evidence)
+    with forward_ad.dual_level():
+        for requires_grad in (False, True):
+            primal = x.clone().requires_grad_(requires_grad)
+            dual = forward_ad.make_dual(primal, torch.randn_like(x))
+            for call in calls:
+                with pytest.raises((_lib.PcbError, RuntimeError), match="tangent|gradient"):
+                    call(dual)
+                with torch.no_grad(), pytest.raises(_lib.PcbError, match="tangent"):
+                    call(dual)
+        for call in calls:   # without a tangent: as ever
+            call(x)

@@ -1,4 +1,4 @@
-"""Sizes that the categorical-head operators refuse before anything is launched: no GPU is needed."""
+"""Sizes and derivatives that the categorical-head operators refuse before anything is launched: no GPU is needed."""
 import ctypes as C
 
 import pytest
@@ -43,3 +43,17 @@ def test_sizes_that_32_bits_do_not_hold():
             with pytest.raises(_lib.PcbError) as e:
                 call()
             assert e.value.code == INVALID
+
+
+def test_tangents_of_forward_mode():
+    import torch.autograd.forward_ad as forward_ad
+
+    from lvd_pg_b200 import heads
+
+    x = torch.zeros(2, 3, 4)
+    heads._no_tangent(x)
+    with forward_ad.dual_level():
+        heads._no_tangent(x)
+        with pytest.raises(_lib.PcbError, match="tangent") as e:
+            heads._no_tangent(forward_ad.make_dual(x, x))
+        assert e.value.code == INVALID
