@@ -54,7 +54,8 @@ __device__ __forceinline__ float scale_f32(uint32_t bits16, int32_t dtype) {
   return dtype == PCB_BF16 ? __uint_as_float(bits16 << 16) : __half2float(__ushort_as_half((unsigned short)bits16));
 }
 
-// One warp per (category, group): scale = max |w| / 7, code = round(w / scale) + 8 with the scale as stored.
+// One warp per (category, group): scale = max |w| / 7, code = round(w / scale) + 8 with the scale as stored.  NaN or an infinite
+// weight makes the scale NaN, and with it all weights of the group: no finite weights stand for it.
 __global__ void __launch_bounds__(256) head_quantize_kernel(const void* w, int32_t dtype, uint32_t cats, uint32_t features, uint32_t group,
                                                             int32_t scale_dtype, uint8_t* codes, uint16_t* scales) {
   const uint32_t lane = threadIdx.x & 31, groups = (features + group - 1) / group, bytes = (features + 1) / 2;
@@ -63,9 +64,14 @@ __global__ void __launch_bounds__(256) head_quantize_kernel(const void* w, int32
     const uint64_t n = i / groups;
     const uint32_t k0 = (uint32_t)(i % groups) * group, k1 = min(features, k0 + group);
     float most = 0.0f;
-    for (uint32_t k = k0 + lane; k < k1; k += 32) most = fmaxf(most, fabsf(load_as_f32(w, n * features + k, dtype)));
+    bool odd = false;
+    for (uint32_t k = k0 + lane; k < k1; k += 32) {
+      const float v = fabsf(load_as_f32(w, n * features + k, dtype));
+      odd |= !(v < INFINITY);
+      most = fmaxf(most, v);
+    }
     for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const float want = most / 7.0f;
+    const float want = __any_sync(0xffffffffu, odd) ? NAN : most / 7.0f;
     const uint16_t bits = scale_dtype == PCB_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(want)) : __half_as_ushort(__float2half_rn(want));
     const float scale = scale_f32(bits, scale_dtype);
     if (lane == 0) scales[i] = bits;

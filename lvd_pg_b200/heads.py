@@ -213,7 +213,7 @@ def soft_evidence(logits: torch.Tensor, miss: Optional[torch.Tensor] = None, tem
 class QuantHead:
     """A categorical head y = x W^T + bias for serving, its weights W [cats, features] in 4 bits: W[n, k] =
     scales[n, k // group] * (code - 8), codes 0..15, 16-bit scales.  `QuantHead(weight)` quantises (scale = max |w| / 7 of the
-    group); `QuantHead.from_codes` takes codes and scales that another program made.  The weights are laid out once, on
+    group, which NaN or an infinite weight makes NaN throughout); `QuantHead.from_codes` takes codes and scales that another program made.  The weights are laid out once, on
     construction, on the weight's device; calls keep nothing.  A captured graph holds their address: keep the head while it
     lives.  For inference: features that require a gradient or carry a tangent are refused."""
 

@@ -79,3 +79,32 @@ def test_forward_mode_derivatives_are_refused():
                     call(dual)
         for call in calls:   # without a tangent: as ever
             call(x)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weights_that_are_no_numbers_stay_so(dtype):
+    """NaN or an infinite weight makes its group NaN, and nothing beside it."""
+    cats, features, group = 20, 150, 32
+    w = torch.randn(cats, features, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    clean = api.QuantHead(w, group).weight()
+    bad = torch.zeros(cats, features, dtype=torch.bool, device="cuda")
+    for n, k, value in ((0, 0, math.nan), (3, 40, math.inf), (4, 149, -math.inf), (19, 95, math.nan)):
+        w[n, k] = value
+        bad[n, k // group * group:(k // group + 1) * group] = True
+    head = api.QuantHead(w, group)
+    got = head.weight()
+    assert torch.equal(torch.isnan(got), bad) and torch.equal(got[~bad], clean[~bad])
+    y = head.logits(torch.ones(2, features, device="cuda"))
+    assert torch.equal(torch.isnan(y), bad.any(1).expand(2, cats))
+
+
+def test_scales_past_the_range_of_their_type():
+    """fp32 weights with fp16 scales, which only the C call combines: from 7 * 65520 on the scale is infinite, the group NaN."""
+    w = torch.ones(3, 64, device="cuda")
+    w[1, 5], w[2, 5] = 7 * 65521.0, 7 * 65503.0
+    codes, scales = torch.empty(3, 32, dtype=torch.uint8, device="cuda"), torch.empty(3, 1, dtype=torch.float16, device="cuda")
+    _lib.check(_lib.lib().pcb_head_quantize(w.data_ptr(), 0, 3, 64, 64, 2, codes.data_ptr(), scales.data_ptr(),
+                                            torch.cuda.current_stream().cuda_stream))
+    head = api.QuantHead.from_codes(codes, scales, 64, 64)
+    nan = torch.isnan(head.weight()).all(1)
+    assert nan.tolist() == [False, True, False] and torch.equal(torch.isnan(head.logits(torch.ones(1, 64, device="cuda")))[0], nan)
