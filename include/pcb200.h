@@ -351,8 +351,8 @@ int32_t pcb_soft_evidence_backward(const void* x_dev, int32_t dtype, uint64_t ro
  * group 32, 64 or 128, scales bf16 or f16, at most 32768 features.  Codes come two a byte, [cats, (features + 1) / 2], the even column in the
  * low half; scales [cats, ceil(features / group)]; both contiguous.
  * pcb_head_quantize makes them of a weight matrix (contiguous, f32 / bf16 / f16): scale = max |w| / 7 rounded to
- * scale_dtype, code = round(w / scale) + 8; a group with NaN, an infinite weight or a scale past the range of scale_dtype is
- * NaN throughout.  pcb_head_pack lays codes and scales out in the order in which
+ * scale_dtype (up, where that is subnormal), code = round(w / scale) + 8; a group with NaN, an infinite weight or a scale
+ * past the range of scale_dtype is NaN throughout.  pcb_head_pack lays codes and scales out in the order in which
  * pcb_head_logits reads them (packed_dev, as many bytes as pcb_head_packed_bytes says, 16-byte aligned); pcb_head_weight writes the
  * weights that a packed head stands for, [cats, features] f32. */
 int32_t pcb_head_packed_bytes(uint32_t cats, uint32_t features, uint32_t group, uint64_t* bytes_out);

@@ -72,7 +72,11 @@ __global__ void __launch_bounds__(256) head_quantize_kernel(const void* w, int32
     }
     for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     const float want = __any_sync(0xffffffffu, odd) ? NAN : most / 7.0f;
-    const uint16_t bits = scale_dtype == PCB_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(want)) : __half_as_ushort(__float2half_rn(want));
+    // To the nearest; a scale that is subnormal in its type, up: half a step is up to half of it there (all of it below the
+    // smallest), and the largest weights would be cut off at 7 of a scale that was rounded down, or all be lost.
+    uint16_t bits;
+    if (scale_dtype == PCB_BF16) bits = __bfloat16_as_ushort(want < 0x1p-126f ? __float2bfloat16_ru(want) : __float2bfloat16_rn(want));
+    else bits = __half_as_ushort(want < 0x1p-14f ? __float2half_ru(want) : __float2half_rn(want));
     const float scale = scale_f32(bits, scale_dtype);
     if (lane == 0) scales[i] = bits;
     for (uint32_t k = k0 + 2 * lane; k < k1; k += 64) {

@@ -108,3 +108,37 @@ def test_scales_past_the_range_of_their_type():
     head = api.QuantHead.from_codes(codes, scales, 64, 64)
     nan = torch.isnan(head.weight()).all(1)
     assert nan.tolist() == [False, True, False] and torch.equal(torch.isnan(head.logits(torch.ones(1, 64, device="cuda")))[0], nan)
+
+
+@pytest.mark.parametrize("largest", [1e-3, 4e-4, 1e-4, 1e-5, 2e-6, 5e-7, 1.2e-7])
+def test_small_weights_of_half_precision(largest):
+    """Where max |w| / 7 is subnormal as an fp16 scale, a step of it is up to all of the scale: rounded up, so that no weight
+    is cut off or lost.  A weight is off by half a scale at most; above that the scale was rounded down by half a step."""
+    cats, features, group = 40, 200, 64
+    gen = torch.Generator().manual_seed(7)
+    w = ((2 * torch.rand(cats, features, generator=gen) - 1) * largest).half().cuda()
+    w[1] = 0
+    got = api.QuantHead(w, group).weight().double()
+    step = 2.0 ** -24   # of subnormal numbers
+    pad = torch.zeros(cats, 4 * group, dtype=torch.float64, device="cuda")
+    pad[:, :features] = w.double()
+    most = pad.view(cats, 4, group).abs().amax(2)
+    scale = (most / 7).repeat_interleave(group, 1)[:, :features]
+    small = scale < 2.0 ** -14
+    each = torch.where(small, (scale / step).ceil() * step, scale * (1 + 2.0 ** -11))
+    tol = torch.where(small, 0.5 * each, (0.5 + 7 * 2.0 ** -11) * each) * (1 + 1e-5)
+    assert ((got - w.double()).abs() <= tol).all()
+    assert (got[1] == 0).all() and (got[0] != 0).any()
+
+
+def test_smallest_weights_under_bfloat16_scales():
+    """fp32 weights around 1e-38: the scale is subnormal, the weights are kept to half of it."""
+    w = ((2 * torch.rand(6, 64, generator=torch.Generator().manual_seed(3)) - 1) * torch.tensor([1e-37, 5e-38, 1e-38, 3e-39, 4e-40, 2e-41])[:, None]).cuda()
+    got = api.QuantHead(w, 64).weight().double()
+    step = 2.0 ** -133   # of subnormal bf16
+    scale = w.double().abs().amax(1, keepdim=True) / 7
+    small = scale < 2.0 ** -126
+    each = torch.where(small, (scale / step).ceil() * step, scale * (1 + 2.0 ** -8))
+    # quotient of fp32 and rounding of max / 7 to fp32: a step of its subnormal numbers each
+    tol = torch.where(small, 0.5 * each, (0.5 + 7 * 2.0 ** -8) * each) * (1 + 1e-5) + 8 * 2.0 ** -149
+    assert small.sum() >= 4 and ((got - w.double()).abs() <= tol).all()
