@@ -363,7 +363,9 @@ int32_t pcb_head_pack(const uint8_t* codes_dev, const void* scales_dev, uint32_t
 int32_t pcb_head_weight(const void* packed_dev, int32_t scale_dtype, uint32_t cats, uint32_t features, uint32_t group,
                         float* weight_dev, pcb_stream s);
 /* y_dev [rows, cats] contiguous in y_dtype = x_dev [rows, features] (dtype, rows at x_row_stride) times the weights,
- * plus bias_dev [cats] (f32, may be NULL).  Codes and features are multiplied exactly, summed in f32. */
+ * plus bias_dev [cats] (f32, may be NULL).  Codes and features are multiplied exactly, summed in f32.  A group's sum of
+ * (code - 8) x is formed before its scale is applied and has to stay in the range of f32 itself, as it does with features up
+ * to 3.3e35 whatever the codes are; past it a logit is infinite or NaN where the scale would have brought it back. */
 int32_t pcb_head_logits(const void* packed_dev, int32_t scale_dtype, uint32_t cats, uint32_t features, uint32_t group,
                         const void* x_dev, int32_t dtype, uint64_t rows, uint64_t x_row_stride, const float* bias_dev,
                         void* y_dev, int32_t y_dtype, pcb_stream s);

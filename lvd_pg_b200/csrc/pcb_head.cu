@@ -3,7 +3,7 @@
 //
 // The weights are the A operand of mma.sync m16n8k16: 16 categories x 16 features, codes turned into integers -8..7 in the
 // features' own type, where they and their products with x are exact; a group's sum stays in the fp32 accumulator and meets
-// its scale there, once.  (fp32 features go in as three bf16 terms, which hold all 24 bits.)
+// its scale there, once: features up to 3.3e35 in magnitude keep it in range (128 of them, times 8).  (fp32 features go in as three bf16 terms, which hold all 24 bits.)
 //
 // Packed order: tiles of 16 categories, in each blocks of 64 features of 512 bytes, a 16-byte word per lane.  Lane 4 g + t
 // holds the codes of categories g and g + 8; its 32-bit word w belongs to the k16 step j = w & 1 of the 32 features
@@ -166,8 +166,10 @@ struct HeadArgs {
 };
 
 // Two 16-bit values of the tensor cores' operand type.  A nibble in the mantissa of BASE is BASE + code 2^offset, exactly;
-// one multiply-add takes it to code - 8.  bf16 has room for the lowest place only (three shifts per word of eight codes),
-// fp16 for two (one shift).
+// one multiply-add takes it to code - 8: the known way from integers to floating point through the mantissa of a power of two,
+// which Kim, Henry, Fahim and Awadalla describe for weights of 4 bits ("Who Says Elephants Can't Run: Bringing Large Scale
+// MoE Models into Cloud Scale Production", 2022).  bf16 has room for the lowest place only (three shifts per word of eight
+// codes), fp16 for two (one shift).
 __device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t base) {   // one instruction
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(base));

@@ -280,7 +280,7 @@ class QuantHead:
 
     def logits(self, x: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """x [..., features] (float32, bfloat16 or float16) -> [..., cats] in `out_dtype` (default: x's type).  Sums are
-        float32.  Meant for few rows: up to 32 of them (10 of float32; fewer beyond about 2400 features, 21 and 7 at 4096)
+        float32, a group's before its scale: features up to 3.3e35 in magnitude keep them in range.  Meant for few rows: up to 32 of them (10 of float32; fewer beyond about 2400 features, 21 and 7 at 4096)
         read the weights once."""
         _need(isinstance(x, torch.Tensor) and x.device == self.device and x.dtype in _DTYPES,
               "features must be float32, bfloat16 or float16 on the head's device")

@@ -142,3 +142,20 @@ def test_smallest_weights_under_bfloat16_scales():
     # quotient of fp32 and rounding of max / 7 to fp32: a step of its subnormal numbers each
     tol = torch.where(small, 0.5 * each, (0.5 + 7 * 2.0 ** -8) * each) * (1 + 1e-5) + 8 * 2.0 ** -149
     assert small.sum() >= 4 and ((got - w.double()).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+def test_features_up_to_where_a_groups_sum_ends(dtype):
+    """Groups of 128 whose every product is -8 times 3.3e35, the documented end, or of alternating sign: finite sums in any
+    order, exact up to the bound of 128 additions, scaled back into range."""
+    codes = torch.zeros(20, 192, dtype=torch.uint8, device="cuda")   # code 0: -8
+    scales = torch.full((20, 3), 2.0 ** -20, dtype=torch.bfloat16, device="cuda")
+    head = api.QuantHead.from_codes(codes, scales, 384, 128)
+    x = torch.full((3, 384), 3.3e35)
+    x[1, ::2] *= -1
+    x[2, 128:] = 0
+    x = x.to(dtype).cuda()   # bf16: 3.2976e35
+    got = head.logits(x, torch.float32)
+    want = (-8.0 * x.double().sum(1) * 2.0 ** -20)[:, None].expand(3, 20)
+    spread = 8.0 * x.double().abs().sum(1)[:, None] * 2.0 ** -20
+    assert torch.isfinite(got).all() and ((got.double() - want).abs() <= 17 * 24 * 2.0 ** -23 * spread).all()
