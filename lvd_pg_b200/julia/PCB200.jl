@@ -481,8 +481,14 @@ end
 
 # ---- categorical heads: what a network's logits are scored with, and made into soft evidence ---------------
 logits_type(::Type{Float32}) = Int32(0)
-logits_type(::Type{Core.BFloat16}) = Int32(1)
 logits_type(::Type{Float16}) = Int32(2)
+# bfloat16 is a type of Julia's from 1.11 on; before that heads of Float32 weights have Float16 scales
+@static if isdefined(Core, :BFloat16)
+    logits_type(::Type{Core.BFloat16}) = Int32(1)
+    const WideScale = Core.BFloat16
+else
+    const WideScale = Float16
+end
 ptr_or_null(x) = x === nothing ? CU_NULL : reinterpret(CuPtr{Cvoid}, pointer(x))
 
 """
@@ -545,7 +551,7 @@ struct QuantHead
     bias::Union{Nothing,CuVector{Float32}}
     cats::Int; features::Int; group::Int; scale_type::Int32
 end
-"codes (ceil(features / 2), cats) UInt8, two a byte; scales (ceil(features / group), cats) Float16 or BFloat16"
+"codes (ceil(features / 2), cats) UInt8, two a byte; scales (ceil(features / group), cats) Float16, or BFloat16 where Julia has it"
 function QuantHead(codes::CuMatrix{UInt8}, scales::CuMatrix, features::Integer; group = 64, bias = nothing)
     cats = size(codes, 2)
     bytes = Ref{UInt64}(0)
@@ -557,7 +563,7 @@ function QuantHead(codes::CuMatrix{UInt8}, scales::CuMatrix, features::Integer; 
 end
 function QuantHead(weight::CuMatrix{T}; group = 64, bias = nothing) where {T}
     K, N = size(weight)
-    S = T == Float16 ? Float16 : Core.BFloat16
+    S = T == Float16 ? Float16 : WideScale
     codes = CuMatrix{UInt8}(undef, cld(K, 2), N); scales = CuMatrix{S}(undef, cld(K, group), N)
     check(ccall((:pcb_head_quantize, libpcb200), Int32,
                 (CuPtr{Cvoid}, Int32, UInt32, UInt32, UInt32, Int32, CuPtr{UInt8}, CuPtr{Cvoid}, Ptr{Cvoid}),
