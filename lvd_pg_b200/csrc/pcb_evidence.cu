@@ -24,7 +24,7 @@ struct EvidenceArgs {
 // for fp32 logits, where four neighbouring granules would share a bank, one more per row of a warp after every 32 columns
 // (37 x 192 x 500: 16.0 -> 15.0 us; 16-bit logits, two to a bank, lose more by the arithmetic than the conflicts cost:
 // 512 x 784 x 256 bf16 119 -> 125).  512 x 784 x 256 bf16 takes 104 us (5.9 TB/s, 92 % of a copy), 37 x 192 x 500 fp32 12.2 us: a
-// few tiles per SM, latency; forward and gradient of 500 x 192 x 256 fp16 83 us (4.1 TB/s with the logits read twice): what
+// few tiles per SM, latency; forward and gradient of 500 x 192 x 256 fp16 81 us (4.2 TB/s with the logits read twice): what
 // bounds the gradient is the way of g and of dx through shared memory between two barriers.  A distribution of more than `cap` categories passes twice, in chunks: once for its
 // sum, once for its values.
 constexpr uint32_t EV_THREADS = 256, EV_WARPS = 8, EV_COLUMNS = 256, EV_PITCH = 33;

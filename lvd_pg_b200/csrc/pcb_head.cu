@@ -253,11 +253,12 @@ __device__ __forceinline__ void store_y(void* y, uint64_t i, float v, int32_t dt
 // columns of the B operand (fp32: three columns each, one per term, joined at the end); codes and scales go straight from
 // memory to registers, four 16-byte loads per lane ahead of the four that are worked on, across the boundaries of rounds.
 //
-// Bound by what turns codes into operands, not by the products: one vector at 131072 x 4096 bf16 takes 62.8 us for 285 MB
+// Bound by what turns codes into operands, not by the products: one vector at 131072 x 4096 bf16 takes 62.6 us for 285 MB
 // (4.5 TB/s, 70 % of what a copy reaches) with the pipe of shifts and masks 60 % busy, three shifts, four masks and four
 // subtractions per eight codes.  Wide multiplies in place of shifts (76 -> 88 us then), a step loop unrolled by two (64 -> 65)
 // and prefetching the next round into the L2 cache (64 -> 78) did not pay.  fp16 needs one shift: 32000 x 2048, sixteen
-// vectors, 15.3 us (2.3 TB/s: launch, feature vectors and the last round weigh there).
+// vectors, 15.2 us (2.3 TB/s: launch, feature vectors and the last round weigh there).  More vectors than a pass takes unpack
+// the weights again for every 32 of them: 1024 at 32000 x 2048 bf16 0.80 ms, 401408 at 256 x 512 bf16 4.0 ms (fp32 13.6).
 constexpr uint32_t HEAD_THREADS = 512, HEAD_WARPS = 16;
 
 template <bool G32>

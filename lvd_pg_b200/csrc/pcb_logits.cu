@@ -34,7 +34,8 @@ __device__ __forceinline__ float token_logp(const LogprobArgs& a, int64_t token,
 //
 // Bound by memory and by the end of each row, where a block reads what it noted: 2048 rows of 131072 bf16 with 8 alternatives
 // 105 us (5.1 TB/s, 79 % of a copy; 96 us without alternatives); a single row of 131072 fp32 with 20 alternatives, on a cluster
-// of eight blocks, 9.4 us, all of it latency (launch, one pass of sixteen tiles, selection, two cluster barriers).
+// of eight blocks, 9.0 us, all of it latency: 2.6 for the shortest row there is, 4.7 for this one without alternatives, 7.0 with
+// one, the rest for ordering twenty.
 constexpr uint32_t SLOTS = 16, CAND = 256, PAIRS = 256, MAX_CLUSTER = 8;
 
 template <typename T> struct Tile { static constexpr uint32_t U = sizeof(T) == 4 ? 8 : 4; };   // granules per thread

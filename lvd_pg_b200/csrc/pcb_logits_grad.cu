@@ -91,9 +91,10 @@ __device__ __forceinline__ void grad_words(const uint32_t* w, const RowGrad& g, 
 
 // A block takes GRAD_TILE bytes of a row: 64 per thread.  Granules are those of dx; x is read in them where it lies alike
 // towards 16-byte boundaries, by elements otherwise.  Small blocks: they wait for one another's stores before what is pointed to
-// is written (us both directions, 256 / 128 / 64 threads: 1021 rows of 50021 bf16 73.0 / 71.3 / 72.6, 20000 of 2000 125 / 87 / 74).
-// The last rows come first: the forward pass read them last, and some of them are still in the L2 cache.  Bound by memory: the
-// logits twice and the gradient once move at 4.3 TB/s in both directions together (two thirds of a copy; 102 MB of logits).
+// is written (us both directions, 256 / 128 / 64 threads: 1021 rows of 50021 bf16 75.3 / 73.2 / 73.6, 20000 of 2000 130 / 92 / 76).
+// The last rows come first: the forward pass read them last, and some of them are still in the L2 cache.  The logits twice and
+// the gradient once move at 4.2 TB/s in both directions together (two thirds of a copy; 102 MB of logits).  Bound by
+// instructions as much as by memory: 72 % of the issue slots are taken, since every thread prepares its row.
 constexpr uint32_t GRAD_THREADS = 64, GRAD_TILE = 64 * GRAD_THREADS;
 static_assert(GRAD_THREADS > MAX_TOP, "a thread for the token and for every alternative");
 template <typename T>
