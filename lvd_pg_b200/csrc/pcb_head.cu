@@ -3,7 +3,8 @@
 //
 // The weights are the A operand of mma.sync m16n8k16: 16 categories x 16 features, codes turned into integers -8..7 in the
 // features' own type, where they and their products with x are exact; a group's sum stays in the fp32 accumulator and meets
-// its scale there, once: features up to 3.3e35 in magnitude keep it in range (128 of them, times 8).  (fp32 features go in as three bf16 terms, which hold all 24 bits.)
+// its scale there, once: features up to 3.3e35 in magnitude keep it in range (128 of them, times 8).  (fp32 features go in as
+// three bf16 terms, which hold all 24 bits.)
 //
 // Packed order: tiles of 16 categories, in each blocks of 64 features of 512 bytes, a 16-byte word per lane.  Lane 4 g + t
 // holds the codes of categories g and g + 8; its 32-bit word w belongs to the k16 step j = w & 1 of the 32 features

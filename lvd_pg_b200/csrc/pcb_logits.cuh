@@ -89,7 +89,7 @@ template <typename T> constexpr uint32_t PER_WORD = 4 / sizeof(T);
 
 // Where the powers of a row count from.
 struct Shift {
-  float m, c, mc;   // mc: m c, rounded (an explicit product: fused into a difference of two it would not be the one that powers count from)
+  float m, c, mc;   // mc: m c, rounded: an explicit product, since fused into a difference it is not what powers count from
   bool near;
 };
 template <typename T>

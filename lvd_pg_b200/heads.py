@@ -194,7 +194,8 @@ def soft_evidence(logits: torch.Tensor, miss: Optional[torch.Tensor] = None, tem
     log-weights log_softmax(logits / temperature) [rows, vars, cats] with the row index fastest, as `forward_ex(soft=...)`,
     `em_step_ex` and `mini_batch_em_soft` take them (regularization/reg_likelihood.jl:51-91).  A variable that is missing in
     a row (`miss` [rows, vars], bool or uint8) weighs all its categories alike: 0.  Differentiable with respect to the logits
-    (not twice, and not in forward mode); where missing, or where all logits are -inf (evidence -inf throughout), the gradient is 0."""
+    (not twice, and not in forward mode); where missing, or where all logits are -inf (evidence -inf throughout), the gradient
+    is 0."""
     dtype = _logits(logits)
     _need(logits.dim() == 3, "logits must be [rows, vars, cats]")
     _need(logits.shape[1] <= MOST, "soft evidence has at most 2^31 - 1 variables")
@@ -213,9 +214,10 @@ def soft_evidence(logits: torch.Tensor, miss: Optional[torch.Tensor] = None, tem
 class QuantHead:
     """A categorical head y = x W^T + bias for serving, its weights W [cats, features] in 4 bits: W[n, k] =
     scales[n, k // group] * (code - 8), codes 0..15, 16-bit scales.  `QuantHead(weight)` quantises (scale = max |w| / 7 of the
-    group, which NaN or an infinite weight makes NaN throughout); `QuantHead.from_codes` takes codes and scales that another program made.  The weights are laid out once, on
-    construction, on the weight's device; calls keep nothing.  A captured graph holds their address: keep the head while it
-    lives.  For inference: features that require a gradient or carry a tangent are refused."""
+    group, which NaN or an infinite weight makes NaN throughout); `QuantHead.from_codes` takes codes and scales that another
+    program made.  The weights are laid out once, on construction, on the weight's device; calls keep nothing.  A captured
+    graph holds their address: keep the head while it lives.  For inference: features that require a gradient or carry a
+    tangent are refused."""
 
     def __init__(self, weight: torch.Tensor, group: int = 64, bias: Optional[torch.Tensor] = None):
         _need(isinstance(weight, torch.Tensor) and weight.is_cuda and weight.dim() == 2 and weight.dtype in _DTYPES,
@@ -280,8 +282,8 @@ class QuantHead:
 
     def logits(self, x: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """x [..., features] (float32, bfloat16 or float16) -> [..., cats] in `out_dtype` (default: x's type).  Sums are
-        float32, a group's before its scale: features up to 3.3e35 in magnitude keep them in range.  Meant for few rows: up to 32 of them (10 of float32; fewer beyond about 2400 features, 21 and 7 at 4096)
-        read the weights once."""
+        float32, a group's before its scale: features up to 3.3e35 in magnitude keep them in range.  Meant for few rows: up
+        to 32 of them (10 of float32; fewer beyond about 2400 features, 21 and 7 at 4096) read the weights once."""
         _need(isinstance(x, torch.Tensor) and x.device == self.device and x.dtype in _DTYPES,
               "features must be float32, bfloat16 or float16 on the head's device")
         if x.dim() < 1 or x.shape[-1] != self.features:
