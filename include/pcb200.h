@@ -308,7 +308,7 @@ int32_t pcb_pairwise_mi(const uint8_t* data_dev, uint64_t num_rows, uint32_t num
  * pcb_pairwise_mi these calls run on the current device.  They allocate nothing, do not synchronise, keep no state,
  * and may be captured; calls that share no output may overlap.  The reference trains its teachers in PyTorch
  * (src/models/) and has no counterpart.
- * Logits are f32, bf16 or f16 with the category index fastest; strides are in elements. */
+ * Logits are f32, bf16 or f16 with the category index fastest; strides are in elements, pointers aligned to their elements. */
 enum { PCB_F32 = 0, PCB_BF16 = 1, PCB_F16 = 2 };
 
 /* For every row of x_dev [rows, cats], with s = x / temperature and logp = s - logsumexp(s):

@@ -530,6 +530,8 @@ extern "C" int32_t pcb_head_quantize(const void* weight_dev, int32_t dtype, uint
   if (int32_t rc = check_shape(cats, features, group)) return rc;
   PCB_REQUIRE(weight_dev && codes_dev && scales_dev, "null argument");
   PCB_REQUIRE(is_dtype(dtype) && is_scale_dtype(scale_dtype), "weights are f32, bf16 or f16, scales bf16 or f16");
+  PCB_REQUIRE(((uintptr_t)weight_dev & (dtype == PCB_F32 ? 3 : 1)) == 0 && ((uintptr_t)scales_dev & 1) == 0,
+              "weights or scales that are not aligned to their own size");
   const uint64_t groups = ((uint64_t)features + group - 1) / group;
   head_quantize_kernel<<<blocks_for(cats * groups * 32), 256, 0, (cudaStream_t)s>>>(weight_dev, dtype, cats, features, group, scale_dtype,
                                                                                    codes_dev, static_cast<uint16_t*>(scales_dev));
@@ -541,6 +543,7 @@ extern "C" int32_t pcb_head_pack(const uint8_t* codes_dev, const void* scales_de
                                  void* packed_dev, pcb_stream s) {
   if (int32_t rc = check_shape(cats, features, group)) return rc;
   PCB_REQUIRE(codes_dev && scales_dev && packed_dev && ((uintptr_t)packed_dev & 15) == 0, "null argument, or a packed head that is not 16-byte aligned");
+  PCB_REQUIRE(((uintptr_t)scales_dev & 1) == 0, "scales that are not aligned to their own size");
   const HeadShape h = head_shape(cats, features, group);
   head_pack_kernel<<<h.tiles, 256, 0, (cudaStream_t)s>>>(h, codes_dev, static_cast<const uint16_t*>(scales_dev), static_cast<uint32_t*>(packed_dev));
   PCB_CUDA(cudaGetLastError());
@@ -550,7 +553,7 @@ extern "C" int32_t pcb_head_pack(const uint8_t* codes_dev, const void* scales_de
 extern "C" int32_t pcb_head_weight(const void* packed_dev, int32_t scale_dtype, uint32_t cats, uint32_t features, uint32_t group,
                                    float* weight_dev, pcb_stream s) {
   if (int32_t rc = check_shape(cats, features, group)) return rc;
-  PCB_REQUIRE(packed_dev && weight_dev, "null argument");
+  PCB_REQUIRE(packed_dev && weight_dev && ((uintptr_t)packed_dev & 15) == 0, "null argument, or a packed head that is not 16-byte aligned");
   PCB_REQUIRE(is_scale_dtype(scale_dtype), "scales are bf16 or f16");
   const HeadShape h = head_shape(cats, features, group);
   head_weight_kernel<<<blocks_for(h.code_words()), 256, 0, (cudaStream_t)s>>>(h, static_cast<const uint32_t*>(packed_dev), scale_dtype, weight_dev);

@@ -613,6 +613,7 @@ extern "C" int32_t pcb_token_logprobs(const void* x_dev, int32_t dtype, uint64_t
   if (int32_t rc = check_logits(x_dev, dtype, cats, temperature)) return rc;
   PCB_REQUIRE(entropy_dev && ((uintptr_t)stats_dev & 7) == 0, "null argument, or statistics that are not 8-byte aligned");
   PCB_REQUIRE(!tokens_dev || (logp_out_dev && (token_bytes == 4 || token_bytes == 8)), "tokens are int32 or int64 and need an output");
+  PCB_REQUIRE(!tokens_dev || (uintptr_t)tokens_dev % token_bytes == 0, "tokens that are not aligned to their own size");
   PCB_REQUIRE(top_k <= MAX_TOP && top_k <= cats, "at most 32 alternatives, and no more than there are categories");
   PCB_REQUIRE(top_k == 0 || (top_ids_dev && top_logp_dev), "alternatives need their outputs");
   LogprobArgs a{x_dev, rows, row_stride, cats, top_k, token_bytes, 1.0f / temperature, LOG2E / temperature, tokens_dev,

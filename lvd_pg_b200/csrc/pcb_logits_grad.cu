@@ -359,6 +359,7 @@ extern "C" int32_t pcb_token_logprobs_backward(const void* x_dev, int32_t dtype,
   PCB_REQUIRE(stats_dev && entropy_dev && dx_dev, "null argument");
   PCB_REQUIRE(((uintptr_t)dx_dev & (dtype == PCB_F32 ? 3 : 1)) == 0, "a gradient that is not aligned to its own size");
   PCB_REQUIRE(!g_logp_dev || (tokens_dev && (token_bytes == 4 || token_bytes == 8)), "a gradient of logp needs the tokens, int32 or int64");
+  PCB_REQUIRE(!g_logp_dev || (uintptr_t)tokens_dev % token_bytes == 0, "tokens that are not aligned to their own size");
   PCB_REQUIRE(top_k <= MAX_TOP && top_k <= cats, "at most 32 alternatives, and no more than there are categories");
   PCB_REQUIRE(!g_top_dev || (top_k > 0 && top_ids_dev), "a gradient of the alternatives needs their indices");
   LogprobGradArgs a{x_dev, rows, row_stride, g_logp_stride, g_entropy_stride, cats, top_k, token_bytes, 1.0f / temperature,

@@ -1,4 +1,4 @@
-"""Sizes and derivatives that the categorical-head operators refuse before anything is launched: no GPU is needed."""
+"""Sizes, alignments and derivatives that the categorical-head operators refuse before anything is launched: no GPU is needed."""
 import ctypes as C
 
 import pytest
@@ -57,3 +57,17 @@ def test_tangents_of_forward_mode():
         with pytest.raises(_lib.PcbError, match="tangent") as e:
             heads._no_tangent(forward_ad.make_dual(x, x))
         assert e.value.code == INVALID
+
+
+def test_pointers_off_their_types_alignment(lib):
+    """Arguments that come without a type: tokens, scales, weights to quantise, a packed head."""
+    b = C.create_string_buffer(512)
+    at = (C.addressof(b) + 15) // 16 * 16
+    for token_bytes, off in ((8, 4), (8, 1), (4, 2)):
+        assert lib.pcb_token_logprobs(at, 0, 1, 5, 5, 1.0, at + off, token_bytes, 0, at, at, None, None, None, None) == INVALID
+        assert lib.pcb_token_logprobs_backward(at, 0, 1, 5, 5, 1.0, at + off, token_bytes, 0, None, at, at, at, 1, None, 0, None, at, None) == INVALID
+    for dtype, off in ((0, 2), (1, 1), (2, 1)):
+        assert lib.pcb_head_quantize(at + off, dtype, 1, 32, 32, 1, at, at, None) == INVALID
+    assert lib.pcb_head_quantize(at, 0, 1, 32, 32, 1, at, at + 1, None) == INVALID
+    assert lib.pcb_head_pack(at, at + 1, 1, 32, 32, at, None) == INVALID
+    assert lib.pcb_head_weight(at + 8, 1, 1, 32, 32, at, None) == INVALID
